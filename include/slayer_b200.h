@@ -404,6 +404,45 @@ int sb_cuba_recurrent_bwd(const float* grad_spike, const float* voltage, const f
                           int64_t batch, int64_t neurons, int64_t T, float threshold, float tau_rho,
                           float scale_rho, int graded, void* stream);
 
+/* ---- linear attention with a decay for each head (no counterpart in the reference) ---------------
+ * S[t] = r S[t-1] + k[t] v[t]^T,  o[t] = S[t]^T q[t],  r = 1 - decay / 4096.
+ * q, k: [heads, Dk, T]; v, out: [heads, Dv, T]; states: [heads, Dk, Dv]; heads = samples * H, decay
+ * float[n_decay] with n_decay 1 or H (head i uses decay[i % H]); 1 <= Dk, Dv <= 128.
+ * state (nullable: zero) is S before the first step, final_state (nullable) receives S after the last.
+ * `scratch` has sb_linear_attention_scratch_bytes(..., backward) bytes (0: may be null). */
+int64_t sb_linear_attention_scratch_bytes(int64_t heads, int64_t Dk, int64_t Dv, int64_t T, int backward);
+int sb_linear_attention_fwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                            const float* state, float* out, float* final_state, int64_t heads, int64_t H,
+                            int64_t Dk, int64_t Dv, int64_t T, void* scratch, void* stream);
+/* Gradients for grad_out and grad_final (nullable: zero); grad_state (nullable) is that of `state`. */
+int sb_linear_attention_bwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                            const float* state, const float* grad_out, const float* grad_final, float* grad_q,
+                            float* grad_k, float* grad_v, float* grad_state, int64_t heads, int64_t H, int64_t Dk,
+                            int64_t Dv, int64_t T, void* scratch, void* stream);
+/* One step: q, k [heads, Dk], v, out [heads, Dv]; state [heads, Dk, Dv] is updated in place. */
+int sb_linear_attention_step(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                             float* state, float* out, int64_t heads, int64_t H, int64_t Dk, int64_t Dv,
+                             void* stream);
+
+/* ---- dense synapse in 8-bit integers (no counterpart in the reference) ----------------------------
+ * y[n, o, t] = (sum_k w[o, k] xq[n, k, t]) * w_scale[o] * 2^p[n, t],  xq = round(x / 2^p) half to even,
+ * p the smallest integer >= -126 with 127 * 2^p >= max_k |x[n, k, t]|.
+ * x: [N, K, T] fp32, y: [N, O, T] fp32, w: [O, Kp] int8 rows padded with zeros to Kp = K rounded up to
+ * 16, 16-byte aligned; 1 <= K <= 131072.  `scratch` has sb_qdense_scratch_bytes(N * T, Kp) bytes. */
+int64_t sb_qdense_scratch_bytes(int64_t tokens, int64_t Kp);
+int sb_qdense_fwd(const float* x, const signed char* w, const float* w_scale, float* y, int64_t N, int64_t K,
+                  int64_t Kp, int64_t O, int64_t T, void* scratch, void* stream);
+
+/* ---- dropout from a counter-based generator --------------------------------------------------------
+ * (src/lava/lib/dl/slayer/neuron/dropout.py drops whole neurons through torch's dropout3d.)
+ * y[i] = x[i] / (1 - p) where word i' % 4 of Philox4x32-10(counter (i' / 4, offset), key seed) is at
+ * least floor(p * 2^32), else 0; i' = i with per_step, i / T (the row) without.  key: device
+ * int64[2] = {seed, offset}.  The same call on the output gradient is the backward pass. */
+int sb_dropout(const float* x, float* y, const int64_t* key, int64_t rows, int64_t T, double p, int per_step,
+               void* stream);
+/* key = state; state[1] += 1 (both device int64[2]): the next call's key, also when replayed in a graph. */
+int sb_dropout_next(int64_t* state, int64_t* key, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,249 @@
+// Linear attention with a decay for each head: the leaky integrator whose input is an outer product.
+//
+//   S[t] = r S[t-1] + k[t] v[t]^T        (Dk x Dv, r = 1 - decay / 4096)
+//   o[t] = S[t]^T q[t]
+//
+// q, k: [heads, Dk, T], v, o: [heads, Dv, T], time contiguous like every tensor of this library.
+// With G[t] = r G[t+1] + q[t] go[t]^T the gradients are
+//
+//   gq[t] = S[t] go[t]      gk[t] = G[t] v[t]      gv[t] = G[t]^T k[t]      gS[-1] = r G[0],
+//
+// i.e. the same operator three more times: gq is the walk with (q, k, v) <- (go, v, k) on the
+// transposed state, gk and gv are walks back in time with (v, go, q) and (k, q, go).  A walk back in
+// time hands its state on already decayed (the first step must see G[T-1] = gS[T-1] + q go^T).
+// So every kernel here takes a direction and an `after` flag and serves all four walks.
+#include "linear_attention.cuh"
+
+using namespace sb;
+using namespace sb::la;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Walk step by step: any size, any length.
+// A block of 128 threads owns one head and 64 columns of its state; a thread holds NI x 4 elements of
+// it (rows dg + 8 i, four neighbouring columns).  The row sums of a tile of steps are joined through
+// shared memory at the end of the tile.
+// r is applied as the sum of two floats: over the thousand steps a slow head remembers, half an ulp of
+// r would grow a thousandfold.  decay / 4096 is exact, and so is what 1 - decay / 4096 loses to rounding.
+// ---------------------------------------------------------------------------
+constexpr int kTile = 8;
+
+template <int NI>
+__global__ void __launch_bounds__(128) walk_kernel(Walk w) {
+  __shared__ float qs[kTile][8 * NI], ks[kTile][8 * NI], vs[kTile][64];
+  __shared__ float part[kTile][8][64];
+  const int tid = threadIdx.x, ec = (tid & 15) * 4, dg = tid >> 4;
+  const int64_t head = blockIdx.x;
+  const int e0 = blockIdx.y * 64;
+  const int ne = min(64, w.Dv - e0);
+  const float delta = w.decay[w.n_decay > 1 ? head % w.n_decay : 0] * (1.0f / 4096.0f);
+  const float r = __fsub_rn(1.0f, delta), r_lo = __fsub_rn(__fsub_rn(1.0f, r), delta);
+  const float* q = w.q + head * w.Dk * w.T;
+  const float* k = w.k + head * w.Dk * w.T;
+  const float* v = w.v + (head * w.Dv + e0) * w.T;
+  float* o = w.o + (head * w.Dv + e0) * w.T;
+
+  float S[NI][4];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = dg + 8 * i;
+      S[i][e] = (w.s_in && d < w.Dk && ec + e < ne)
+                    ? w.s_in[head * w.Dk * w.Dv + (int64_t)d * w.s_row + (int64_t)(e0 + ec + e) * w.s_col]
+                    : 0.f;
+    }
+
+  for (int64_t t0 = 0; t0 < w.T; t0 += kTile) {
+    const int nt = (int)min((int64_t)kTile, w.T - t0);
+    __syncthreads();
+    for (int i = tid; i < kTile * 8 * NI; i += 128) {
+      const int d = i / kTile, s = i % kTile;
+      const int64_t t = w.reverse ? w.T - 1 - (t0 + s) : t0 + s;
+      const bool in = d < w.Dk && s < nt;
+      qs[s][d] = in ? q[d * w.T + t] : 0.f;
+      ks[s][d] = in ? k[d * w.T + t] : 0.f;
+    }
+    for (int i = tid; i < kTile * 64; i += 128) {
+      const int e = i / kTile, s = i % kTile;
+      const int64_t t = w.reverse ? w.T - 1 - (t0 + s) : t0 + s;
+      vs[s][e] = (e < ne && s < nt) ? v[e * w.T + t] : 0.f;
+    }
+    __syncthreads();
+    for (int s = 0; s < nt; ++s) {
+      const float4 vv = *reinterpret_cast<const float4*>(&vs[s][ec]);
+      const float ve[4] = {vv.x, vv.y, vv.z, vv.w};
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const float kd = ks[s][dg + 8 * i], qd = qs[s][dg + 8 * i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = S[i][e];
+          if (w.after) {
+            x = fmaf(r, x, fmaf(r_lo, x, kd * ve[e]));
+            acc[e] = fmaf(qd, x, acc[e]);
+          } else {
+            x = fmaf(kd, ve[e], x);
+            acc[e] = fmaf(qd, x, acc[e]);
+            x = fmaf(r, x, r_lo * x);
+          }
+          S[i][e] = x;
+        }
+      }
+      *reinterpret_cast<float4*>(&part[s][dg][ec]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    }
+    __syncthreads();
+    for (int i = tid; i < kTile * 64; i += 128) {
+      const int e = i / kTile, s = i % kTile;
+      if (e >= ne || s >= nt) continue;
+      float sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) sum += part[s][g][e];
+      const int64_t t = w.reverse ? w.T - 1 - (t0 + s) : t0 + s;
+      o[e * w.T + t] = sum;
+    }
+  }
+  if (w.s_out) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = dg + 8 * i;
+        if (d < w.Dk && ec + e < ne)
+          w.s_out[head * w.Dk * w.Dv + (int64_t)d * w.s_row + (int64_t)(e0 + ec + e) * w.s_col] = S[i][e];
+      }
+  }
+}
+
+int launch_walk(const Walk& w, cudaStream_t s) {
+  const dim3 grid((unsigned)w.heads, (unsigned)((w.Dv + 63) / 64));
+  if (w.Dk <= 64) walk_kernel<8><<<grid, 128, 0, s>>>(w);
+  else walk_kernel<16><<<grid, 128, 0, s>>>(w);
+  SB_CUDA(cudaGetLastError());
+  return SB_OK;
+}
+
+// ---------------------------------------------------------------------------
+// One step on a kept state: reads and writes the state once, Dk x Dv floats each way.
+// Threads lie over the columns of a state row (four each) and over groups of rows.
+// ---------------------------------------------------------------------------
+template <bool VEC>
+__global__ void __launch_bounds__(256)
+step_kernel(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+            const float* __restrict__ decay, int n_decay, float* __restrict__ state, float* __restrict__ o, int Dk,
+            int Dv, int lanes) {
+  __shared__ float qs[kMaxDim], ks[kMaxDim];
+  __shared__ float part[256 * 4];
+  const int64_t head = blockIdx.x;
+  const int tid = threadIdx.x, col = (tid % lanes) * 4, group = tid / lanes, groups = 256 / lanes;
+  if (tid < Dk) {
+    qs[tid] = q[head * Dk + tid];
+    ks[tid] = k[head * Dk + tid];
+  }
+  const float r = 1.0f - decay[n_decay > 1 ? head % n_decay : 0] * (1.0f / 4096.0f);
+  float ve[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) ve[e] = col + e < Dv ? v[head * Dv + col + e] : 0.f;
+  __syncthreads();
+  float* S = state + head * Dk * Dv + col;
+  if (col < Dv) {
+#pragma unroll 8
+    for (int d = group; d < Dk; d += groups) {
+      float x[4];
+      if (VEC) {
+        const float4 a = *reinterpret_cast<const float4*>(S + (int64_t)d * Dv);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = col + e < Dv ? S[(int64_t)d * Dv + e] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = fmaf(r, x[e], ks[d] * ve[e]);
+        acc[e] = fmaf(qs[d], x[e], acc[e]);
+      }
+      if (VEC) {
+        *reinterpret_cast<float4*>(S + (int64_t)d * Dv) = make_float4(x[0], x[1], x[2], x[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < Dv) S[(int64_t)d * Dv + e] = x[e];
+      }
+    }
+  }
+  *reinterpret_cast<float4*>(&part[tid * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (tid < Dv) {
+    float sum = 0.f;
+    for (int g = 0; g < groups; ++g) sum += part[g * lanes * 4 + tid];
+    o[head * Dv + tid] = sum;
+  }
+}
+
+int check_shape(int64_t heads, int64_t H, int64_t n_decay, int64_t Dk, int64_t Dv, int64_t T) {
+  SB_REQUIRE(heads >= 0 && T >= 0 && H >= 1, "negative geometry");
+  SB_REQUIRE(Dk >= 1 && Dk <= kMaxDim && Dv >= 1 && Dv <= kMaxDim, "head widths %lld, %lld outside 1..%d",
+             (long long)Dk, (long long)Dv, kMaxDim);
+  SB_REQUIRE(heads % H == 0, "%lld heads are no multiple of %lld heads a sample", (long long)heads, (long long)H);
+  SB_REQUIRE(n_decay == 1 || n_decay == H, "decay has %lld elements, expected 1 or %lld", (long long)n_decay,
+             (long long)H);
+  SB_REQUIRE(T < (1LL << 31) - 256 && heads < (1LL << 31), "geometry too large");
+  return SB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t sb_linear_attention_scratch_bytes(int64_t heads, int64_t Dk, int64_t Dv, int64_t T, int backward) {
+  (void)heads; (void)Dk; (void)Dv; (void)T; (void)backward;
+  return 0;
+}
+
+int sb_linear_attention_fwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                            const float* state, float* out, float* final_state, int64_t heads, int64_t H, int64_t Dk,
+                            int64_t Dv, int64_t T, void* scratch, void* stream) {
+  SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
+  if (heads == 0) return SB_OK;
+  SB_REQUIRE(decay && (T == 0 || (q && k && v && out)), "null tensor pointer");
+  (void)scratch;
+  Walk w{q, k, v, out, decay, state, final_state, (int)n_decay, heads, (int)Dk, (int)Dv, T, Dv, 1, 0, 1};
+  return launch_walk(w, (cudaStream_t)stream);
+}
+
+int sb_linear_attention_bwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                            const float* state, const float* grad_out, const float* grad_final, float* grad_q,
+                            float* grad_k, float* grad_v, float* grad_state, int64_t heads, int64_t H, int64_t Dk,
+                            int64_t Dv, int64_t T, void* scratch, void* stream) {
+  SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
+  if (heads == 0) return SB_OK;
+  SB_REQUIRE(decay && (T == 0 || (q && k && v && grad_out && grad_q && grad_k && grad_v)), "null tensor pointer");
+  (void)scratch;
+  const int nd = (int)n_decay, dk = (int)Dk, dv = (int)Dv;
+  const cudaStream_t s = (cudaStream_t)stream;
+  SB_TRY(launch_walk(Walk{grad_out, v, k, grad_q, decay, state, nullptr, nd, heads, dv, dk, T, 1, Dv, 0, 1}, s));
+  SB_TRY(launch_walk(Walk{v, grad_out, q, grad_k, decay, grad_final, nullptr, nd, heads, dv, dk, T, 1, Dv, 1, 0}, s));
+  return launch_walk(Walk{k, q, grad_out, grad_v, decay, grad_final, grad_state, nd, heads, dk, dv, T, Dv, 1, 1, 0}, s);
+}
+
+int sb_linear_attention_step(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                             float* state, float* out, int64_t heads, int64_t H, int64_t Dk, int64_t Dv,
+                             void* stream) {
+  SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, 1));
+  if (heads == 0) return SB_OK;
+  SB_REQUIRE(q && k && v && decay && state && out, "null tensor pointer");
+  int lanes = 1;
+  while (lanes * 4 < Dv) lanes *= 2;
+  const bool vec = Dv % 4 == 0 && ((uintptr_t)state & 15u) == 0;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (vec)
+    step_kernel<true><<<(unsigned)heads, 256, 0, s>>>(q, k, v, decay, (int)n_decay, state, out, (int)Dk, (int)Dv, lanes);
+  else
+    step_kernel<false><<<(unsigned)heads, 256, 0, s>>>(q, k, v, decay, (int)n_decay, state, out, (int)Dk, (int)Dv, lanes);
+  SB_CUDA(cudaGetLastError());
+  return SB_OK;
+}
+
+}  // extern "C"

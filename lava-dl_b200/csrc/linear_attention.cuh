@@ -1,0 +1,31 @@
+// Shared by the translation units of the linear attention (api_linear_attention*.cu).
+#pragma once
+
+#include "api_util.cuh"
+
+namespace sb {
+namespace la {
+
+constexpr int kMaxDim = 128;   // widest head
+
+// One walk over time: o[t] = S[t]^T q[t].  The state's element (d, e) of a head lies at
+// d * s_row + e * s_col, so that a walk on the transposed state reads and writes the caller's layout.
+struct Walk {
+  const float* q;
+  const float* k;
+  const float* v;
+  float* o;
+  const float* decay;
+  const float* s_in;    // nullable: zero
+  float* s_out;         // nullable
+  int n_decay;          // 1 or heads per sample
+  int64_t heads;
+  int Dk, Dv;
+  int64_t T;
+  int64_t s_row, s_col;
+  int reverse;          // from the last step to the first
+  int after;            // the state decays before a step is added (1) or after it has been read (0)
+};
+
+}  // namespace la
+}  // namespace sb

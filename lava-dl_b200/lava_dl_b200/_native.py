@@ -85,6 +85,14 @@ SIGNATURES = {
     'sb_conv_wgrad_scratch_bytes': (_I64, [_I64] * 7),
     'sb_conv_wgrad': (c_int, [_P, _P, _P, _P] + [_I64] * 10 + [_P]),
     'sb_conv_wgrad_fits': (c_int, [_I64] * 10),
+    'sb_linear_attention_scratch_bytes': (_I64, [_I64, _I64, _I64, _I64, c_int]),
+    'sb_linear_attention_fwd': (c_int, [_P, _P, _P, _P, _I64, _P, _P, _P] + [_I64] * 5 + [_P, _P]),
+    'sb_linear_attention_bwd': (c_int, [_P, _P, _P, _P, _I64] + [_P] * 7 + [_I64] * 5 + [_P, _P]),
+    'sb_linear_attention_step': (c_int, [_P, _P, _P, _P, _I64, _P, _P] + [_I64] * 4 + [_P]),
+    'sb_qdense_scratch_bytes': (_I64, [_I64, _I64]),
+    'sb_qdense_fwd': (c_int, [_P, _P, _P, _P] + [_I64] * 5 + [_P, _P]),
+    'sb_dropout': (c_int, [_P, _P, _P, _I64, _I64, c_double, c_int, _P]),
+    'sb_dropout_next': (c_int, [_P, _P, _P]),
     'sb_unpack_spikes_host': (c_int, [_P, _P, _I64, _I64, c_int, c_int, _P]),
     'sb_broadcast_fill': (c_int, [_P, _P, _I64, _P]),
     'sb_shift_fir_bwd': (c_int, [_P, _P, _I64, c_float, c_float, _P, _I64, c_float, _P, _I64, _I64, _P]),

@@ -771,3 +771,141 @@ def conv_dgrad(grad_y, weight, padding):
     # than the fp32 kernel where the swapped problem fits it); the library chooses
     pad = (kh - 1 - int(padding[0]), kw - 1 - int(padding[1]))
     return conv_fwd(grad_y, wt, pad, path=-1)
+
+
+# --------------------------------------------------------------------------
+# linear attention
+# --------------------------------------------------------------------------
+def _same_device(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f'{name} is on {t.device}, expected {first.device}')
+
+
+def _written(t):
+    """Tell autograd that a kernel wrote to ``t``: a graph that saved it must not use the new values."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
+def _attention_check(q, k, v, decay, state, time):
+    """Argument checks of the linear attention; returns (samples, H, Dk, Dv)."""
+    N.require_cuda(q, k, v, decay, state)
+    _same_device(q, key=k, value=v, decay=decay, state=state)
+    dims = 4 if time else 3
+    if q.dim() != dims or k.shape != q.shape:
+        raise ValueError(f'query and key must have one shape [batch, heads, width{", time" if time else ""}], '
+                         f'found {tuple(q.shape)} and {tuple(k.shape)}')
+    if v.dim() != dims or v.shape[:2] != q.shape[:2] or (time and v.shape[3] != q.shape[3]):
+        raise ValueError(f'value of shape {tuple(v.shape)} does not match query of shape {tuple(q.shape)}')
+    n, h, dk, dv = q.shape[0], q.shape[1], q.shape[2], v.shape[2]
+    if not (1 <= dk <= 128 and 1 <= dv <= 128):
+        raise ValueError(f'head widths of 1 to 128 are supported, found {dk} (query, key) and {dv} (value)')
+    if decay.numel() not in (1, h):
+        raise ValueError(f'decay must have 1 or {h} elements, found {decay.numel()}')
+    if state is not None and tuple(state.shape) != (n, h, dk, dv):
+        raise ValueError(f'state must have shape {(n, h, dk, dv)}, found {tuple(state.shape)}')
+    return n, h, dk, dv
+
+
+def _attention_scratch(heads, dk, dv, T, backward, device):
+    nbytes = N.load().sb_linear_attention_scratch_bytes(heads, dk, dv, T, int(backward))
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def linear_attention_fwd(q, k, v, decay, state=None, want_final=False):
+    n, h, dk, dv = _attention_check(q, k, v, decay, state, True)
+    q, k, v, decay = _c(q), _c(k), _c(v), _param(decay, q)
+    state = None if state is None else _c(state)
+    T = q.shape[-1]
+    out = torch.empty_like(v)
+    final = torch.empty(n, h, dk, dv, device=q.device, dtype=torch.float32) if want_final else None
+    scratch = _attention_scratch(n * h, dk, dv, T, False, q.device)
+    N.call('sb_linear_attention_fwd', q, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(), N.ptr(state),
+           N.ptr(out), N.ptr(final), n * h, max(h, 1), dk, dv, T, N.ptr(scratch), N.stream_of(q))
+    return out, final
+
+
+def linear_attention_bwd(q, k, v, decay, state, grad_out, grad_final, want_grad_state):
+    n, h, dk, dv = _attention_check(q, k, v, decay, state, True)
+    q, k, v, decay, grad_out = _c(q), _c(k), _c(v), _param(decay, q), _c(grad_out)
+    state = None if state is None else _c(state)
+    grad_final = None if grad_final is None else _c(grad_final)
+    T = q.shape[-1]
+    gq, gk, gv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    gs = torch.empty(n, h, dk, dv, device=q.device, dtype=torch.float32) if want_grad_state else None
+    scratch = _attention_scratch(n * h, dk, dv, T, True, q.device)
+    N.call('sb_linear_attention_bwd', q, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(), N.ptr(state),
+           N.ptr(grad_out), N.ptr(grad_final), N.ptr(gq), N.ptr(gk), N.ptr(gv), N.ptr(gs), n * h, max(h, 1), dk, dv,
+           T, N.ptr(scratch), N.stream_of(q))
+    return gq, gk, gv, gs
+
+
+def linear_attention_step(q, k, v, decay, state):
+    if state is None:
+        raise ValueError('step needs the state that it updates')
+    n, h, dk, dv = _attention_check(q, k, v, decay, state, False)
+    if not state.is_contiguous():
+        raise ValueError('state is updated in place and must be contiguous')
+    q, k, v, decay = _c(q), _c(k), _c(v), _param(decay, q)
+    out = torch.empty_like(v)
+    N.call('sb_linear_attention_step', q, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(), N.ptr(state),
+           N.ptr(out), n * h, max(h, 1), dk, dv, N.stream_of(q))
+    _written(state)
+    return out
+
+
+# --------------------------------------------------------------------------
+# 8-bit dense synapse
+# --------------------------------------------------------------------------
+def qdense_fwd(x, weight, weight_scale, in_neurons):
+    """``[N, K, T]`` fp32 times int8 rows ``[O, Kp]`` (zero-padded) -> ``[N, O, T]`` fp32."""
+    N.require_cuda(x, weight_scale)
+    if weight.dtype != torch.int8:
+        raise TypeError(f'expected int8 weights, got {weight.dtype}')
+    _same_device(x, weight=weight, weight_scale=weight_scale)
+    n, k, T = x.shape
+    if k != in_neurons:
+        raise ValueError(f'expected {in_neurons} input neurons, found {k}')
+    x, weight, weight_scale = _c(x), _c(weight), _c(weight_scale)
+    o, kp = weight.shape
+    y = torch.empty(n, o, T, device=x.device, dtype=torch.float32)
+    nbytes = N.load().sb_qdense_scratch_bytes(n * T, kp)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes > 0 else None
+    N.call('sb_qdense_fwd', x, N.ptr(x), N.ptr(weight), N.ptr(weight_scale), N.ptr(y), n, k, kp, o, T,
+           N.ptr(scratch), N.stream_of(x))
+    return y
+
+
+# --------------------------------------------------------------------------
+# dropout
+# --------------------------------------------------------------------------
+def _key_check(key, what):
+    if key.dtype != torch.int64 or key.numel() != 2 or not key.is_contiguous():
+        raise ValueError(f'{what} must be a contiguous int64 tensor of 2 elements (seed, offset)')
+    if not key.is_cuda:
+        raise RuntimeError(f'{what} must be a CUDA tensor, it is on {key.device}')
+
+
+def dropout(x, p, key, per_step):
+    N.require_cuda(x)
+    _key_check(key, 'key')
+    _same_device(x, key=key)
+    if x.dim() < 1:
+        raise ValueError('dropout needs a tensor with a time axis')
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f'dropout probability has to be between 0 and 1, but got {p}')
+    x = _c(x)
+    rows, T = _rows_T(x)
+    out = torch.empty_like(x)
+    N.call('sb_dropout', x, N.ptr(x), N.ptr(out), N.ptr(key), rows, T, float(p), int(bool(per_step)), N.stream_of(x))
+    return out
+
+
+def dropout_next(state):
+    """Key of this call out of a generator state ``(seed, offset)`` on the device; moves the offset on."""
+    _key_check(state, 'generator state')
+    key = torch.empty_like(state)
+    N.call('sb_dropout_next', state, N.ptr(state), N.ptr(key), N.stream_of(state))
+    _written(state)
+    return key

@@ -50,6 +50,21 @@ def make_family(neuron_class, default_delay_shift=True, synapse=real_synapse):
             super().__init__(*args, **kwargs)
             self._attach(synapse.Dense, kwargs)
 
+    class Attention(_Family, base.AbstractAttention):
+        __doc__ = base.AbstractAttention.__doc__
+
+        def __init__(self, *args, **kwargs):
+            super().__init__(*args, **kwargs)
+            for name in ('query', 'key', 'value'):
+                neuron = neuron_class(**self.neuron_params)
+                part = synapse.Dense(**self.head_params)
+                if 'pre_hook_fx' not in kwargs:
+                    part.pre_hook_fx = neuron.quantize_8bit
+                setattr(self, name + '_neuron', neuron)
+                setattr(self, name + '_synapse', part)
+            self._attach(synapse.Dense, kwargs)
+            del self.head_params
+
     class Conv(_Family, base.AbstractConv):
         __doc__ = base.AbstractConv.__doc__
 
@@ -90,4 +105,4 @@ def make_family(neuron_class, default_delay_shift=True, synapse=real_synapse):
             del self.neuron_params, self.synapse_params, self.recurrent_params
 
     return dict(Input=Input, Flatten=Flatten, Average=Average, Dense=Dense, Conv=Conv, Pool=Pool, KWTA=KWTA,
-                Recurrent=Recurrent)
+                Recurrent=Recurrent, Attention=Attention)

@@ -6,6 +6,8 @@ import numpy as np
 import torch
 
 from ..axon import delay
+from ..neuron.dynamics import linear_attention
+from ..synapse import QuantDense
 
 
 def step_delay(module, x):
@@ -185,6 +187,111 @@ class AbstractDense(_Block):
             self.mask = None
         else:
             self.register_buffer('mask', mask.reshape(mask.shape[0], mask.shape[1], 1, 1, 1))
+
+
+    def quantize(self):
+        """Replace the synapse by its 8-bit inference form (``synapse.QuantDense``), mask included;
+        weights on the neuron's grid are kept exactly.  Returns the block."""
+        if self.mask is not None:
+            self.synapse.weight.data *= self.mask
+            self.mask = None
+        self.synapse = _quantized(self.synapse, self.neuron)
+        return self
+
+
+def _quantized(dense, neuron):
+    """The 8-bit form of a dense synapse, on the neuron's weight grid when that is its pre-hook."""
+    if isinstance(dense, QuantDense):
+        return dense
+    if dense.complex:
+        raise NotImplementedError('complex synapses have no 8-bit form')
+    on_grid = dense.pre_hook_fx == neuron.quantize_8bit
+    return QuantDense.from_dense(dense, 2 / neuron.w_scale if on_grid else None)
+
+
+class AbstractAttention(_Block):
+    """Attention block (no counterpart in lava-dl): three dense synapses with neurons make query, key
+    and value spikes, heads of decaying linear attention relate the time steps
+    (``neuron.dynamics.linear_attention``), and a dense synapse with a neuron, the one-step delay and
+    the optional axonal delay make the output spikes.
+
+    With ``persistent_state`` neurons the attention state is kept between calls as well; a call of
+    one time step without gradients then takes the single-step kernel.
+
+    Parameters
+    ----------
+    neuron_params : dict
+        parameters of all four neuron groups.
+    in_neurons, out_neurons, num_heads : int
+    head_neurons : int or None
+        width of a head, at most 128; ``None`` is ``out_neurons // num_heads``.
+    memory_decay : float, (float, float) or sequence of num_heads floats
+        fraction of the state a head loses at each step; a pair is spread over the heads in equal
+        ratios.
+    weight_scale, weight_norm, pre_hook_fx : options of all synapses
+    delay, delay_shift, count_log : bool
+    """
+
+    def __init__(self, neuron_params, in_neurons, out_neurons, num_heads, head_neurons=None,
+                 memory_decay=(0.5, 0.004), weight_scale=1, weight_norm=False, pre_hook_fx=None, delay=False,
+                 delay_shift=True, count_log=False):
+        super().__init__()
+        if head_neurons is None:
+            if out_neurons % num_heads:
+                raise ValueError(f'{out_neurons} neurons cannot be split over {num_heads} heads; set head_neurons')
+            head_neurons = out_neurons // num_heads
+        if not 1 <= head_neurons <= 128:
+            raise ValueError(f'heads of 1 to 128 neurons are supported, found {head_neurons}')
+        options = dict(weight_scale=weight_scale, weight_norm=weight_norm, pre_hook_fx=pre_hook_fx)
+        inner = num_heads * head_neurons
+        self._init_block(neuron_params, dict(in_neurons=inner, out_neurons=out_neurons, **options), delay_shift,
+                         count_log)
+        self.head_params = dict(in_neurons=in_neurons, out_neurons=inner, **options)
+        self.num_heads, self.head_neurons = num_heads, head_neurons
+        values = np.atleast_1d(np.asarray(memory_decay, dtype=np.float64))
+        if values.size == 1:
+            values = np.repeat(values, num_heads)
+        elif values.size == 2 and num_heads != 2:
+            values = np.geomspace(values[0], values[1], num_heads)
+        if values.size != num_heads or values.min() < 0 or values.max() > 1:
+            raise ValueError(f'memory_decay {memory_decay} does not give {num_heads} fractions')
+        self.register_buffer('memory_decay', torch.tensor(4096 * values, dtype=torch.float32))
+        self.memory_state = None
+
+    def _heads(self, x):
+        return x.reshape(x.shape[0], self.num_heads, self.head_neurons, x.shape[-1])
+
+    def _remember(self, query, key, value):
+        if self.neuron.persistent_state is not True:
+            return linear_attention.dynamics(query, key, value, self.memory_decay)
+        state = self.memory_state
+        if state is not None and (state.shape[0] != query.shape[0] or state.device != query.device):
+            state = None    # batch size changed
+        if query.shape[-1] == 1 and not torch.is_grad_enabled():
+            if state is None:
+                state = query.new_zeros(query.shape[0], self.num_heads, self.head_neurons, self.head_neurons)
+            out = linear_attention.step(query[..., 0], key[..., 0], value[..., 0], self.memory_decay, state)
+            self.memory_state = state
+            return out.unsqueeze(-1)
+        out, state = linear_attention.dynamics(query, key, value, self.memory_decay, state, return_state=True)
+        self.memory_state = state.detach()
+        return out
+
+    def forward(self, x):
+        """``NCT`` input -> spikes (and event rate when ``count_log``)."""
+        query, key, value = (self._heads(neuron(synapse(x))) for synapse, neuron in (
+            (self.query_synapse, self.query_neuron), (self.key_synapse, self.key_neuron),
+            (self.value_synapse, self.value_neuron)))
+        read = self._remember(query, key, value)
+        return super().forward(read.reshape(read.shape[0], -1, read.shape[-1]))
+
+    def quantize(self):
+        """Replace the synapses by their 8-bit inference forms; returns the block."""
+        for name in ('query', 'key', 'value'):
+            synapse, neuron = getattr(self, name + '_synapse'), getattr(self, name + '_neuron')
+            setattr(self, name + '_synapse', _quantized(synapse, neuron))
+        self.synapse = _quantized(self.synapse, self.neuron)
+        return self
 
 
 class AbstractConv(_Block):

@@ -1,0 +1,90 @@
+"""Linear attention with a decay for each head (no counterpart in lava-dl): a leaky integrator whose
+input is the outer product of a key and a value, read out by a query."""
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .... import _ops
+
+
+def dynamics(query, key, value, decay, state=None, return_state=False):
+    """Linear attention over whole sequences.
+
+    .. math::
+        S[t] &= (1 - \\alpha / 4096)\\,S[t-1] + k[t]\\,v[t]^\\top \\
+
+        o[t] &= S[t]^\\top q[t]
+
+    Differentiable in ``query``, ``key``, ``value`` and ``state``.  ``decay`` is a constant of the
+    head: one that requires a gradient is refused.  Values that are not finite reach the outputs of
+    their own step and of later steps, never earlier ones.
+
+    Parameters
+    ----------
+    query, key : torch tensor
+        CUDA tensors ``[batch, heads, width, time]``, width 1 to 128.
+    value : torch tensor
+        CUDA tensor ``[batch, heads, width of the value, time]``, width 1 to 128.
+    decay : torch tensor
+        decay (un-scaled value, 0..4096, not rounded), 1 element or one per head.
+    state : torch tensor or None
+        state before the first step, ``[batch, heads, width, width of the value]``; ``None`` is zero.
+    return_state : bool
+        also return the state after the last step.
+
+    Returns
+    -------
+    torch tensor or pair of torch tensors
+        output, shaped like ``value`` (and the state).
+    """
+    if torch.is_grad_enabled() and decay.requires_grad:
+        raise RuntimeError('linear attention has no gradient for its decay; pass decay.detach()')
+    output, final = _LinearAttention.apply(query, key, value, decay, state, return_state)
+    return (output, final) if return_state else output
+
+
+def step(query, key, value, decay, state):
+    """One step of :func:`dynamics` on a kept state, for inference.
+
+    Parameters
+    ----------
+    query, key : torch tensor
+        CUDA tensors ``[batch, heads, width]``.
+    value : torch tensor
+        CUDA tensor ``[batch, heads, width of the value]``.
+    decay : torch tensor
+        as in :func:`dynamics`.
+    state : torch tensor
+        contiguous ``[batch, heads, width, width of the value]``; UPDATED IN PLACE.
+
+    Returns
+    -------
+    torch tensor
+        output, shaped like ``value``.
+    """
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (query, key, value, decay, state)):
+        raise RuntimeError('linear attention steps update their state in place and have no gradient; use dynamics(), '
+                           'or call step() under torch.no_grad()')
+    return _ops.linear_attention_step(query, key, value, decay, state)
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, value, decay, state, return_state):
+        ctx.set_materialize_grads(False)
+        output, final = _ops.linear_attention_fwd(query, key, value, decay, state, return_state)
+        ctx.save_for_backward(query, key, value, decay, state)
+        return output, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output, grad_final):
+        query, key, value, decay, state = ctx.saved_tensors
+        if grad_output is None and grad_final is None:
+            return None, None, None, None, None, None
+        if grad_output is None:
+            grad_output = torch.zeros_like(value)
+        grad_q, grad_k, grad_v, grad_s = _ops.linear_attention_bwd(
+            query, key, value, decay, state, grad_output, grad_final, ctx.needs_input_grad[4])
+        return grad_q, grad_k, grad_v, None, grad_s, None

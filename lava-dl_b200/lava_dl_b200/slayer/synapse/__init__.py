@@ -10,5 +10,6 @@ networks, can be assembled around the neuron kernels.
 
 from . import complex
 from .layer import Dense, Conv, Pool
+from .quantized import QuantDense
 
-__all__ = ['Dense', 'Conv', 'Pool', 'complex']
+__all__ = ['Dense', 'Conv', 'Pool', 'QuantDense', 'complex']
