@@ -10,6 +10,7 @@ from ..neuron import adrf
 _blocks = make_family(adrf.Neuron, synapse=synapse.complex)
 Input, Flatten, Average = _blocks['Input'], _blocks['Flatten'], _blocks['Average']
 Dense, Conv, Pool = _blocks['Dense'], _blocks['Conv'], _blocks['Pool']
-KWTA, Recurrent, Attention = _blocks['KWTA'], _blocks['Recurrent'], _blocks['Attention']
+KWTA, Recurrent = _blocks['KWTA'], _blocks['Recurrent']
+Attention = _blocks['Attention']   # beyond the reference's blocks, which __all__ lists
 
-__all__ = ['Input', 'Flatten', 'Average', 'Dense', 'Conv', 'Pool', 'KWTA', 'Recurrent', 'Attention']
+__all__ = ['Input', 'Flatten', 'Average', 'Dense', 'Conv', 'Pool', 'KWTA', 'Recurrent']
