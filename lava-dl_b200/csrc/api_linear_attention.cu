@@ -125,6 +125,54 @@ int launch_walk(const Walk& w, cudaStream_t s) {
   return SB_OK;
 }
 
+// Short sequences walk step by step; from kMinSteps on the chunked kernel is ahead.
+constexpr int64_t kMinSteps = 48;
+
+// Splits walks into the two widths of the chunked kernel; returns how many come first.
+int by_width(const Walk* in, int n, Walk* out) {
+  int k = 0;
+  for (int i = 0; i < n; ++i)
+    if (in[i].Dk <= 64) out[k++] = in[i];
+  const int narrow = k;
+  for (int i = 0; i < n; ++i)
+    if (in[i].Dk > 64) out[k++] = in[i];
+  return narrow;
+}
+
+int run_walks(const Walk* walks, int n, void* scratch, cudaStream_t s) {
+  if (walks[0].T < kMinSteps) {
+    for (int i = 0; i < n; ++i) SB_TRY(launch_walk(walks[i], s));
+    return SB_OK;
+  }
+  Walk w[3];
+  const int narrow = by_width(walks, n, w);
+  float* f = static_cast<float*>(scratch);
+  if (narrow) {
+    const int64_t need = tc_scratch_floats(w, narrow);
+    SB_REQUIRE(need == 0 || f, "null scratch pointer");
+    SB_TRY(tc_walks(w, narrow, f, s));
+    f += need;
+  }
+  if (narrow < n) {
+    SB_REQUIRE(tc_scratch_floats(w + narrow, n - narrow) == 0 || scratch, "null scratch pointer");
+    SB_TRY(tc_walks(w + narrow, n - narrow, f, s));
+  }
+  return SB_OK;
+}
+
+// The walks of a forward or backward pass, without tensors: what the scratch size is computed from.
+int shape_walks(int64_t heads, int dk, int dv, int64_t T, bool backward, Walk* w) {
+  Walk f{}, b{};
+  f.heads = b.heads = heads;
+  f.T = b.T = T;
+  f.Dk = b.Dv = dk;
+  f.Dv = b.Dk = dv;
+  w[0] = backward ? b : f;
+  w[1] = b;
+  w[2] = f;
+  return backward ? 3 : 1;
+}
+
 // ---------------------------------------------------------------------------
 // One step on a kept state: reads and writes the state once, Dk x Dv floats each way.
 // Threads lie over the columns of a state row (four each) and over groups of rows.
@@ -198,8 +246,14 @@ int check_shape(int64_t heads, int64_t H, int64_t n_decay, int64_t Dk, int64_t D
 extern "C" {
 
 int64_t sb_linear_attention_scratch_bytes(int64_t heads, int64_t Dk, int64_t Dv, int64_t T, int backward) {
-  (void)heads; (void)Dk; (void)Dv; (void)T; (void)backward;
-  return 0;
+  if (check_shape(heads, 1, 1, Dk, Dv, T) != SB_OK || heads == 0 || T < kMinSteps) return 0;
+  Walk all[3], w[3];
+  const int n = shape_walks(heads, (int)Dk, (int)Dv, T, backward != 0, all);
+  const int narrow = by_width(all, n, w);
+  int64_t floats = 0;
+  if (narrow) floats += tc_scratch_floats(w, narrow);
+  if (narrow < n) floats += tc_scratch_floats(w + narrow, n - narrow);
+  return floats * (int64_t)sizeof(float);
 }
 
 int sb_linear_attention_fwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
@@ -208,9 +262,8 @@ int sb_linear_attention_fwd(const float* q, const float* k, const float* v, cons
   SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
   if (heads == 0) return SB_OK;
   SB_REQUIRE(decay && (T == 0 || (q && k && v && out)), "null tensor pointer");
-  (void)scratch;
-  Walk w{q, k, v, out, decay, state, final_state, (int)n_decay, heads, (int)Dk, (int)Dv, T, Dv, 1, 0, 1};
-  return launch_walk(w, (cudaStream_t)stream);
+  const Walk w{q, k, v, out, decay, state, final_state, (int)n_decay, heads, (int)Dk, (int)Dv, T, Dv, 1, 0, 1};
+  return run_walks(&w, 1, scratch, (cudaStream_t)stream);
 }
 
 int sb_linear_attention_bwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
@@ -220,12 +273,11 @@ int sb_linear_attention_bwd(const float* q, const float* k, const float* v, cons
   SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
   if (heads == 0) return SB_OK;
   SB_REQUIRE(decay && (T == 0 || (q && k && v && grad_out && grad_q && grad_k && grad_v)), "null tensor pointer");
-  (void)scratch;
   const int nd = (int)n_decay, dk = (int)Dk, dv = (int)Dv;
-  const cudaStream_t s = (cudaStream_t)stream;
-  SB_TRY(launch_walk(Walk{grad_out, v, k, grad_q, decay, state, nullptr, nd, heads, dv, dk, T, 1, Dv, 0, 1}, s));
-  SB_TRY(launch_walk(Walk{v, grad_out, q, grad_k, decay, grad_final, nullptr, nd, heads, dv, dk, T, 1, Dv, 1, 0}, s));
-  return launch_walk(Walk{k, q, grad_out, grad_v, decay, grad_final, grad_state, nd, heads, dk, dv, T, Dv, 1, 1, 0}, s);
+  const Walk w[3] = {{grad_out, v, k, grad_q, decay, state, nullptr, nd, heads, dv, dk, T, 1, Dv, 0, 1},
+                     {v, grad_out, q, grad_k, decay, grad_final, nullptr, nd, heads, dv, dk, T, 1, Dv, 1, 0},
+                     {k, q, grad_out, grad_v, decay, grad_final, grad_state, nd, heads, dk, dv, T, Dv, 1, 1, 0}};
+  return run_walks(w, 3, scratch, (cudaStream_t)stream);
 }
 
 int sb_linear_attention_step(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,

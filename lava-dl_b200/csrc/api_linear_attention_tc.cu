@@ -1,0 +1,823 @@
+// Linear attention on the tensor cores: the walk of api_linear_attention.cu in chunks of 128 steps.
+//
+// With i, j the steps of a chunk, S the state before it and a = 1 (the state decays before a step is
+// added) or 0 (after it has been read),
+//
+//   o_i  = sum_{j <= i} r^(i-j) (q_i . k_j) v_j  +  r^(i+a) S^T q_i
+//   S'   = r^L S + sum_j r^(L-a-j) k_j v_j^T                        (L = 128, or what is left of T)
+//
+// i.e. four products per chunk and 64 columns of v: scores q k^T [128 x Dk x 128], read-out P v
+// [128 x 128 x 64], the state's part q S [128 x Dk x 64] and its growth v^T k [64 x 128 x Dk].
+//
+// Precision.  The operands are fp32.  Each is split into two fp16 numbers, x 2^-f = hi + lo, 22 bits
+// together, and a product is hi hi + lo hi + hi lo with fp32 accumulators: what is dropped is below
+// 2^-22 of a term.  fp16 rather than TF32 pairs because an MMA step then takes 16 elements of the
+// contraction instead of 8 and a tile half the shared memory, which is what leaves room to stage the
+// next chunk.  fp16 has no range, so the powers of two travel beside the mantissas: q, k and v have one
+// exponent per step, the state one per column of v, and a row of P one per step i: |q_i . k_j| is at most
+// |q_i| |k_j|, so the largest of 2^f |k_j| 2^g over j <= i (a running maximum that decays with r) bounds
+// the row without looking at it, and no outlier costs the accuracy of a step that does not read it.
+// A vector's largest element has 2^13 or more and an fp16 pair steps of 2^-24.
+//
+// Values that are not finite must not meet a zero of the causal mask in an MMA (0 * NaN): the loader
+// zeroes them and notes from which step on a column of the output is spoilt.
+//
+// Layout.  Time is contiguous in memory, so a thread that owns one step reads 64 rows with coalesced
+// loads and holds that step's whole vector: its exponent needs no exchange, and its hi and lo halves are
+// written as one 128-byte row of a [step][channel] tile each.  That one tile of k is the K-major B
+// operand of the scores and the MN-major B operand of the growth; v is MN-major in the read-out, and a
+// copy weighted by r^(L-a-j) is the MN-major A operand of the growth (hi and lo stacked to M = 128, so
+// two MMAs cover the three products).  q goes to tensor memory (it is A of two products) and so does P,
+// converted in place of the scores.
+//
+// Roles of a CTA (one per SM; 384 threads): warps 0-3 load and convert (one step per thread), warps 4-7
+// turn scores into P, keep the state (32 elements per thread and 64 of Dk in registers, fp32), and write
+// the output, warp 8 issues the MMAs.  A head with T steps is one CTA, or several when there are fewer
+// heads than SMs: the axis is then cut into segments, a first launch takes each segment's growth from
+// zero, a small one joins them, and the walk starts every segment from its own state.
+#include "linear_attention.cuh"
+#include "tc.cuh"
+
+namespace sb {
+namespace la {
+namespace {
+
+constexpr int kL = 128;                      // steps per chunk
+constexpr int kTileB = kL * 128;             // bytes of a [128 steps][64 channels] fp16 tile
+constexpr int kThreads = 384;
+// Registers per thread of the three warpgroups: 168 at launch (65536 / 384, in steps of 8), moved to where
+// the vectors live.  232 + 224 + 40 <= 3 * 168.
+constexpr int kRegsLoad = 232, kRegsSoft = 224, kRegsMma = 40;
+constexpr int kMaxSub = 6;
+
+struct TcArgs {
+  Walk w[3];
+  float* seg[3];        // [nseg][heads][Dk * Dv]: states after each segment
+  int nsub;             // CTAs per head and segment: (walk, 64 columns of v)
+  int sub_walk[kMaxSub], sub_e0[kMaxSub];
+  int64_t heads;
+  int nseg, seg_chunks;
+  unsigned int* status;
+};
+
+template <int KT>
+struct Shape {
+  static constexpr int stages = KT == 1 ? 2 : 1;      // KT = 2 has room for one
+  static constexpr int nsp = KT == 1 ? 2 : 1;         // score accumulators
+  static constexpr int stage_bytes = (2 * KT + 4) * kTileB;
+  static constexpr int state_bytes = 2 * KT * 64 * 128;
+  static constexpr int smem = 1024 + stages * stage_bytes + state_bytes;
+  // tensor memory columns
+  static constexpr uint32_t q = 0, sp = 64 * KT, oi = sp + 128 * nsp, ox = oi + 64, ds = ox + 64;
+};
+
+__device__ __forceinline__ float p2(int n) { return __int_as_float((n + 127) << 23); }   // -126 <= n <= 127
+struct Factors {
+  float a, b;
+};
+// 2^n as two factors, so that n may leave the range of a float's exponent
+__device__ __forceinline__ Factors p2_wide(int n) {
+  n = max(-252, min(n, 254));
+  return Factors{p2(n >> 1), p2(n - (n >> 1))};
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// hi = fp16(x), lo = fp16(x - hi) of two neighbours, packed
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t* hi, uint32_t* lo) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(x1), "f"(x0));
+  float h0, h1;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+      : "=f"(h0), "=f"(h1) : "r"(h));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(*lo) : "f"(x1 - h1), "f"(x0 - h0));
+  *hi = h;
+}
+
+// D (+)= A B^T, fp16 operands, fp32 accumulator: A in tensor memory or shared memory, B in shared memory
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(acc)
+      : "memory");
+}
+// fp16 x fp16 -> fp32, M = 128; bits 15 and 16 mark an MN-major A and B
+__host__ __device__ constexpr uint32_t idesc_f16(int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kL >> 4) << 24);
+}
+constexpr uint32_t kAMajorMN = 1u << 15, kBMajorMN = 1u << 16;
+// Low descriptor word: K-major (the leading offset is unused with the 128-byte swizzle), or MN-major
+// with the next 64 channels one tile further on; groups of eight rows lie 1024 bytes apart either way.
+__device__ __forceinline__ uint32_t desc_mn(uint32_t saddr) {
+  return ((saddr & 0x3ffffu) >> 4) | ((uint32_t)(kTileB >> 4) << 16);
+}
+
+// 64 rows of one step
+__device__ __forceinline__ void load64(float (&x)[64], const float* p, int64_t T, int rows, bool in) {
+#pragma unroll
+  for (int d = 0; d < 64; ++d) {
+    x[d] = (in && d < rows) ? __ldg(p) : 0.f;
+    p += T;
+  }
+}
+__device__ __forceinline__ float top64(const float (&x)[64], float m = 0.f) {
+#pragma unroll
+  for (int d = 0; d < 64; ++d) m = max_nan(m, fabsf(x[d]));
+  return m;
+}
+// Exponent that brings a largest magnitude into [2^13, 2^14); a zero vector gets one that no sum prefers.
+constexpr int kNoTerm = -400;
+__device__ __forceinline__ int fit_exponent(float top) {
+  const int e = (int)(__float_as_uint(top) >> 23) - 127;
+  return max(e, -113) - 13;
+}
+__device__ __forceinline__ bool not_finite(float top) { return __float_as_uint(top) >= 0x7f800000u; }
+// Smallest u (up to one) with |x| <= 2^u, from |x|^2.
+__device__ __forceinline__ int norm_exponent(float n2) {
+  return ((int)(__float_as_uint(n2) >> 23) - 127 + 2) >> 1;
+}
+// Scaled by `s`, split and written as one row of a hi and a lo tile (128-byte swizzle); NORM returns the
+// scaled row's sum of squares.
+template <bool NORM>
+__device__ __forceinline__ float store_row(const float (&x)[64], float s, uint32_t hi_tile, uint32_t lo_tile, int row) {
+  float n2 = 0.f;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x0 = x[8 * c + 2 * e] * s, x1 = x[8 * c + 2 * e + 1] * s;
+      if constexpr (NORM) n2 = fmaf(x0, x0, fmaf(x1, x1, n2));
+      split2(x0, x1, &h[e], &l[e]);
+    }
+    const uint32_t at = (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4));
+    sts128(hi_tile + at, h[0], h[1], h[2], h[3]);
+    sts128(lo_tile + at, l[0], l[1], l[2], l[3]);
+  }
+  return n2;
+}
+
+// KT: 64-wide tiles of Dk.  FULL: the walk itself; otherwise only the state after each segment but the last.
+template <int R>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+
+template <int KT, bool FULL>
+__global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ TcArgs args) {
+  using S_ = Shape<KT>;
+  constexpr int NS = S_::stages, NSP = S_::nsp;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(16) int fg_s[2][kL];
+  __shared__ int m_s[2][kL], qe_s[2][kL], uq_s[2][kL], kmax_s[2][4], mw_s[4];
+  __shared__ float scan_s[2][4];
+  __shared__ float pow_pad[32 + kL + 1];       // r^n at 32 + n; zeros before it are the causal mask
+  __shared__ float scale_s[2][64];
+  __shared__ float top_s[kL];
+  __shared__ int poison_s[64];
+  __shared__ int any_poison_s, dead_s;
+  __shared__ uint32_t tmem_s;
+  __shared__ __align__(8) uint64_t bars[2 + 2 + 2 + 9];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t sbase = base + NS * S_::stage_bytes;
+  volatile int* dead = &dead_s;
+  volatile int* any_poison = &any_poison_s;
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t bar_kv = bar0, bar_free = bar0 + 16, bar_sp = bar0 + 32;
+  const uint32_t bar_q = bar0 + 48, bar_qfree = bar0 + 56, bar_p = bar0 + 64, bar_ds = bar0 + 72, bar_s = bar0 + 80,
+                 bar_o = bar0 + 88, bar_ofree = bar0 + 96, bar_end = bar0 + 104;
+
+  // which head, segment, walk and columns
+  const int64_t bid = blockIdx.x;
+  const int sub = (int)(bid % args.nsub);
+  const int64_t head = (bid / args.nsub) % args.heads;
+  const int seg = (int)(bid / args.nsub / args.heads);
+  const int wi = args.sub_walk[sub], e0 = args.sub_e0[sub];
+  const Walk& w = args.w[wi];
+  const int64_t T = w.T;
+  const int Dk = w.Dk, ne = min(64, w.Dv - e0);
+  const int64_t c0 = (int64_t)seg * args.seg_chunks;
+  const int64_t call = (T + kL - 1) / kL;
+  const int nc = (int)min((int64_t)args.seg_chunks, call - c0);
+  const int after = w.after;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_kv + 8 * i, 128);
+      mbar_init(bar_free + 8 * i, 1);
+      mbar_init(bar_sp + 8 * i, 2);
+    }
+    mbar_init(bar_q, 128);
+    mbar_init(bar_qfree, 1);
+    mbar_init(bar_p, 128);
+    mbar_init(bar_ds, 2);
+    mbar_init(bar_s, 128);
+    mbar_init(bar_o, 1);
+    mbar_init(bar_ofree, 128);
+    mbar_init(bar_end, 1);
+    fence_mbar_init();
+    dead_s = 0;
+    any_poison_s = 0;
+  }
+  if (tid < 64) poison_s[tid] = 0x7fffffff;
+  if (tid < 32) pow_pad[tid] = 0.f;
+  if (tid <= kL) {
+    // r^n by squaring in 64 bits: r itself does not fit 32 (a slow head multiplies it a thousandfold)
+    double b = 1.0 - (double)w.decay[w.n_decay > 1 ? head % w.n_decay : 0] / 4096.0, p = 1.0;
+    for (int n = tid; n; n >>= 1) {
+      if (n & 1) p *= b;
+      b *= b;
+    }
+    pow_pad[32 + tid] = (float)p;
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+
+  if (warp < 4) {
+    // ---------------- load and convert: thread = step of the chunk ----------------
+    regs_inc<kRegsLoad>();
+    const int j = tid;
+    // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
+    const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
+    const float* kb = w.k + head * (int64_t)Dk * T;
+    const float* qb = FULL ? w.q + head * (int64_t)Dk * T : nullptr;
+    const float* vb = w.v + (head * (int64_t)w.Dv + e0) * T;
+    auto at = [&](int c, int64_t* tt) {
+      const int64_t t = (c0 + c) * kL + j;
+      *tt = w.reverse ? T - 1 - t : t;
+      return c < nc && t < T;
+    };
+    // One chunk; A holds k (KT = 1) on entry and B the next chunk's k on exit.  The loads of an operand
+    // are issued as soon as the registers it needs have been converted.
+    auto chunk = [&](int c, float (&A)[64], float (&B)[64]) {
+      const int st = c % NS;
+      const uint32_t stage = base + st * S_::stage_bytes;
+      const uint32_t k_hi = stage, k_lo = stage + KT * kTileB, v_hi = stage + 2 * KT * kTileB, v_lo = v_hi + kTileB,
+                     vw_hi = v_lo + kTileB, vw_lo = vw_hi + kTileB;
+      const int64_t t = (c0 + c) * kL + j;
+      const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
+      int64_t tt;
+      const bool in = at(c, &tt);
+      if constexpr (KT == 1) {
+        load64(B, vb + tt, T, ne, in);
+      } else {
+        load64(A, kb + tt, T, 64, in);
+        load64(B, kb + 64 * T + tt, T, Dk - 64, in);
+      }
+      // k
+      float top = top64(A);
+      if constexpr (KT == 2) top = top64(B, top);
+      bool spoilt = false;
+      if (not_finite(top)) {   // every column is spoilt from this step on
+        spoilt = true;
+#pragma unroll
+        for (int d = 0; d < 64; ++d) {
+          A[d] = 0.f;
+          if constexpr (KT == 2) B[d] = 0.f;
+        }
+        for (int e = 0; e < 64; ++e) atomicMin(&poison_s[e], (int)t);
+        any_poison_s = 1;
+        top = 0.f;
+      }
+      const int f = fit_exponent(top);
+      int fg = top > 0.f ? f : kNoTerm;
+      if (c >= NS) wait_or_dead(bar_free + 8 * st, (uint32_t)(c / NS - 1) & 1u, dead);
+      float n2 = store_row<true>(A, p2(-f), k_hi, k_lo, j);
+      if constexpr (KT == 2) {
+        n2 += store_row<true>(B, p2(-f), k_hi + kTileB, k_lo + kTileB, j);
+        load64(A, vb + tt, T, ne, in);
+      } else if (FULL) {
+        load64(A, qb + tt, T, Dk, in);
+      }
+      // v
+      float(&V)[64] = KT == 1 ? B : A;
+      float vtop = top64(V);
+      if (spoilt || not_finite(vtop)) {
+        vtop = 0.f;
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+          if (spoilt) V[e] = 0.f;
+          if (not_finite(fabsf(V[e]))) {
+            V[e] = 0.f;
+            atomicMin(&poison_s[e], (int)t);
+            any_poison_s = 1;
+          }
+          vtop = fmaxf(vtop, fabsf(V[e]));
+        }
+      }
+      const int g = fit_exponent(vtop);
+      fg = (vtop > 0.f && fg != kNoTerm) ? fg + g : kNoTerm;
+      // weight of the step in the state, and the largest exponents: of the steps so far, of the weighted all
+      const float wt = (j < len) ? pow_pad[32 + len - after - j] : 0.f;
+      const int we = (int)((__float_as_uint(wt) >> 23) & 0xff) - 127;
+      const int key = wt != 0.f && fg != kNoTerm ? fg + we : kNoTerm;
+      // running maximum of log2(2^fg |k_j|) + (i - j) log2 r: the scan runs on that less i log2 r
+      float mk = fg == kNoTerm ? -1e30f : (float)(fg + norm_exponent(n2)) - (float)j * slope;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float up = __shfl_up_sync(0xffffffffu, mk, o);
+        if (lane >= o) mk = fmaxf(mk, up);
+      }
+      const int kmax = __reduce_max_sync(0xffffffffu, key);
+      if (lane == 31) {
+        scan_s[c & 1][warp] = mk;
+        kmax_s[c & 1][warp] = kmax;
+      }
+      bar_sync(1, 128);
+      int mw = kNoTerm;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < warp) mk = fmaxf(mk, scan_s[c & 1][i]);
+        mw = max(mw, kmax_s[c & 1][i]);
+      }
+      const int m = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
+      fg_s[c & 1][j] = fg == kNoTerm ? -100000 : fg;   // so far down that its column of P is zero
+      m_s[c & 1][j] = m;
+      if (j == 0) mw_s[c & 3] = mw;
+      if constexpr (FULL) store_row<false>(V, p2(-g), v_hi, v_lo, j);
+      {
+        // v 2^-g r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa last
+        float s = 0.f;
+        if (key != kNoTerm) {
+          const int n = max(fg + we - mw, -100);            // <= 0
+          s = (wt * p2(max(-we, -126))) * p2(n);            // [1, 2) * 2^n
+        }
+#pragma unroll
+        for (int e = 0; e < 64; ++e) V[e] *= p2(-g);
+        store_row<false>(V, s, vw_hi, vw_lo, j);
+      }
+      fence_proxy_async();
+      mbar_arrive(bar_kv + 8 * st);
+      // q
+      if constexpr (FULL) {
+        int64_t tn;
+        const bool next_in = at(c + 1, &tn);
+        if constexpr (KT == 1) {
+          load64(B, kb + tn, T, Dk, next_in);
+        } else {
+          load64(A, qb + tt, T, 64, in);
+          load64(B, qb + 64 * T + tt, T, Dk - 64, in);
+        }
+        float qtop = top64(A);
+        if constexpr (KT == 2) qtop = top64(B, qtop);
+        const bool qbad = not_finite(qtop);
+        const int qe = qbad ? 0 : fit_exponent(qtop);
+        const float qs = p2(-qe);
+        qe_s[c & 1][j] = qbad ? 0x7fffffff : qe;
+        if (c >= 1) wait_or_dead(bar_qfree, (uint32_t)(c - 1) & 1u, dead);
+        tc_fence_after();
+        const uint32_t row = tmem + ((uint32_t)(warp * 32) << 16) + S_::q;
+        float q2 = 0.f;
+#pragma unroll
+        for (int half = 0; half < KT; ++half) {
+          float(&Q)[64] = half == 0 ? A : B;
+          uint32_t hi[32], lo[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float x0 = Q[2 * e] * qs, x1 = Q[2 * e + 1] * qs;
+            if (qbad) x0 = x1 = 0.f;
+            q2 = fmaf(x0, x0, fmaf(x1, x1, q2));
+            split2(x0, x1, &hi[e], &lo[e]);
+          }
+          tmem_st32(row + half * 32, hi);
+          tmem_st32(row + 32 * KT + half * 32, lo);
+        }
+        uq_s[c & 1][j] = q2 > 0.f ? norm_exponent(q2) : 0;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar_q);
+      } else if constexpr (KT == 1) {
+        int64_t tn;
+        const bool next_in = at(c + 1, &tn);
+        load64(B, kb + tn, T, Dk, next_in);
+      }
+    };
+    float A[64], B[64];
+    if constexpr (KT == 1) {
+      int64_t tt;
+      const bool in = at(0, &tt);
+      load64(A, kb + tt, T, Dk, in);
+    }
+    for (int c = 0; c < nc; c += 2) {
+      chunk(c, A, B);
+      if (c + 1 < nc) chunk(c + 1, B, A);
+    }
+  } else if (warp < 8) {
+    // ---------------- scores -> P, state, output: thread = step i, or (column e, half of Dk) ----------------
+    regs_inc<kRegsSoft>();
+    const int l = tid - 128;
+    const int e = l & 63, half = l >> 6;
+    constexpr int NSt = 32 * KT;                 // state elements per thread: d = half * NSt ...
+    const uint32_t trow = tmem + ((uint32_t)((warp - 4) * 32) << 16);
+    float St[NSt];
+    {
+      const float* src = nullptr;
+      int64_t rs = 0, cs = 0;
+      if (seg == 0) {
+        if (w.s_in) { src = w.s_in + head * (int64_t)Dk * w.Dv; rs = w.s_row; cs = w.s_col; }
+      } else if (FULL) {
+        src = args.seg[wi] + ((int64_t)(seg - 1) * args.heads + head) * Dk * w.Dv; rs = w.Dv; cs = 1;
+      }
+#pragma unroll
+      for (int i = 0; i < NSt; ++i) {
+        const int d = half * NSt + i;
+        St[i] = (src && d < Dk && e < ne) ? src[d * rs + (int64_t)(e0 + e) * cs] : 0.f;
+      }
+    }
+    // the state as the B operand [e][d] of the read-out, one exponent per row
+    auto publish = [&](int slot) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < NSt; ++i) top = fmaxf(top, fabsf(St[i]));
+      top_s[l] = top;
+      bar_sync(2, 128);
+      top = fmaxf(top, top_s[l ^ 64]);
+      const int se = min(fit_exponent(top), 113);
+      const float s = p2(-se);
+      if (half == 0) scale_s[slot][e] = p2(se);
+      const uint32_t tile = sbase + (KT == 2 ? half * 8192 : 0);
+#pragma unroll
+      for (int c = 0; c < NSt / 8; ++c) {
+        uint32_t h[4], lo[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) split2(St[8 * c + 2 * x] * s, St[8 * c + 2 * x + 1] * s, &h[x], &lo[x]);
+        const int chunk = (KT == 1 ? half * 4 : 0) + c;
+        const uint32_t at = tile + (uint32_t)(e * 128 + ((chunk ^ (e & 7)) << 4));
+        sts128(at, h[0], h[1], h[2], h[3]);
+        sts128(at + KT * 8192, lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async();
+    };
+    if (FULL) publish(0);
+    mbar_arrive(bar_s);
+
+    for (int c = 0; c < nc; ++c) {
+      const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
+      int qe = 0, m = 0;
+      if constexpr (FULL) {
+        const uint32_t sp = trow + S_::sp + (uint32_t)(c % NSP) * 128u;
+        wait_or_dead(bar_sp + 8 * (c % NSP), (uint32_t)(c / NSP) & 1u, dead);
+        tc_fence_after();
+        qe = qe_s[c & 1][l];
+        m = m_s[c & 1][l] + uq_s[c & 1][l] - 15; // P is held as its multiple of 2^m, at most 2^15
+        const int off = 127 - m;                 // exponent field of 2^(fg - m)
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+          uint32_t hi[16], lo[16];
+          if (g * 32 <= (l | 31)) {
+            uint32_t r[32];
+            tmem_ld32(sp + g * 32, r);
+            tmem_ld_wait();
+            const float* pw = &pow_pad[32 + l - g * 32];
+#pragma unroll
+            for (int jj = 0; jj < 32; jj += 4) {
+              const int4 f4 = *reinterpret_cast<const int4*>(&fg_s[c & 1][g * 32 + jj]);
+              const int fs[4] = {f4.x, f4.y, f4.z, f4.w};
+              float x[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int ex = min(max(fs[u] + off, 0), 254);
+                x[u] = __uint_as_float(r[jj + u]) * pw[-(jj + u)] * __int_as_float(ex << 23);
+              }
+              split2(x[0], x[1], &hi[jj / 2], &lo[jj / 2]);
+              split2(x[2], x[3], &hi[jj / 2 + 1], &lo[jj / 2 + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) hi[x] = lo[x] = 0u;
+          }
+          tmem_st16(sp + g * 32, hi);
+          tmem_st16(sp + g * 32 + 16, lo);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar_p);
+      }
+      // the state after the chunk
+      wait_or_dead(bar_ds, (uint32_t)c & 1u, dead);
+      tc_fence_after();
+      {
+        const Factors mw = p2_wide(mw_s[c & 3]);
+        const float carry = pow_pad[32 + len];
+        // rows 0-63 of the accumulator come from the hi half of v, rows 64-127 from the lo half: each
+        // thread adds the other's to its own half of the columns (exchanged where the published state lay)
+        const uint32_t mine = trow + S_::ds + (uint32_t)half * NSt, other = trow + S_::ds + (uint32_t)(half ^ 1) * NSt;
+        const uint32_t ex_row = sbase + (uint32_t)(l ^ 64) * (NSt * 4), my_row = sbase + (uint32_t)l * (NSt * 4);
+#pragma unroll
+        for (int b = 0; b < NSt; b += 32) {
+          uint32_t r[32];
+          tmem_ld32(other + b, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            sts128(ex_row + (uint32_t)(((b / 4 + x) ^ (l & 7)) << 4), r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]);
+        }
+        bar_sync(2, 128);
+#pragma unroll
+        for (int b = 0; b < NSt; b += 32) {
+          uint32_t r[32];
+          tmem_ld32(mine + b, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            float y[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3])
+                         : "r"(my_row + (uint32_t)(((b / 4 + x) ^ (l & 7)) << 4)));
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              St[b + 4 * x + u] = fmaf(carry, St[b + 4 * x + u],
+                                       (__uint_as_float(r[4 * x + u]) + y[u]) * mw.a * mw.b);
+          }
+        }
+        tc_fence_before();
+        if (FULL && c + 1 < nc) publish((c + 1) & 1);      // its barrier also ends the exchange
+        else bar_sync(2, 128);
+        mbar_arrive(bar_s);
+      }
+      if constexpr (FULL) {
+        const int64_t t = (c0 + c) * kL + l;
+        const int64_t tt = w.reverse ? T - 1 - t : t;
+        float* out = w.o + (head * (int64_t)w.Dv + e0) * T + tt;
+        const bool live = t < T;
+        const Factors fi = p2_wide((qe == 0x7fffffff ? 0 : qe) + m);
+        const Factors fx = p2_wide(qe == 0x7fffffff ? 0 : qe);
+        const float nan = __int_as_float(0x7fffffff);
+        const float ia = qe == 0x7fffffff ? nan : fi.a, ib = fi.b;
+        const float xa = fx.a, xb = fx.b * pow_pad[32 + l + after];
+        wait_or_dead(bar_o, (uint32_t)c & 1u, dead);
+        tc_fence_after();
+        const bool poisoned = *any_poison != 0;
+#pragma unroll
+        for (int b = 0; b < 64; b += 32) {
+          uint32_t ri[32], rx[32];
+          tmem_ld32(trow + S_::oi + b, ri);
+          tmem_ld32(trow + S_::ox + b, rx);
+          tmem_ld_wait();
+          if (b == 32) {
+            tc_fence_before();
+            mbar_arrive(bar_ofree);
+          }
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            float y = __uint_as_float(ri[x]) * ia * ib + __uint_as_float(rx[x]) * xa * (xb * scale_s[c & 1][b + x]);
+            if (poisoned && poison_s[b + x] <= (int)t) y = nan;
+            if (live && b + x < ne) out[(int64_t)(b + x) * T] = y;
+          }
+        }
+      }
+    }
+    // the state after the last chunk
+    float* dst = nullptr;
+    int64_t rs = 0, cs = 0;
+    if (!FULL) {
+      dst = args.seg[wi] + ((int64_t)seg * args.heads + head) * Dk * w.Dv; rs = w.Dv; cs = 1;
+    } else if (seg == args.nseg - 1 && w.s_out) {
+      dst = w.s_out + head * (int64_t)Dk * w.Dv; rs = w.s_row; cs = w.s_col;
+    }
+    if (dst && e < ne) {
+      const bool bad = poison_s[e] != 0x7fffffff;
+#pragma unroll
+      for (int i = 0; i < NSt; ++i) {
+        const int d = half * NSt + i;
+        if (d < Dk) dst[d * rs + (int64_t)(e0 + e) * cs] = bad ? __int_as_float(0x7fffffff) : St[i];
+      }
+    }
+  } else {
+    regs_dec<kRegsMma>();
+    if (tid == 256) {
+    // ---------------- MMAs ----------------
+    constexpr uint32_t id_scores = idesc_f16(kL), id_inter = idesc_f16(64), id_intra = idesc_f16(64) | kBMajorMN,
+                       id_grow = idesc_f16(64 * KT) | kAMajorMN | kBMajorMN;
+    const uint32_t tq = tmem + S_::q, toi = tmem + S_::oi, tox = tmem + S_::ox, tds = tmem + S_::ds;
+    bool ok = true;
+    auto stage_of = [&](int c) { return base + (uint32_t)(c % NS) * S_::stage_bytes; };
+    auto scores = [&](int c) {
+      ok = wait_or_dead(bar_q, (uint32_t)c & 1u, dead) && ok;
+      ok = wait_or_dead(bar_kv + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t k_hi = stage_of(c), k_lo = k_hi + KT * kTileB, d = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
+#pragma unroll
+      for (int s = 0; s < 4 * KT; ++s) {
+        const uint32_t at = (uint32_t)((s >> 2) * kTileB + (s & 3) * 32);
+        mma_f16_ts(d, tq + s * 8, desc_lo(k_hi + at), id_scores, s > 0);
+        mma_f16_ts(d, tq + 32 * KT + s * 8, desc_lo(k_hi + at), id_scores, 1u);
+        mma_f16_ts(d, tq + s * 8, desc_lo(k_lo + at), id_scores, 1u);
+      }
+      umma_commit(bar_sp + 8 * (c % NSP));
+      mbar_arrive(bar_sp + 8 * (c % NSP));   // hands on what the loaders wrote beside the operands
+    };
+    if (FULL) scores(0);
+    for (int c = 0; c < nc && ok; ++c) {
+      const uint32_t stage = stage_of(c);
+      const uint32_t k_hi = stage, k_lo = stage + KT * kTileB, v_hi = stage + 2 * KT * kTileB, v_lo = v_hi + kTileB,
+                     vw_hi = v_lo + kTileB;
+      ok = wait_or_dead(bar_s, (uint32_t)c & 1u, dead) && ok;
+      if (FULL) {
+        if (c >= 1) ok = wait_or_dead(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
+      } else {
+        ok = wait_or_dead(bar_kv + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+      }
+      if (!ok) break;
+      tc_fence_after();
+      if (FULL) {
+#pragma unroll
+        for (int s = 0; s < 4 * KT; ++s) {
+          const uint32_t at = sbase + (uint32_t)((s >> 2) * 8192 + (s & 3) * 32);
+          mma_f16_ts(tox, tq + s * 8, desc_lo(at), id_inter, s > 0);
+          mma_f16_ts(tox, tq + 32 * KT + s * 8, desc_lo(at), id_inter, 1u);
+          mma_f16_ts(tox, tq + s * 8, desc_lo(at + KT * 8192), id_inter, 1u);
+        }
+        umma_commit(bar_qfree);
+      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        mma_f16_ss(tds, desc_mn(vw_hi + s * 2048), desc_mn(k_hi + s * 2048), id_grow, s > 0);
+        mma_f16_ss(tds, desc_mn(vw_hi + s * 2048), desc_mn(k_lo + s * 2048), id_grow, 1u);
+      }
+      umma_commit(bar_ds);
+      mbar_arrive(bar_ds);
+      if (!FULL) {
+        umma_commit(bar_free + 8 * (c % NS));
+        continue;
+      }
+      if (NSP == 2 && c + 1 < nc) scores(c + 1);
+      ok = wait_or_dead(bar_p, (uint32_t)c & 1u, dead) && ok;
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t sp = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const uint32_t p_hi = sp + (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
+        mma_f16_ts(toi, p_hi, desc_mn(v_hi + s * 2048), id_intra, s > 0);
+        mma_f16_ts(toi, p_hi + 16, desc_mn(v_hi + s * 2048), id_intra, 1u);
+        mma_f16_ts(toi, p_hi, desc_mn(v_lo + s * 2048), id_intra, 1u);
+      }
+      umma_commit(bar_o);
+      umma_commit(bar_free + 8 * (c % NS));
+      if (NSP == 1 && c + 1 < nc) scores(c + 1);
+    }
+    umma_commit(bar_end);          // everything issued has landed before tensor memory is given back
+    if (!mbar_wait(bar_end, 0)) *dead = 1;
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*dead && tid == 0) dev_flag(args.status, SB_DEV_TMA_TIMEOUT);
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// States after each segment from their growths: seg[s] += r^(steps of segment s) seg[s - 1].
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs args, int nwalks) {
+  for (int wi = 0; wi < nwalks; ++wi) {
+    const Walk& w = args.w[wi];
+    const int64_t per = (int64_t)w.Dk * w.Dv, total = per * args.heads;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+      const int64_t head = i / per;
+      double b = 1.0 - (double)w.decay[w.n_decay > 1 ? head % w.n_decay : 0] / 4096.0, p = 1.0;
+      for (int64_t n = (int64_t)args.seg_chunks * kL; n; n >>= 1) {
+        if (n & 1) p *= b;
+        b *= b;
+      }
+      const float r = (float)p;
+      float* s = args.seg[wi] + i;
+      float x = *s;
+      for (int g = 1; g < args.nseg - 1; ++g) {
+        s += total;
+        x = fmaf(r, x, *s);
+        *s = x;
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// Segments the axis is cut into: `ctas` CTAs per segment walk `chunks` chunks.  The fewest waves of
+// (segments x chunks) win; a cut axis is walked by the first launch too, at about half the cost of a
+// chunk, and every CTA pays about two chunks to fill and drain.
+int plan_segments(int64_t ctas, int64_t chunks) {
+  const int64_t sms = sm_count();
+  int best = 1;
+  double best_cost = 0;
+  for (int64_t n = 1; n <= chunks && n <= 256; ++n) {
+    const int64_t per = (chunks + n - 1) / n;
+    if ((chunks + per - 1) / per != n) continue;       // the same cut as a smaller n
+    double cost = (double)((ctas * n + sms - 1) / sms) * (double)(per + 2);
+    if (n > 1) cost += (double)((ctas * (n - 1) + sms - 1) / sms) * (0.5 * (double)per + 2) + 4;
+    if (n == 1 || cost < best_cost) { best = (int)n; best_cost = cost; }
+    if (ctas * n > 16 * sms) break;
+  }
+  return best;
+}
+
+int64_t tc_scratch_floats(const Walk* walks, int n) {
+  int64_t ctas = 0, floats = 0;
+  for (int i = 0; i < n; ++i) ctas += walks[i].heads * ((walks[i].Dv + 63) / 64);
+  const int nseg = plan_segments(ctas, (walks[0].T + kL - 1) / kL);
+  if (nseg > 1)
+    for (int i = 0; i < n; ++i) floats += (int64_t)(nseg - 1) * walks[i].heads * walks[i].Dk * walks[i].Dv;
+  return floats;
+}
+
+template <int KT>
+static int go(const TcArgs& a, cudaStream_t s) {
+  constexpr int smem = Shape<KT>::smem;
+  SB_CUDA(cudaFuncSetAttribute(attention_tc_kernel<KT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t ctas = a.heads * a.nsub;
+  SB_REQUIRE(ctas * a.nseg < (1LL << 31), "geometry too large");
+  if (a.nseg > 1) {
+    SB_CUDA(cudaFuncSetAttribute(attention_tc_kernel<KT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attention_tc_kernel<KT, false><<<(unsigned)(ctas * (a.nseg - 1)), kThreads, smem, s>>>(a);
+    SB_CUDA(cudaGetLastError());
+  }
+  return SB_OK;
+}
+
+// Walks of one launch: the same heads and T, Dk on the same side of 64.
+int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
+  TcArgs a{};
+  int64_t ctas = 0;
+  a.nsub = 0;
+  for (int i = 0; i < n; ++i) {
+    a.w[i] = walks[i];
+    for (int e0 = 0; e0 < walks[i].Dv; e0 += 64) {
+      a.sub_walk[a.nsub] = i;
+      a.sub_e0[a.nsub++] = e0;
+    }
+  }
+  a.heads = walks[0].heads;
+  ctas = a.heads * a.nsub;
+  const int64_t chunks = (walks[0].T + kL - 1) / kL;
+  a.nseg = plan_segments(ctas, chunks);
+  a.seg_chunks = (int)((chunks + a.nseg - 1) / a.nseg);
+  if (a.nseg > 1) {
+    float* p = scratch;
+    for (int i = 0; i < n; ++i) {
+      a.seg[i] = p;
+      p += (int64_t)(a.nseg - 1) * a.heads * walks[i].Dk * walks[i].Dv;
+    }
+  }
+  a.status = status_ptr();
+  if (!a.status) return SB_ERR_CUDA;
+  const bool wide = walks[0].Dk > 64;
+  if (wide) SB_TRY(go<2>(a, s));
+  else SB_TRY(go<1>(a, s));
+  if (a.nseg > 2) {
+    int64_t most = 0;
+    for (int i = 0; i < n; ++i) {
+      const int64_t total = a.heads * walks[i].Dk * walks[i].Dv;
+      most = total > most ? total : most;
+    }
+    const int64_t blocks = (most + 255) / 256;
+    join_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(a, n);
+    SB_CUDA(cudaGetLastError());
+  }
+  const unsigned grid = (unsigned)(ctas * a.nseg);
+  if (wide) attention_tc_kernel<2, true><<<grid, kThreads, Shape<2>::smem, s>>>(a);
+  else attention_tc_kernel<1, true><<<grid, kThreads, Shape<1>::smem, s>>>(a);
+  SB_CUDA(cudaGetLastError());
+  return SB_OK;
+}
+
+}  // namespace la
+}  // namespace sb

@@ -27,5 +27,10 @@ struct Walk {
   int after;            // the state decays before a step is added (1) or after it has been read (0)
 };
 
+// Tensor-core walks (api_linear_attention_tc.cu): one launch for n <= 3 walks over the same heads and
+// steps whose Dk lie on the same side of 64, with tc_scratch_floats() floats of scratch.
+int64_t tc_scratch_floats(const Walk* walks, int n);
+int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s);
+
 }  // namespace la
 }  // namespace sb

@@ -9,6 +9,15 @@ Tolerances (derived, used by the tests of every kernel):
   roundings of splits, weights and scales, each at most 2^-23 (half a step, 2^-24, for an fp32
   operation; a whole one for the tensor cores' truncating sums):
   ``tol = 2^-23 (Dk + 128 + 3 min(T, 1 / (1 - r)) + 32)``.
+  The chunked kernel splits each vector (q, k, v of a step, a row of scores, a row of the state) into
+  fp16 pairs: an element is held to 22 bits, or to 2^-25 (half of fp16's smallest step) where that is
+  more.  What the second case can add, against sums over the vectors' LARGEST magnitudes q', k', v' (a
+  score then is Dk q' k'): q, k, v and state rows are scaled to a largest element of at least 2^13,
+  2^-38 relative to it each.  A row of scores is scaled by 2^(15 - u), 2^u >= |q_i| max_j |k_j| r^(i-j)
+  2^g_j with u at most 3 too large (three roundings up to a power of two), v to at most 2^14 = 2^-g v':
+  2^-25 2^14 2^(u - 15) <= 2^-36 of the largest term, for each of up to 128 terms: 2^-29.  The state's
+  growth is a sum of 128 such terms as well, 2^-37 of the largest each.  Together below 2^-28
+  (``attention_floor``).
 * dense and dropout: the sums are whole numbers and the products are rounded in a stated order, so
   the results are compared bit for bit.
 """
@@ -57,13 +66,31 @@ def attention_tol(dk, T, decay):
     return 2.0 ** -23 * (dk + 128 + 3 * remembered + 32)
 
 
-def assert_sum_close(got, want, scale, tol, what=''):
+def attention_floor(q, k, v, decay, state=None):
+    """What the smallest step of an fp16 pair can add up to: the sums (output, state) over the largest
+    magnitudes of each step's vectors, times 2^-28."""
+    def top(a):
+        return np.abs(a).max(axis=2, keepdims=True) + np.zeros_like(a)
+    s = None if state is None else np.abs(state).max(axis=(2, 3), keepdims=True) + np.zeros_like(state)
+    o, f = attention(top(q), top(k), top(v), decay, s)
+    return 2.0 ** -28 * o, 2.0 ** -28 * f
+
+
+def attention_grads_floor(q, k, v, decay, state, go, gf):
+    def top(a):
+        return np.abs(a).max(axis=2, keepdims=True) + np.zeros_like(a)
+    def whole(a):
+        return None if a is None else np.abs(a).max(axis=(2, 3), keepdims=True) + np.zeros_like(a)
+    return [2.0 ** -28 * g for g in attention_grads(top(q), top(k), top(v), decay, whole(state), top(go), whole(gf))]
+
+
+def assert_sum_close(got, want, scale, tol, what='', floor=0.0):
     got = got.detach().cpu().numpy().astype(np.float64)
     assert got.shape == want.shape, f'{what}: shape {got.shape} vs {want.shape}'
     if got.size == 0:
         return
     assert np.isfinite(got).all(), f'{what}: non-finite values'
-    err, lim = np.abs(got - want), tol * scale + 1e-37
+    err, lim = np.abs(got - want), tol * scale + floor + 1e-37
     assert (err <= lim).all(), f'{what}: worst ratio to the bound {np.max(err / lim):.3g}'
 
 

@@ -35,9 +35,10 @@ def check_walk(arrays, out, final, T):
     tol = O.attention_tol(q.shape[2], T, decay)
     want, ws = O.attention(q, k, v, decay, s)
     size, ss = O.attention(*(np.abs(a) for a in (q, k, v)), decay, None if s is None else np.abs(s))
-    O.assert_sum_close(out, want, size, tol, 'output')
+    fo, fs = O.attention_floor(*arrays)
+    O.assert_sum_close(out, want, size, tol, 'output', fo)
     if final is not None:
-        O.assert_sum_close(final, ws, ss, tol, 'state')
+        O.assert_sum_close(final, ws, ss, tol, 'state', fs)
 
 
 SHAPES = [   # n, h, dk, dv, T
@@ -74,8 +75,9 @@ def test_attention_backward(cuda, shape, ends):
     size = O.attention_grads(*(np.abs(a) for a in (q, k, v)), decay, None if s is None else np.abs(s), np.abs(go),
                              None if gf is None else np.abs(gf))
     tol = O.attention_tol(max(shape[2:4]), shape[4], decay)
-    for name, g, w, z in zip(('query', 'key', 'value', 'state'), grads, want, size):
-        O.assert_sum_close(g, w, z, tol, name)
+    floor = O.attention_grads_floor(q, k, v, decay, s, go, gf)
+    for name, g, w, z, f in zip(('query', 'key', 'value', 'state'), grads, want, size, floor):
+        O.assert_sum_close(g, w, z, tol, name, f)
 
 
 def test_attention_gradient_against_differences(cuda):
@@ -115,8 +117,9 @@ def test_attention_decays(cuda, decay):
     grads = torch.autograd.grad(attention.dynamics(*leaves, dev(arrays[3])), leaves, dev(go))
     want = O.attention_grads(*arrays[:4], None, go, None)
     size = O.attention_grads(*(np.abs(a) for a in arrays[:3]), arrays[3], None, np.abs(go), None)
-    for g, w, z in zip(grads, want, size):
-        O.assert_sum_close(g, w, z, O.attention_tol(24, 400, arrays[3]))
+    floor = O.attention_grads_floor(*arrays[:4], None, go, None)
+    for g, w, z, f in zip(grads, want, size, floor):
+        O.assert_sum_close(g, w, z, O.attention_tol(24, 400, arrays[3]), '', f)
 
 
 def test_attention_of_sizes_far_apart(cuda):
@@ -154,7 +157,8 @@ def test_attention_values_that_are_not_finite(cuda, which, bad):
     size, _ = O.attention(*(np.abs(a.cpu().numpy()) for a in clean[:3]), arrays[3], np.abs(arrays[4]))
     diff = (got - want).abs().double().cpu().numpy()
     mask = expect.cpu().numpy()
-    assert (diff[mask] <= 2 * tol * size[mask]).all()
+    floor, _ = O.attention_floor(*(a.cpu().numpy() for a in clean))
+    assert (diff[mask] <= 2 * (tol * size + floor)[mask]).all()
 
 
 def test_attention_in_pieces_and_steps(cuda):
