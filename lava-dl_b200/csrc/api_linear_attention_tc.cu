@@ -30,11 +30,15 @@
 // two MMAs cover the three products).  q goes to tensor memory (it is A of two products) and so does P,
 // converted in place of the scores.
 //
-// Roles of a CTA (one per SM; 384 threads): warps 0-3 load and convert (one step per thread), warps 4-7
-// turn scores into P, keep the state (32 elements per thread and 64 of Dk in registers, fp32), and write
-// the output, warp 8 issues the MMAs.  A head with T steps is one CTA, or several when there are fewer
-// heads than SMs: the axis is then cut into segments, a first launch takes each segment's growth from
-// zero, a small one joins them, and the walk starts every segment from its own state.
+// Roles of a CTA (one per SM, six warpgroups): k, v and q are each loaded and converted by a warpgroup
+// (one step per thread), one turns scores into P, one keeps the state (32 elements per thread and 64 of
+// Dk in registers, fp32) and writes the output, and one thread issues the MMAs.  An earlier form with one
+// loading warpgroup that held two operands at a time in 232 registers ran at 15.3 us per chunk of
+// [128 x 64]: 6650 instructions per scheduler in straight-line code that missed the instruction cache.
+//
+// A head with T steps is one CTA, or several when there are fewer heads than SMs: the axis is then cut
+// into segments, a first launch takes each segment's growth from zero, a small one joins them, and the
+// walk starts every segment from its own state.
 #include "linear_attention.cuh"
 #include "tc.cuh"
 
@@ -44,10 +48,14 @@ namespace {
 
 constexpr int kL = 128;                      // steps per chunk
 constexpr int kTileB = kL * 128;             // bytes of a [128 steps][64 channels] fp16 tile
-constexpr int kThreads = 384;
-// Registers per thread of the three warpgroups: 168 at launch (65536 / 384, in steps of 8), moved to where
-// the vectors live.  232 + 224 + 40 <= 3 * 168.
-constexpr int kRegsLoad = 232, kRegsSoft = 224, kRegsMma = 40;
+constexpr int kThreads = 768;
+// Registers per thread of the six warpgroups: 80 at launch (65536 / 768, in steps of 8), moved to where
+// the vectors live.  Each row adds up to 6 * 80.
+template <int KT>
+struct Regs {
+  static constexpr int k = 88, v = KT == 1 ? 96 : 88, q = 88, p = KT == 1 ? 96 : 80, s = KT == 1 ? 88 : 112, mma = 24;
+  static_assert(k + v + q + p + s + mma <= 480, "more registers than the block was launched with");
+};
 constexpr int kMaxSub = 6;
 
 struct TcArgs {
@@ -80,9 +88,10 @@ __device__ __forceinline__ Factors p2_wide(int n) {
   n = max(-252, min(n, 254));
   return Factors{p2(n >> 1), p2(n - (n >> 1))};
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+// largest magnitude of three, NaN if one is NaN
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) {
@@ -133,17 +142,29 @@ __device__ __forceinline__ uint32_t desc_mn(uint32_t saddr) {
   return ((saddr & 0x3ffffu) >> 4) | ((uint32_t)(kTileB >> 4) << 16);
 }
 
-// 64 rows of one step
-__device__ __forceinline__ void load64(float (&x)[64], const float* p, int64_t T, int rows, bool in) {
+// 64 rows of one step.  volatile: the loads stay where they are issued, in one batch ahead of the waits
+// and conversions (left to itself the compiler sinks them to their use).
+__device__ __forceinline__ void load64(float (&x)[64], const float* p, int64_t T, int rows, bool in, bool whole) {
+  if (whole && rows >= 64) {
 #pragma unroll
-  for (int d = 0; d < 64; ++d) {
-    x[d] = (in && d < rows) ? __ldg(p) : 0.f;
-    p += T;
+    for (int d = 0; d < 64; ++d) {
+      asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(x[d]) : "l"(p));
+      p += T;
+    }
+  } else {
+    const int n = in ? rows : 0;
+#pragma unroll
+    for (int d = 0; d < 64; ++d) {
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.nc.f32 %0, [%1];\n\t}"
+          : "=f"(x[d]) : "l"(p), "r"(n), "r"(d));
+      p += T;
+    }
   }
 }
 __device__ __forceinline__ float top64(const float (&x)[64], float m = 0.f) {
 #pragma unroll
-  for (int d = 0; d < 64; ++d) m = max_nan(m, fabsf(x[d]));
+  for (int d = 0; d < 64; d += 2) m = max_abs3(m, x[d], x[d + 1]);
   return m;
 }
 // Exponent that brings a largest magnitude into [2^13, 2^14); a zero vector gets one that no sum prefers.
@@ -193,26 +214,30 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   using S_ = Shape<KT>;
   constexpr int NS = S_::stages, NSP = S_::nsp;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(16) int fg_s[2][kL];
-  __shared__ int m_s[2][kL], qe_s[2][kL], uq_s[2][kL], kmax_s[2][4], mw_s[4];
+  // What travels beside the mantissas.  A slot of two is rewritten for chunk c + 2 once the read-out of
+  // chunk c has ended, a slot of four once the output of chunk c + 1 has been written.
+  __shared__ int f_s[2][kL], u_s[2][kL];                            // k: exponent, norm exponent
+  __shared__ __align__(16) float col_s[2][kL], colr_s[2][kL];       // of a column of P: 2^(fg - mc), that times r^(32 - j % 32)
+  __shared__ int mc_s[2], m_s[4][kL], qe_s[4][kL], uq_s[4][kL], mw_s[4];
   __shared__ float scan_s[2][4];
+  __shared__ int kmax_s[2][8];
   __shared__ float pow_pad[32 + kL + 1];       // r^n at 32 + n; zeros before it are the causal mask
   __shared__ float scale_s[2][64];
   __shared__ float top_s[kL];
   __shared__ int poison_s[64];
   __shared__ int any_poison_s, dead_s;
   __shared__ uint32_t tmem_s;
-  __shared__ __align__(8) uint64_t bars[2 + 2 + 2 + 9];
+  __shared__ __align__(8) uint64_t bars[20];
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = tid >> 7, th = tid & 127, tw = warp & 3;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t sbase = base + NS * S_::stage_bytes;
   volatile int* dead = &dead_s;
   volatile int* any_poison = &any_poison_s;
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t bar_kv = bar0, bar_free = bar0 + 16, bar_sp = bar0 + 32;
-  const uint32_t bar_q = bar0 + 48, bar_qfree = bar0 + 56, bar_p = bar0 + 64, bar_ds = bar0 + 72, bar_s = bar0 + 80,
-                 bar_o = bar0 + 88, bar_ofree = bar0 + 96, bar_end = bar0 + 104;
+  const uint32_t bar_k = bar0, bar_v = bar0 + 16, bar_free = bar0 + 32, bar_sp = bar0 + 48, bar_kx = bar0 + 64;   // two each
+  const uint32_t bar_q = bar0 + 80, bar_qfree = bar0 + 88, bar_p = bar0 + 96, bar_ds = bar0 + 104, bar_s = bar0 + 112,
+                 bar_o = bar0 + 120, bar_ofree = bar0 + 128, bar_end = bar0 + 136;
 
   // which head, segment, walk and columns
   const int64_t bid = blockIdx.x;
@@ -224,22 +249,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   const int64_t T = w.T;
   const int Dk = w.Dk, ne = min(64, w.Dv - e0);
   const int64_t c0 = (int64_t)seg * args.seg_chunks;
-  const int64_t call = (T + kL - 1) / kL;
-  const int nc = (int)min((int64_t)args.seg_chunks, call - c0);
+  const int nc = (int)min((int64_t)args.seg_chunks, (T + kL - 1) / kL - c0);
   const int after = w.after;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar_kv + 8 * i, 128);
+      mbar_init(bar_k + 8 * i, 128);
+      mbar_init(bar_v + 8 * i, 128);
       mbar_init(bar_free + 8 * i, 1);
       mbar_init(bar_sp + 8 * i, 2);
+      mbar_init(bar_kx + 8 * i, 128);
     }
     mbar_init(bar_q, 128);
     mbar_init(bar_qfree, 1);
     mbar_init(bar_p, 128);
     mbar_init(bar_ds, 2);
     mbar_init(bar_s, 128);
-    mbar_init(bar_o, 1);
+    mbar_init(bar_o, 2);
     mbar_init(bar_ofree, 128);
     mbar_init(bar_end, 1);
     fence_mbar_init();
@@ -257,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     }
     pow_pad[32 + tid] = (float)p;
   }
-  if (warp == 8) {
+  if (role == 5 && tw == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -266,183 +292,246 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
+  const uint32_t trow = tmem + ((uint32_t)(tw * 32) << 16);   // this warp's lanes of tensor memory
 
-  if (warp < 4) {
-    // ---------------- load and convert: thread = step of the chunk ----------------
-    regs_inc<kRegsLoad>();
-    const int j = tid;
-    // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
-    const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
+  // a thread's step of chunk c, walked in the CTA's direction: memory index, inside the axis, chunk complete
+  auto step_at = [&](int c, int64_t* tt, bool* whole) {
+    const int64_t t = (c0 + c) * kL + th;
+    *tt = w.reverse ? T - 1 - t : t;
+    *whole = (c0 + c + 1) * kL <= T;
+    return t < T;
+  };
+
+  if (role == 0) {
+    // ---------------- k ----------------
+    regs_inc<Regs<KT>::k>();
     const float* kb = w.k + head * (int64_t)Dk * T;
-    const float* qb = FULL ? w.q + head * (int64_t)Dk * T : nullptr;
-    const float* vb = w.v + (head * (int64_t)w.Dv + e0) * T;
-    auto at = [&](int c, int64_t* tt) {
-      const int64_t t = (c0 + c) * kL + j;
-      *tt = w.reverse ? T - 1 - t : t;
-      return c < nc && t < T;
-    };
-    // One chunk; A holds k (KT = 1) on entry and B the next chunk's k on exit.  The loads of an operand
-    // are issued as soon as the registers it needs have been converted.
-    auto chunk = [&](int c, float (&A)[64], float (&B)[64]) {
-      const int st = c % NS;
-      const uint32_t stage = base + st * S_::stage_bytes;
-      const uint32_t k_hi = stage, k_lo = stage + KT * kTileB, v_hi = stage + 2 * KT * kTileB, v_lo = v_hi + kTileB,
-                     vw_hi = v_lo + kTileB, vw_lo = vw_hi + kTileB;
-      const int64_t t = (c0 + c) * kL + j;
-      const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
+#pragma unroll 1
+    for (int c = 0; c < nc; ++c) {
+      const uint32_t k_hi = base + (c % NS) * S_::stage_bytes, k_lo = k_hi + KT * kTileB;
       int64_t tt;
-      const bool in = at(c, &tt);
-      if constexpr (KT == 1) {
-        load64(B, vb + tt, T, ne, in);
-      } else {
-        load64(A, kb + tt, T, 64, in);
-        load64(B, kb + 64 * T + tt, T, Dk - 64, in);
+      bool whole;
+      const bool in = step_at(c, &tt, &whole);
+      float x[64];
+      load64(x, kb + tt, T, Dk, in, whole);
+      float top = top64(x);
+      if constexpr (KT == 2) {     // the second half stays, the first is fetched again once the exponent is known
+        load64(x, kb + 64 * T + tt, T, Dk - 64, in, whole);
+        top = top64(x, top);
       }
-      // k
-      float top = top64(A);
-      if constexpr (KT == 2) top = top64(B, top);
-      bool spoilt = false;
-      if (not_finite(top)) {   // every column is spoilt from this step on
-        spoilt = true;
-#pragma unroll
-        for (int d = 0; d < 64; ++d) {
-          A[d] = 0.f;
-          if constexpr (KT == 2) B[d] = 0.f;
-        }
-        for (int e = 0; e < 64; ++e) atomicMin(&poison_s[e], (int)t);
-        any_poison_s = 1;
+      bool spoilt = not_finite(top);
+      if (spoilt) {                // every column of the output is spoilt from this step on
         top = 0.f;
+        for (int e = 0; e < 64; ++e) atomicMin(&poison_s[e], (int)((c0 + c) * kL + th));
+        any_poison_s = 1;
+#pragma unroll
+        for (int d = 0; d < 64; ++d) x[d] = 0.f;
       }
       const int f = fit_exponent(top);
-      int fg = top > 0.f ? f : kNoTerm;
-      if (c >= NS) wait_or_dead(bar_free + 8 * st, (uint32_t)(c / NS - 1) & 1u, dead);
-      float n2 = store_row<true>(A, p2(-f), k_hi, k_lo, j);
+      if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+      float n2;
       if constexpr (KT == 2) {
-        n2 += store_row<true>(B, p2(-f), k_hi + kTileB, k_lo + kTileB, j);
-        load64(A, vb + tt, T, ne, in);
-      } else if (FULL) {
-        load64(A, qb + tt, T, Dk, in);
+        n2 = store_row<true>(x, p2(-f), k_hi + kTileB, k_lo + kTileB, th);
+        load64(x, kb + tt, T, 64, in && !spoilt, whole && !__any_sync(0xffffffffu, spoilt));
+        n2 += store_row<true>(x, p2(-f), k_hi, k_lo, th);
+      } else {
+        n2 = store_row<true>(x, p2(-f), k_hi, k_lo, th);
       }
-      // v
-      float(&V)[64] = KT == 1 ? B : A;
-      float vtop = top64(V);
-      if (spoilt || not_finite(vtop)) {
-        vtop = 0.f;
+      f_s[c & 1][th] = top > 0.f ? f : kNoTerm - (spoilt ? 1 : 0);
+      u_s[c & 1][th] = norm_exponent(n2);
+      mbar_arrive(bar_kx + 8 * (c & 1));
+      fence_proxy_async();
+      mbar_arrive(bar_k + 8 * (c % NS));
+    }
+  } else if (role == 1) {
+    // ---------------- v, and what P and the growth need to know of the steps ----------------
+    regs_inc<Regs<KT>::v>();
+    // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
+    const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
+    const float* vb = w.v + (head * (int64_t)w.Dv + e0) * T;
+    const int j = th;
+#pragma unroll 1
+    for (int c = 0; c < nc; ++c) {
+      const uint32_t v_hi = base + (c % NS) * S_::stage_bytes + 2 * KT * kTileB, v_lo = v_hi + kTileB,
+                     vw_hi = v_lo + kTileB, vw_lo = vw_hi + kTileB;
+      const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
+      int64_t tt;
+      bool whole;
+      const bool in = step_at(c, &tt, &whole);
+      float x[64];
+      load64(x, vb + tt, T, ne, in, whole);
+      float top = top64(x);
+      wait_or_dead(bar_kx + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
+      const int f = f_s[c & 1][j], u = u_s[c & 1][j];
+      const bool spoilt = f == kNoTerm - 1;
+      if (spoilt || not_finite(top)) {
+        if (!spoilt) {
+          for (int e = 0; e < ne; ++e)
+            if (not_finite(fabsf(vb[(int64_t)e * T + tt]))) atomicMin(&poison_s[e], (int)((c0 + c) * kL + j));
+          any_poison_s = 1;
+        }
+        top = 0.f;
 #pragma unroll
         for (int e = 0; e < 64; ++e) {
-          if (spoilt) V[e] = 0.f;
-          if (not_finite(fabsf(V[e]))) {
-            V[e] = 0.f;
-            atomicMin(&poison_s[e], (int)t);
-            any_poison_s = 1;
-          }
-          vtop = fmaxf(vtop, fabsf(V[e]));
+          if (spoilt || not_finite(fabsf(x[e]))) x[e] = 0.f;
+          top = fmaxf(top, fabsf(x[e]));
         }
       }
-      const int g = fit_exponent(vtop);
-      fg = (vtop > 0.f && fg != kNoTerm) ? fg + g : kNoTerm;
-      // weight of the step in the state, and the largest exponents: of the steps so far, of the weighted all
+      const int g = fit_exponent(top);
+      const int fg = (top > 0.f && f > kNoTerm) ? f + g : kNoTerm;
+      // weight of the step in the state, and the largest exponents: of all steps, of the weighted ones
       const float wt = (j < len) ? pow_pad[32 + len - after - j] : 0.f;
       const int we = (int)((__float_as_uint(wt) >> 23) & 0xff) - 127;
       const int key = wt != 0.f && fg != kNoTerm ? fg + we : kNoTerm;
       // running maximum of log2(2^fg |k_j|) + (i - j) log2 r: the scan runs on that less i log2 r
-      float mk = fg == kNoTerm ? -1e30f : (float)(fg + norm_exponent(n2)) - (float)j * slope;
+      float mk = fg == kNoTerm ? -1e30f : (float)(fg + u) - (float)j * slope;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const float up = __shfl_up_sync(0xffffffffu, mk, o);
         if (lane >= o) mk = fmaxf(mk, up);
       }
-      const int kmax = __reduce_max_sync(0xffffffffu, key);
+      const int kmax = __reduce_max_sync(0xffffffffu, key), fmax = __reduce_max_sync(0xffffffffu, fg);
       if (lane == 31) {
-        scan_s[c & 1][warp] = mk;
-        kmax_s[c & 1][warp] = kmax;
+        scan_s[c & 1][tw] = mk;
+        kmax_s[c & 1][tw] = kmax;
+        kmax_s[c & 1][4 + tw] = fmax;
       }
       bar_sync(1, 128);
-      int mw = kNoTerm;
+      int mw = kNoTerm, mc = kNoTerm;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (i < warp) mk = fmaxf(mk, scan_s[c & 1][i]);
+        if (i < tw) mk = fmaxf(mk, scan_s[c & 1][i]);
         mw = max(mw, kmax_s[c & 1][i]);
+        mc = max(mc, kmax_s[c & 1][4 + i]);
       }
-      const int m = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
-      fg_s[c & 1][j] = fg == kNoTerm ? -100000 : fg;   // so far down that its column of P is zero
-      m_s[c & 1][j] = m;
-      if (j == 0) mw_s[c & 3] = mw;
-      if constexpr (FULL) store_row<false>(V, p2(-g), v_hi, v_lo, j);
-      {
-        // v 2^-g r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa last
-        float s = 0.f;
-        if (key != kNoTerm) {
-          const int n = max(fg + we - mw, -100);            // <= 0
-          s = (wt * p2(max(-we, -126))) * p2(n);            // [1, 2) * 2^n
-        }
-#pragma unroll
-        for (int e = 0; e < 64; ++e) V[e] *= p2(-g);
-        store_row<false>(V, s, vw_hi, vw_lo, j);
-      }
-      fence_proxy_async();
-      mbar_arrive(bar_kv + 8 * st);
-      // q
+      if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
       if constexpr (FULL) {
-        int64_t tn;
-        const bool next_in = at(c + 1, &tn);
-        if constexpr (KT == 1) {
-          load64(B, kb + tn, T, Dk, next_in);
-        } else {
-          load64(A, qb + tt, T, 64, in);
-          load64(B, qb + 64 * T + tt, T, Dk - 64, in);
+        const float col = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
+        col_s[c & 1][j] = col;
+        colr_s[c & 1][j] = col * pow_pad[64 - (j & 31)];
+        m_s[c & 3][j] = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
+        if (j == 0) mc_s[c & 1] = mc;
+      }
+      if (j == 0) mw_s[c & 3] = mw;
+      const float gs = p2(-g);
+#pragma unroll
+      for (int e = 0; e < 64; ++e) x[e] *= gs;
+      if constexpr (FULL) store_row<false>(x, 1.f, v_hi, v_lo, j);
+      // times r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa first
+      const float s = key != kNoTerm ? (wt * p2(max(-we, -126))) * p2(max(fg + we - mw, -100)) : 0.f;
+      store_row<false>(x, s, vw_hi, vw_lo, j);
+      fence_proxy_async();
+      mbar_arrive(bar_v + 8 * (c % NS));
+    }
+  } else if (role == 2) {
+    // ---------------- q, to tensor memory ----------------
+    regs_inc<Regs<KT>::q>();
+    if constexpr (FULL) {
+      const float* qb = w.q + head * (int64_t)Dk * T;
+#pragma unroll 1
+      for (int c = 0; c < nc; ++c) {
+        int64_t tt;
+        bool whole;
+        const bool in = step_at(c, &tt, &whole);
+        float x[64];
+        load64(x, qb + tt, T, Dk, in, whole);
+        float top = top64(x);
+        if constexpr (KT == 2) {
+          load64(x, qb + 64 * T + tt, T, Dk - 64, in, whole);
+          top = top64(x, top);
         }
-        float qtop = top64(A);
-        if constexpr (KT == 2) qtop = top64(B, qtop);
-        const bool qbad = not_finite(qtop);
-        const int qe = qbad ? 0 : fit_exponent(qtop);
+        const bool bad = not_finite(top);
+        const int qe = bad ? 0 : fit_exponent(top);
         const float qs = p2(-qe);
-        qe_s[c & 1][j] = qbad ? 0x7fffffff : qe;
         if (c >= 1) wait_or_dead(bar_qfree, (uint32_t)(c - 1) & 1u, dead);
         tc_fence_after();
-        const uint32_t row = tmem + ((uint32_t)(warp * 32) << 16) + S_::q;
-        float q2 = 0.f;
+        float n2 = 0.f;
+#pragma unroll 1
+        for (int t = KT - 1; t >= 0; --t) {
+          if (KT == 2 && t == 0) load64(x, qb + tt, T, 64, in, whole);
+          if (bad) {
 #pragma unroll
-        for (int half = 0; half < KT; ++half) {
-          float(&Q)[64] = half == 0 ? A : B;
-          uint32_t hi[32], lo[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float x0 = Q[2 * e] * qs, x1 = Q[2 * e + 1] * qs;
-            if (qbad) x0 = x1 = 0.f;
-            q2 = fmaf(x0, x0, fmaf(x1, x1, q2));
-            split2(x0, x1, &hi[e], &lo[e]);
+            for (int d = 0; d < 64; ++d) x[d] = 0.f;
           }
-          tmem_st32(row + half * 32, hi);
-          tmem_st32(row + 32 * KT + half * 32, lo);
+#pragma unroll
+          for (int b = 0; b < 64; b += 32) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x0 = x[b + 2 * e] * qs, x1 = x[b + 2 * e + 1] * qs;
+              n2 = fmaf(x0, x0, fmaf(x1, x1, n2));
+              split2(x0, x1, &hi[e], &lo[e]);
+            }
+            tmem_st16(trow + S_::q + t * 32 + b / 2, hi);
+            tmem_st16(trow + S_::q + 32 * KT + t * 32 + b / 2, lo);
+          }
         }
-        uq_s[c & 1][j] = q2 > 0.f ? norm_exponent(q2) : 0;
+        qe_s[c & 3][th] = bad ? 0x7fffffff : qe;
+        uq_s[c & 3][th] = n2 > 0.f ? norm_exponent(n2) : 0;
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(bar_q);
-      } else if constexpr (KT == 1) {
-        int64_t tn;
-        const bool next_in = at(c + 1, &tn);
-        load64(B, kb + tn, T, Dk, next_in);
       }
-    };
-    float A[64], B[64];
-    if constexpr (KT == 1) {
-      int64_t tt;
-      const bool in = at(0, &tt);
-      load64(A, kb + tt, T, Dk, in);
     }
-    for (int c = 0; c < nc; c += 2) {
-      chunk(c, A, B);
-      if (c + 1 < nc) chunk(c + 1, B, A);
+  } else if (role == 3) {
+    // ---------------- scores -> P: thread = row i ----------------
+    if constexpr (Regs<KT>::p > 80) regs_inc<Regs<KT>::p>();
+    if constexpr (FULL) {
+      const int l = th;
+#pragma unroll 1
+      for (int c = 0; c < nc; ++c) {
+        const uint32_t sp = trow + S_::sp + (uint32_t)(c % NSP) * 128u;
+        wait_or_dead(bar_sp + 8 * (c % NSP), (uint32_t)(c / NSP) & 1u, dead);
+        wait_or_dead(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);    // the columns' factors
+        tc_fence_after();
+        // P is held as its multiple of 2^(m + uq - 15): at most 2^15
+        const float rowf = p2(max(-126, min(mc_s[c & 1] - (m_s[c & 3][l] + uq_s[c & 3][l] - 15), 127)));
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+          uint32_t hi[16], lo[16];
+          if (g > tw) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) hi[x] = lo[x] = 0u;
+          } else {
+            uint32_t r[32];
+            tmem_ld32(sp + g * 32, r);
+            tmem_ld_wait();
+            if (g < tw) {
+              // r^(i - j) = r^(i - 32 (g + 1)) r^(32 - j % 32)
+              const float rf = rowf * pow_pad[l - g * 32];
+#pragma unroll
+              for (int jj = 0; jj < 32; jj += 4) {
+                const float4 cf = *reinterpret_cast<const float4*>(&colr_s[c & 1][g * 32 + jj]);
+                split2(__uint_as_float(r[jj]) * cf.x * rf, __uint_as_float(r[jj + 1]) * cf.y * rf, &hi[jj / 2],
+                       &lo[jj / 2]);
+                split2(__uint_as_float(r[jj + 2]) * cf.z * rf, __uint_as_float(r[jj + 3]) * cf.w * rf, &hi[jj / 2 + 1],
+                       &lo[jj / 2 + 1]);
+              }
+            } else {
+              const float* pw = &pow_pad[32 + lane];    // the power first: its zeros are the mask
+#pragma unroll
+              for (int jj = 0; jj < 32; jj += 4) {
+                const float4 cf = *reinterpret_cast<const float4*>(&col_s[c & 1][g * 32 + jj]);
+                split2(__uint_as_float(r[jj]) * pw[-jj] * cf.x * rowf,
+                       __uint_as_float(r[jj + 1]) * pw[-jj - 1] * cf.y * rowf, &hi[jj / 2], &lo[jj / 2]);
+                split2(__uint_as_float(r[jj + 2]) * pw[-jj - 2] * cf.z * rowf,
+                       __uint_as_float(r[jj + 3]) * pw[-jj - 3] * cf.w * rowf, &hi[jj / 2 + 1], &lo[jj / 2 + 1]);
+              }
+            }
+          }
+          tmem_st16(sp + g * 32, hi);
+          tmem_st16(sp + g * 32 + 16, lo);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar_p);
+      }
     }
-  } else if (warp < 8) {
-    // ---------------- scores -> P, state, output: thread = step i, or (column e, half of Dk) ----------------
-    regs_inc<kRegsSoft>();
-    const int l = tid - 128;
-    const int e = l & 63, half = l >> 6;
+  } else if (role == 4) {
+    // ---------------- state (column e, half of Dk) and output (step i) ----------------
+    regs_inc<Regs<KT>::s>();
+    const int l = th, e = l & 63, half = l >> 6;
     constexpr int NSt = 32 * KT;                 // state elements per thread: d = half * NSt ...
-    const uint32_t trow = tmem + ((uint32_t)((warp - 4) * 32) << 16);
     float St[NSt];
     {
       const float* src = nullptr;
@@ -482,55 +571,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       fence_proxy_async();
     };
-    if (FULL) publish(0);
-    mbar_arrive(bar_s);
-
-    for (int c = 0; c < nc; ++c) {
-      const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
-      int qe = 0, m = 0;
-      if constexpr (FULL) {
-        const uint32_t sp = trow + S_::sp + (uint32_t)(c % NSP) * 128u;
-        wait_or_dead(bar_sp + 8 * (c % NSP), (uint32_t)(c / NSP) & 1u, dead);
-        tc_fence_after();
-        qe = qe_s[c & 1][l];
-        m = m_s[c & 1][l] + uq_s[c & 1][l] - 15; // P is held as its multiple of 2^m, at most 2^15
-        const int off = 127 - m;                 // exponent field of 2^(fg - m)
+    // two call sites in one: c = -1 publishes the state the walk starts from
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
-          uint32_t hi[16], lo[16];
-          if (g * 32 <= (l | 31)) {
-            uint32_t r[32];
-            tmem_ld32(sp + g * 32, r);
-            tmem_ld_wait();
-            const float* pw = &pow_pad[32 + l - g * 32];
-#pragma unroll
-            for (int jj = 0; jj < 32; jj += 4) {
-              const int4 f4 = *reinterpret_cast<const int4*>(&fg_s[c & 1][g * 32 + jj]);
-              const int fs[4] = {f4.x, f4.y, f4.z, f4.w};
-              float x[4];
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                const int ex = min(max(fs[u] + off, 0), 254);
-                x[u] = __uint_as_float(r[jj + u]) * pw[-(jj + u)] * __int_as_float(ex << 23);
-              }
-              split2(x[0], x[1], &hi[jj / 2], &lo[jj / 2]);
-              split2(x[2], x[3], &hi[jj / 2 + 1], &lo[jj / 2 + 1]);
-            }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) hi[x] = lo[x] = 0u;
-          }
-          tmem_st16(sp + g * 32, hi);
-          tmem_st16(sp + g * 32 + 16, lo);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(bar_p);
-      }
-      // the state after the chunk
-      wait_or_dead(bar_ds, (uint32_t)c & 1u, dead);
-      tc_fence_after();
-      {
+    for (int c = -1; c < nc; ++c) {
+      if (c >= 0) {
+        // the state after chunk c
+        const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
+        wait_or_dead(bar_ds, (uint32_t)c & 1u, dead);
+        tc_fence_after();
         const Factors mw = p2_wide(mw_s[c & 3]);
         const float carry = pow_pad[32 + len];
         // rows 0-63 of the accumulator come from the hi half of v, rows 64-127 from the lo half: each
@@ -565,38 +613,55 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
         }
         tc_fence_before();
-        if (FULL && c + 1 < nc) publish((c + 1) & 1);      // its barrier also ends the exchange
-        else bar_sync(2, 128);
-        mbar_arrive(bar_s);
       }
-      if constexpr (FULL) {
+      if (FULL && c + 1 < nc) publish((c + 1) & 1);      // its barrier also ends the exchange
+      else bar_sync(2, 128);
+      mbar_arrive(bar_s);
+      if (FULL && c >= 0) {
         const int64_t t = (c0 + c) * kL + l;
         const int64_t tt = w.reverse ? T - 1 - t : t;
         float* out = w.o + (head * (int64_t)w.Dv + e0) * T + tt;
-        const bool live = t < T;
-        const Factors fi = p2_wide((qe == 0x7fffffff ? 0 : qe) + m);
-        const Factors fx = p2_wide(qe == 0x7fffffff ? 0 : qe);
-        const float nan = __int_as_float(0x7fffffff);
-        const float ia = qe == 0x7fffffff ? nan : fi.a, ib = fi.b;
-        const float xa = fx.a, xb = fx.b * pow_pad[32 + l + after];
+        const bool live = t < T, plain = (c0 + c + 1) * kL <= T && ne == 64;
         wait_or_dead(bar_o, (uint32_t)c & 1u, dead);
         tc_fence_after();
+        const int qe = qe_s[c & 3][l], m = m_s[c & 3][l] + uq_s[c & 3][l] - 15;
+        const bool bad = qe == 0x7fffffff;
+        const Factors fi = p2_wide((bad ? 0 : qe) + m), fx = p2_wide(bad ? 0 : qe);
+        const float nan = __int_as_float(0x7fffffff);
+        const float ia = bad ? nan : fi.a, ib = fi.b, xa = fx.a, xb = fx.b * pow_pad[32 + l + after];
         const bool poisoned = *any_poison != 0;
-#pragma unroll
-        for (int b = 0; b < 64; b += 32) {
-          uint32_t ri[32], rx[32];
-          tmem_ld32(trow + S_::oi + b, ri);
-          tmem_ld32(trow + S_::ox + b, rx);
+#pragma unroll 1
+        for (int b = 0; b < 64; b += 16) {
+          uint32_t ri[16], rx[16];
+          tmem_ld16(trow + S_::oi + b, ri);
+          tmem_ld16(trow + S_::ox + b, rx);
           tmem_ld_wait();
-          if (b == 32) {
+          if (b == 48) {
             tc_fence_before();
             mbar_arrive(bar_ofree);
           }
+          const float* sc = &scale_s[c & 1][b];
+          float y[16];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            float y = __uint_as_float(ri[x]) * ia * ib + __uint_as_float(rx[x]) * xa * (xb * scale_s[c & 1][b + x]);
-            if (poisoned && poison_s[b + x] <= (int)t) y = nan;
-            if (live && b + x < ne) out[(int64_t)(b + x) * T] = y;
+          for (int x = 0; x < 16; ++x)
+            y[x] = __uint_as_float(ri[x]) * ia * ib + __uint_as_float(rx[x]) * xa * (xb * sc[x]);
+          if (poisoned) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              if (poison_s[b + x] <= (int)t) y[x] = nan;
+          }
+          if (plain) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              *out = y[x];
+              out += T;
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              if (live && b + x < ne) *out = y[x];
+              out += T;
+            }
           }
         }
       }
@@ -618,89 +683,95 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
     }
   } else {
-    regs_dec<kRegsMma>();
-    if (tid == 256) {
-    // ---------------- MMAs ----------------
-    constexpr uint32_t id_scores = idesc_f16(kL), id_inter = idesc_f16(64), id_intra = idesc_f16(64) | kBMajorMN,
-                       id_grow = idesc_f16(64 * KT) | kAMajorMN | kBMajorMN;
-    const uint32_t tq = tmem + S_::q, toi = tmem + S_::oi, tox = tmem + S_::ox, tds = tmem + S_::ds;
-    bool ok = true;
-    auto stage_of = [&](int c) { return base + (uint32_t)(c % NS) * S_::stage_bytes; };
-    auto scores = [&](int c) {
-      ok = wait_or_dead(bar_q, (uint32_t)c & 1u, dead) && ok;
-      ok = wait_or_dead(bar_kv + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
-      if (!ok) return;
-      tc_fence_after();
-      const uint32_t k_hi = stage_of(c), k_lo = k_hi + KT * kTileB, d = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
-#pragma unroll
-      for (int s = 0; s < 4 * KT; ++s) {
-        const uint32_t at = (uint32_t)((s >> 2) * kTileB + (s & 3) * 32);
-        mma_f16_ts(d, tq + s * 8, desc_lo(k_hi + at), id_scores, s > 0);
-        mma_f16_ts(d, tq + 32 * KT + s * 8, desc_lo(k_hi + at), id_scores, 1u);
-        mma_f16_ts(d, tq + s * 8, desc_lo(k_lo + at), id_scores, 1u);
-      }
-      umma_commit(bar_sp + 8 * (c % NSP));
-      mbar_arrive(bar_sp + 8 * (c % NSP));   // hands on what the loaders wrote beside the operands
-    };
-    if (FULL) scores(0);
-    for (int c = 0; c < nc && ok; ++c) {
-      const uint32_t stage = stage_of(c);
-      const uint32_t k_hi = stage, k_lo = stage + KT * kTileB, v_hi = stage + 2 * KT * kTileB, v_lo = v_hi + kTileB,
-                     vw_hi = v_lo + kTileB;
-      ok = wait_or_dead(bar_s, (uint32_t)c & 1u, dead) && ok;
-      if (FULL) {
-        if (c >= 1) ok = wait_or_dead(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
-      } else {
-        ok = wait_or_dead(bar_kv + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
-      }
-      if (!ok) break;
-      tc_fence_after();
-      if (FULL) {
-#pragma unroll
+    regs_dec<Regs<KT>::mma>();
+    if (th == 0) {
+      // ---------------- MMAs ----------------
+      constexpr uint32_t id_scores = idesc_f16(kL), id_inter = idesc_f16(64), id_intra = idesc_f16(64) | kBMajorMN,
+                         id_grow = idesc_f16(64 * KT) | kAMajorMN | kBMajorMN;
+      const uint32_t tq = tmem + S_::q, toi = tmem + S_::oi, tox = tmem + S_::ox, tds = tmem + S_::ds;
+      bool ok = true;
+      // The barriers that count to two take an arrival of this thread beside the commit: it hands on what
+      // the loaders wrote beside the operands.
+      auto scores = [&](int c) {
+        ok = wait_or_dead(bar_q, (uint32_t)c & 1u, dead) && ok;
+        ok = wait_or_dead(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::stage_bytes, d = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
+#pragma unroll 1
         for (int s = 0; s < 4 * KT; ++s) {
-          const uint32_t at = sbase + (uint32_t)((s >> 2) * 8192 + (s & 3) * 32);
-          mma_f16_ts(tox, tq + s * 8, desc_lo(at), id_inter, s > 0);
-          mma_f16_ts(tox, tq + 32 * KT + s * 8, desc_lo(at), id_inter, 1u);
-          mma_f16_ts(tox, tq + s * 8, desc_lo(at + KT * 8192), id_inter, 1u);
+          const uint32_t bh = desc_lo(k_hi + (uint32_t)((s >> 2) * kTileB + (s & 3) * 32));
+          mma_f16_ts(d, tq + s * 8, bh, id_scores, s > 0);
+          mma_f16_ts(d, tq + 32 * KT + s * 8, bh, id_scores, 1u);
+          mma_f16_ts(d, tq + s * 8, bh + (KT * kTileB >> 4), id_scores, 1u);
         }
-        umma_commit(bar_qfree);
-      }
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        mma_f16_ss(tds, desc_mn(vw_hi + s * 2048), desc_mn(k_hi + s * 2048), id_grow, s > 0);
-        mma_f16_ss(tds, desc_mn(vw_hi + s * 2048), desc_mn(k_lo + s * 2048), id_grow, 1u);
-      }
-      umma_commit(bar_ds);
-      mbar_arrive(bar_ds);
-      if (!FULL) {
+        umma_commit(bar_sp + 8 * (c % NSP));
+        mbar_arrive(bar_sp + 8 * (c % NSP));
+      };
+      if (FULL) scores(0);
+#pragma unroll 1
+      for (int c = 0; c < nc && ok; ++c) {
+        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::stage_bytes, v_hi = k_hi + 2 * KT * kTileB,
+                       vw_hi = v_hi + 2 * kTileB;
+        ok = wait_or_dead(bar_s, (uint32_t)c & 1u, dead) && ok;
+        if (FULL) {
+          if (c >= 1) ok = wait_or_dead(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
+        } else {
+          ok = wait_or_dead(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        }
+        if (!ok) break;
+        tc_fence_after();
+        if (FULL) {
+#pragma unroll 1
+          for (int s = 0; s < 4 * KT; ++s) {
+            const uint32_t bh = desc_lo(sbase + (uint32_t)((s >> 2) * 8192 + (s & 3) * 32));
+            mma_f16_ts(tox, tq + s * 8, bh, id_inter, s > 0);
+            mma_f16_ts(tox, tq + 32 * KT + s * 8, bh, id_inter, 1u);
+            mma_f16_ts(tox, tq + s * 8, bh + (KT * 8192 >> 4), id_inter, 1u);
+          }
+          umma_commit(bar_qfree);
+        }
+        ok = wait_or_dead(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int s = 0; s < 8; ++s) {
+          const uint32_t a = desc_mn(vw_hi + s * 2048), b = desc_mn(k_hi + s * 2048);
+          mma_f16_ss(tds, a, b, id_grow, s > 0);
+          mma_f16_ss(tds, a, b + (KT * kTileB >> 4), id_grow, 1u);
+        }
+        umma_commit(bar_ds);
+        mbar_arrive(bar_ds);
+        if (!FULL) {
+          umma_commit(bar_free + 8 * (c % NS));
+          continue;
+        }
+        if (NSP == 2 && c + 1 < nc) scores(c + 1);
+        ok = wait_or_dead(bar_p, (uint32_t)c & 1u, dead) && ok;
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sp = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
+#pragma unroll 1
+        for (int s = 0; s < 8; ++s) {
+          const uint32_t p_hi = sp + (uint32_t)((s >> 1) * 32 + (s & 1) * 8), bh = desc_mn(v_hi + s * 2048);
+          mma_f16_ts(toi, p_hi, bh, id_intra, s > 0);
+          mma_f16_ts(toi, p_hi + 16, bh, id_intra, 1u);
+          mma_f16_ts(toi, p_hi, bh + (kTileB >> 4), id_intra, 1u);
+        }
+        umma_commit(bar_o);
+        mbar_arrive(bar_o);
         umma_commit(bar_free + 8 * (c % NS));
-        continue;
+        if (NSP == 1 && c + 1 < nc) scores(c + 1);
       }
-      if (NSP == 2 && c + 1 < nc) scores(c + 1);
-      ok = wait_or_dead(bar_p, (uint32_t)c & 1u, dead) && ok;
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t sp = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const uint32_t p_hi = sp + (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
-        mma_f16_ts(toi, p_hi, desc_mn(v_hi + s * 2048), id_intra, s > 0);
-        mma_f16_ts(toi, p_hi + 16, desc_mn(v_hi + s * 2048), id_intra, 1u);
-        mma_f16_ts(toi, p_hi, desc_mn(v_lo + s * 2048), id_intra, 1u);
-      }
-      umma_commit(bar_o);
-      umma_commit(bar_free + 8 * (c % NS));
-      if (NSP == 1 && c + 1 < nc) scores(c + 1);
-    }
-    umma_commit(bar_end);          // everything issued has landed before tensor memory is given back
-    if (!mbar_wait(bar_end, 0)) *dead = 1;
+      umma_commit(bar_end);          // everything issued has landed before tensor memory is given back
+      if (!mbar_wait(bar_end, 0)) *dead = 1;
     }
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   if (*dead && tid == 0) dev_flag(args.status, SB_DEV_TMA_TIMEOUT);
-  if (warp == 8) {
+  if (role == 5 && tw == 0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
