@@ -15,9 +15,9 @@
 // contraction instead of 8 and a tile half the shared memory, which is what leaves room to stage the
 // next chunk.  fp16 has no range, so the powers of two travel beside the mantissas: q, k and v have one
 // exponent per step, the state one per column of v, and a row of P one per step i: |q_i . k_j| is at most
-// |q_i| |k_j|, so the largest of 2^f |k_j| 2^g over j <= i (a running maximum that decays with r) bounds
-// the row without looking at it, and no outlier costs the accuracy of a step that does not read it.
-// A vector's largest element has 2^13 or more and an fp16 pair steps of 2^-24.
+// Dk times the two largest elements, so the largest of 2^(f + g) over j <= i (a running maximum that
+// decays with r) bounds the row without looking at it, and no outlier costs the accuracy of a step that
+// does not read it.  A vector's largest element has 2^13 or more and an fp16 pair steps of 2^-24.
 //
 // Values that are not finite must not meet a zero of the causal mask in an MMA (0 * NaN): the loader
 // zeroes them and notes from which step on a column of the output is spoilt.
@@ -32,9 +32,11 @@
 //
 // Roles of a CTA (one per SM, six warpgroups): k, v and q are each loaded and converted by a warpgroup
 // (one step per thread), one turns scores into P, one keeps the state (32 elements per thread and 64 of
-// Dk in registers, fp32) and writes the output, and one thread issues the MMAs.  An earlier form with one
-// loading warpgroup that held two operands at a time in 232 registers ran at 15.3 us per chunk of
-// [128 x 64]: 6650 instructions per scheduler in straight-line code that missed the instruction cache.
+// Dk in registers, fp32) and writes the output, and one thread issues the MMAs.  What decides the speed
+// is the instruction cache: a first form (one loading warpgroup with two operands in 232 registers) ran at
+// 15.3 us per chunk of [128 x 64], separate code for k, v and q at 8.4 us with 41 % of the fetches missing.
+// So the three loaders run the same instructions, the branches between them are uniform, and loops over
+// columns stay rolled where registers allow.
 //
 // A head with T steps is one CTA, or several when there are fewer heads than SMs: the axis is then cut
 // into segments, a first launch takes each segment's growth from zero, a small one joins them, and the
@@ -53,8 +55,8 @@ constexpr int kThreads = 768;
 // the vectors live.  Each row adds up to 6 * 80.
 template <int KT>
 struct Regs {
-  static constexpr int k = 88, v = KT == 1 ? 96 : 88, q = 88, p = KT == 1 ? 96 : 80, s = KT == 1 ? 88 : 112, mma = 24;
-  static_assert(k + v + q + p + s + mma <= 480, "more registers than the block was launched with");
+  static constexpr int load = KT == 1 ? 96 : 88, p = KT == 1 ? 80 : 72, s = KT == 1 ? 88 : 112, mma = 24;
+  static_assert(3 * load + p + s + mma <= 480, "more registers than the block was launched with");
 };
 constexpr int kMaxSub = 6;
 
@@ -74,6 +76,7 @@ struct Shape {
   static constexpr int nsp = KT == 1 ? 2 : 1;         // score accumulators
   static constexpr int stage_bytes = (2 * KT + 4) * kTileB;
   static constexpr int state_bytes = 2 * KT * 64 * 128;
+  static constexpr int score = KT == 1 ? 34 : 35;     // 2^14 2^14 Dk
   static constexpr int smem = 1024 + stages * stage_bytes + state_bytes;
   // tensor memory columns
   static constexpr uint32_t q = 0, sp = 64 * KT, oi = sp + 128 * nsp, ox = oi + 64, ds = ox + 64;
@@ -94,6 +97,32 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// pairs of floats in one 64-bit register: two products or sums per instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -101,14 +130,20 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 // hi = fp16(x), lo = fp16(x - hi) of two neighbours, packed
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t* hi, uint32_t* lo) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(x1), "f"(x0));
+__device__ __forceinline__ void split2(uint64_t x, uint32_t* hi, uint32_t* lo) {
+  const float2 v = unpair(x);
   float h0, h1;
+  uint32_t h;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(v.y), "f"(v.x));
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
       : "=f"(h0), "=f"(h1) : "r"(h));
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(*lo) : "f"(x1 - h1), "f"(x0 - h0));
+  const float2 d = unpair(fma2(pair(h0, h1), pair(-1.f, -1.f), x));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(*lo) : "f"(d.y), "f"(d.x));
   *hi = h;
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
+               ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 // D (+)= A B^T, fp16 operands, fp32 accumulator: A in tensor memory or shared memory, B in shared memory
@@ -144,27 +179,40 @@ __device__ __forceinline__ uint32_t desc_mn(uint32_t saddr) {
 
 // 64 rows of one step.  volatile: the loads stay where they are issued, in one batch ahead of the waits
 // and conversions (left to itself the compiler sinks them to their use).
-__device__ __forceinline__ void load64(float (&x)[64], const float* p, int64_t T, int rows, bool in, bool whole) {
+__device__ __forceinline__ void load64(uint64_t (&x)[32], const float* p, int64_t T, int rows, bool in, bool whole) {
   if (whole && rows >= 64) {
 #pragma unroll
-    for (int d = 0; d < 64; ++d) {
-      asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(x[d]) : "l"(p));
+    for (int d = 0; d < 64; d += 2) {
+      float a, b;
+      asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(a) : "l"(p));
       p += T;
+      asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(b) : "l"(p));
+      p += T;
+      x[d / 2] = pair(a, b);
     }
   } else {
     const int n = in ? rows : 0;
 #pragma unroll
-    for (int d = 0; d < 64; ++d) {
+    for (int d = 0; d < 64; d += 2) {
+      float a, b;
       asm volatile(
           "{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.nc.f32 %0, [%1];\n\t}"
-          : "=f"(x[d]) : "l"(p), "r"(n), "r"(d));
+          : "=f"(a) : "l"(p), "r"(n), "r"(d));
       p += T;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.nc.f32 %0, [%1];\n\t}"
+          : "=f"(b) : "l"(p), "r"(n), "r"(d + 1));
+      p += T;
+      x[d / 2] = pair(a, b);
     }
   }
 }
-__device__ __forceinline__ float top64(const float (&x)[64], float m = 0.f) {
+__device__ __forceinline__ float top64(const uint64_t (&x)[32], float m = 0.f) {
 #pragma unroll
-  for (int d = 0; d < 64; d += 2) m = max_abs3(m, x[d], x[d + 1]);
+  for (int d = 0; d < 32; ++d) {
+    const float2 v = unpair(x[d]);
+    m = max_abs3(m, v.x, v.y);
+  }
   return m;
 }
 // Exponent that brings a largest magnitude into [2^13, 2^14); a zero vector gets one that no sum prefers.
@@ -174,31 +222,6 @@ __device__ __forceinline__ int fit_exponent(float top) {
   return max(e, -113) - 13;
 }
 __device__ __forceinline__ bool not_finite(float top) { return __float_as_uint(top) >= 0x7f800000u; }
-// Smallest u (up to one) with |x| <= 2^u, from |x|^2.
-__device__ __forceinline__ int norm_exponent(float n2) {
-  return ((int)(__float_as_uint(n2) >> 23) - 127 + 2) >> 1;
-}
-// Scaled by `s`, split and written as one row of a hi and a lo tile (128-byte swizzle); NORM returns the
-// scaled row's sum of squares.
-template <bool NORM>
-__device__ __forceinline__ float store_row(const float (&x)[64], float s, uint32_t hi_tile, uint32_t lo_tile, int row) {
-  float n2 = 0.f;
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x0 = x[8 * c + 2 * e] * s, x1 = x[8 * c + 2 * e + 1] * s;
-      if constexpr (NORM) n2 = fmaf(x0, x0, fmaf(x1, x1, n2));
-      split2(x0, x1, &h[e], &l[e]);
-    }
-    const uint32_t at = (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4));
-    sts128(hi_tile + at, h[0], h[1], h[2], h[3]);
-    sts128(lo_tile + at, l[0], l[1], l[2], l[3]);
-  }
-  return n2;
-}
-
 // KT: 64-wide tiles of Dk.  FULL: the walk itself; otherwise only the state after each segment but the last.
 template <int R>
 __device__ __forceinline__ void regs_inc() {
@@ -216,9 +239,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   extern __shared__ uint8_t raw[];
   // What travels beside the mantissas.  A slot of two is rewritten for chunk c + 2 once the read-out of
   // chunk c has ended, a slot of four once the output of chunk c + 1 has been written.
-  __shared__ int f_s[2][kL], u_s[2][kL];                            // k: exponent, norm exponent
-  __shared__ __align__(16) float col_s[2][kL], colr_s[2][kL];       // of a column of P: 2^(fg - mc), that times r^(32 - j % 32)
-  __shared__ int mc_s[2], m_s[4][kL], qe_s[4][kL], uq_s[4][kL], mw_s[4];
+  __shared__ int f_s[2][kL];                                        // k's exponent
+  __shared__ __align__(16) float col_s[2][kL];                      // of a column of P: 2^(fg - mc)
+  __shared__ int mc_s[2], m_s[4][kL], qe_s[4][kL], mw_s[4];
   __shared__ float scan_s[2][4];
   __shared__ int kmax_s[2][8];
   __shared__ float pow_pad[32 + kL + 1];       // r^n at 32 + n; zeros before it are the causal mask
@@ -294,188 +317,167 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   const uint32_t tmem = tmem_s;
   const uint32_t trow = tmem + ((uint32_t)(tw * 32) << 16);   // this warp's lanes of tensor memory
 
-  // a thread's step of chunk c, walked in the CTA's direction: memory index, inside the axis, chunk complete
-  auto step_at = [&](int c, int64_t* tt, bool* whole) {
-    const int64_t t = (c0 + c) * kL + th;
-    *tt = w.reverse ? T - 1 - t : t;
-    *whole = (c0 + c + 1) * kL <= T;
-    return t < T;
-  };
-
-  if (role == 0) {
-    // ---------------- k ----------------
-    regs_inc<Regs<KT>::k>();
-    const float* kb = w.k + head * (int64_t)Dk * T;
-#pragma unroll 1
-    for (int c = 0; c < nc; ++c) {
-      const uint32_t k_hi = base + (c % NS) * S_::stage_bytes, k_lo = k_hi + KT * kTileB;
-      int64_t tt;
-      bool whole;
-      const bool in = step_at(c, &tt, &whole);
-      float x[64];
-      load64(x, kb + tt, T, Dk, in, whole);
-      float top = top64(x);
-      if constexpr (KT == 2) {     // the second half stays, the first is fetched again once the exponent is known
-        load64(x, kb + 64 * T + tt, T, Dk - 64, in, whole);
-        top = top64(x, top);
-      }
-      bool spoilt = not_finite(top);
-      if (spoilt) {                // every column of the output is spoilt from this step on
-        top = 0.f;
-        for (int e = 0; e < 64; ++e) atomicMin(&poison_s[e], (int)((c0 + c) * kL + th));
-        any_poison_s = 1;
-#pragma unroll
-        for (int d = 0; d < 64; ++d) x[d] = 0.f;
-      }
-      const int f = fit_exponent(top);
-      if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
-      float n2;
-      if constexpr (KT == 2) {
-        n2 = store_row<true>(x, p2(-f), k_hi + kTileB, k_lo + kTileB, th);
-        load64(x, kb + tt, T, 64, in && !spoilt, whole && !__any_sync(0xffffffffu, spoilt));
-        n2 += store_row<true>(x, p2(-f), k_hi, k_lo, th);
-      } else {
-        n2 = store_row<true>(x, p2(-f), k_hi, k_lo, th);
-      }
-      f_s[c & 1][th] = top > 0.f ? f : kNoTerm - (spoilt ? 1 : 0);
-      u_s[c & 1][th] = norm_exponent(n2);
-      mbar_arrive(bar_kx + 8 * (c & 1));
-      fence_proxy_async();
-      mbar_arrive(bar_k + 8 * (c % NS));
-    }
-  } else if (role == 1) {
-    // ---------------- v, and what P and the growth need to know of the steps ----------------
-    regs_inc<Regs<KT>::v>();
+  if (role < 3) {
+    // ---------------- k, v, q: load, convert, hand on; the same instructions for the three ----------------
+    regs_inc<Regs<KT>::load>();
+    const int j = th;
+    const bool is_k = role == 0, is_v = role == 1, is_q = role == 2;
+    const float* src = is_k ? w.k + head * (int64_t)Dk * T
+                            : (is_v ? w.v + (head * (int64_t)w.Dv + e0) * T : w.q + head * (int64_t)Dk * T);
+    const int rows = is_v ? ne : Dk;
+    // Passes over an operand.  Dk > 64: the largest magnitude of the first half, then of the second, which
+    // is converted while it is there, then the first half again.  v: as it is, and weighted.
+    const int passes = is_v ? (FULL ? 2 : 1) : (KT == 2 ? 3 : 1);
+    const int mid = is_v ? 0 : KT - 1;           // the pass after whose load the exponent is known
     // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
     const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
-    const float* vb = w.v + (head * (int64_t)w.Dv + e0) * T;
-    const int j = th;
+    uint64_t x[32];
 #pragma unroll 1
-    for (int c = 0; c < nc; ++c) {
-      const uint32_t v_hi = base + (c % NS) * S_::stage_bytes + 2 * KT * kTileB, v_lo = v_hi + kTileB,
-                     vw_hi = v_lo + kTileB, vw_lo = vw_hi + kTileB;
+    for (int c = (FULL || !is_q) ? 0 : nc; c < nc; ++c) {
+      const uint32_t stage = base + (uint32_t)(c % NS) * S_::stage_bytes;
+      const int64_t t = (c0 + c) * kL + j;
       const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
-      int64_t tt;
-      bool whole;
-      const bool in = step_at(c, &tt, &whole);
-      float x[64];
-      load64(x, vb + tt, T, ne, in, whole);
-      float top = top64(x);
-      wait_or_dead(bar_kx + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
-      const int f = f_s[c & 1][j], u = u_s[c & 1][j];
-      const bool spoilt = f == kNoTerm - 1;
-      if (spoilt || not_finite(top)) {
-        if (!spoilt) {
-          for (int e = 0; e < ne; ++e)
-            if (not_finite(fabsf(vb[(int64_t)e * T + tt]))) atomicMin(&poison_s[e], (int)((c0 + c) * kL + j));
-          any_poison_s = 1;
-        }
-        top = 0.f;
-#pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          if (spoilt || not_finite(fabsf(x[e]))) x[e] = 0.f;
-          top = fmaxf(top, fabsf(x[e]));
-        }
-      }
-      const int g = fit_exponent(top);
-      const int fg = (top > 0.f && f > kNoTerm) ? f + g : kNoTerm;
-      // weight of the step in the state, and the largest exponents: of all steps, of the weighted ones
-      const float wt = (j < len) ? pow_pad[32 + len - after - j] : 0.f;
-      const int we = (int)((__float_as_uint(wt) >> 23) & 0xff) - 127;
-      const int key = wt != 0.f && fg != kNoTerm ? fg + we : kNoTerm;
-      // running maximum of log2(2^fg |k_j|) + (i - j) log2 r: the scan runs on that less i log2 r
-      float mk = fg == kNoTerm ? -1e30f : (float)(fg + u) - (float)j * slope;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float up = __shfl_up_sync(0xffffffffu, mk, o);
-        if (lane >= o) mk = fmaxf(mk, up);
-      }
-      const int kmax = __reduce_max_sync(0xffffffffu, key), fmax = __reduce_max_sync(0xffffffffu, fg);
-      if (lane == 31) {
-        scan_s[c & 1][tw] = mk;
-        kmax_s[c & 1][tw] = kmax;
-        kmax_s[c & 1][4 + tw] = fmax;
-      }
-      bar_sync(1, 128);
-      int mw = kNoTerm, mc = kNoTerm;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i < tw) mk = fmaxf(mk, scan_s[c & 1][i]);
-        mw = max(mw, kmax_s[c & 1][i]);
-        mc = max(mc, kmax_s[c & 1][4 + i]);
-      }
-      if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
-      if constexpr (FULL) {
-        const float col = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
-        col_s[c & 1][j] = col;
-        colr_s[c & 1][j] = col * pow_pad[64 - (j & 31)];
-        m_s[c & 3][j] = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
-        if (j == 0) mc_s[c & 1] = mc;
-      }
-      if (j == 0) mw_s[c & 3] = mw;
-      const float gs = p2(-g);
-#pragma unroll
-      for (int e = 0; e < 64; ++e) x[e] *= gs;
-      if constexpr (FULL) store_row<false>(x, 1.f, v_hi, v_lo, j);
-      // times r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa first
-      const float s = key != kNoTerm ? (wt * p2(max(-we, -126))) * p2(max(fg + we - mw, -100)) : 0.f;
-      store_row<false>(x, s, vw_hi, vw_lo, j);
-      fence_proxy_async();
-      mbar_arrive(bar_v + 8 * (c % NS));
-    }
-  } else if (role == 2) {
-    // ---------------- q, to tensor memory ----------------
-    regs_inc<Regs<KT>::q>();
-    if constexpr (FULL) {
-      const float* qb = w.q + head * (int64_t)Dk * T;
+      const bool in = j < len, whole = len == kL;
+      const float* at = src + (w.reverse ? T - 1 - t : t);
+      float top = 0.f, scale = 0.f, scale_w = 0.f;
+      bool zero = false;                         // the whole vector is left out
 #pragma unroll 1
-      for (int c = 0; c < nc; ++c) {
-        int64_t tt;
-        bool whole;
-        const bool in = step_at(c, &tt, &whole);
-        float x[64];
-        load64(x, qb + tt, T, Dk, in, whole);
-        float top = top64(x);
-        if constexpr (KT == 2) {
-          load64(x, qb + 64 * T + tt, T, Dk - 64, in, whole);
-          top = top64(x, top);
-        }
-        const bool bad = not_finite(top);
-        const int qe = bad ? 0 : fit_exponent(top);
-        const float qs = p2(-qe);
-        if (c >= 1) wait_or_dead(bar_qfree, (uint32_t)(c - 1) & 1u, dead);
-        tc_fence_after();
-        float n2 = 0.f;
-#pragma unroll 1
-        for (int t = KT - 1; t >= 0; --t) {
-          if (KT == 2 && t == 0) load64(x, qb + tt, T, 64, in, whole);
-          if (bad) {
-#pragma unroll
-            for (int d = 0; d < 64; ++d) x[d] = 0.f;
-          }
-#pragma unroll
-          for (int b = 0; b < 64; b += 32) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x0 = x[b + 2 * e] * qs, x1 = x[b + 2 * e + 1] * qs;
-              n2 = fmaf(x0, x0, fmaf(x1, x1, n2));
-              split2(x0, x1, &hi[e], &lo[e]);
+      for (int pass = 0; pass < passes; ++pass) {
+        const int half = (KT == 2 && !is_v && pass == 1) ? 1 : 0;
+        if (!is_v || pass == 0) load64(x, at + (int64_t)half * 64 * T, T, rows - half * 64, in, whole);
+        if (pass <= mid) top = top64(x, top);
+        if (pass == mid) {
+          const bool bad = not_finite(top);
+          if (is_k) {
+            if (bad) {                           // every column of the output is spoilt from this step on
+              for (int e = 0; e < 64; ++e) atomicMin(&poison_s[e], (int)t);
+              any_poison_s = 1;
+              zero = true;
             }
-            tmem_st16(trow + S_::q + t * 32 + b / 2, hi);
-            tmem_st16(trow + S_::q + 32 * KT + t * 32 + b / 2, lo);
+            const int f = fit_exponent(bad ? 0.f : top);
+            scale = p2(-f);
+            if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+            f_s[c & 1][j] = bad ? kNoTerm - 1 : (top > 0.f ? f : kNoTerm);
+            mbar_arrive(bar_kx + 8 * (c & 1));
+          } else if (is_q) {
+            zero = bad;
+            const int qe = bad ? 0 : fit_exponent(top);
+            scale = p2(-qe);
+            if (c >= 1) wait_or_dead(bar_qfree, (uint32_t)(c - 1) & 1u, dead);
+            tc_fence_after();
+            qe_s[c & 3][j] = bad ? 0x7fffffff : qe;
+          } else {
+            // v, and what P and the growth need to know of the steps
+            wait_or_dead(bar_kx + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
+            const int f = f_s[c & 1][j];
+            zero = f == kNoTerm - 1;
+            if (bad && !zero) {                  // single columns are spoilt; the rest of the vector counts
+              for (int e = 0; e < ne; ++e)
+                if (not_finite(fabsf(at[(int64_t)e * T]))) atomicMin(&poison_s[e], (int)t);
+              any_poison_s = 1;
+            }
+            if (bad || zero) {
+              top = 0.f;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                float2 v = unpair(x[e]);
+                if (zero || not_finite(fabsf(v.x))) v.x = 0.f;
+                if (zero || not_finite(fabsf(v.y))) v.y = 0.f;
+                top = max_abs3(top, v.x, v.y);
+                x[e] = pair(v.x, v.y);
+              }
+            }
+            const int g = fit_exponent(top);
+            const int fg = (top > 0.f && f > kNoTerm) ? f + g : kNoTerm;
+            // weight of the step in the state, and the largest exponents: of all steps, of the weighted ones
+            const float wt = in ? pow_pad[32 + len - after - j] : 0.f;
+            const int we = (int)((__float_as_uint(wt) >> 23) & 0xff) - 127;
+            const int key = wt != 0.f && fg != kNoTerm ? fg + we : kNoTerm;
+            // running maximum of fg_j + (i - j) log2 r: the scan runs on that less i log2 r
+            float mk = fg == kNoTerm ? -1e30f : (float)fg - (float)j * slope;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const float up = __shfl_up_sync(0xffffffffu, mk, o);
+              if (lane >= o) mk = fmaxf(mk, up);
+            }
+            const int kmax = __reduce_max_sync(0xffffffffu, key), fmax = __reduce_max_sync(0xffffffffu, fg);
+            if (lane == 31) {
+              scan_s[c & 1][tw] = mk;
+              kmax_s[c & 1][tw] = kmax;
+              kmax_s[c & 1][4 + tw] = fmax;
+            }
+            bar_sync(1, 128);
+            int mw = kNoTerm, mc = kNoTerm;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (i < tw) mk = fmaxf(mk, scan_s[c & 1][i]);
+              mw = max(mw, kmax_s[c & 1][i]);
+              mc = max(mc, kmax_s[c & 1][4 + i]);
+            }
+            if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+            if (FULL) {
+              col_s[c & 1][j] = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
+              m_s[c & 3][j] = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
+            }
+            if (j == 0) {
+              mc_s[c & 1] = mc;
+              mw_s[c & 3] = mw;
+            }
+            scale = p2(-g);
+            // r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa first
+            scale_w = key != kNoTerm ? (wt * p2(max(-we, -126))) * p2(max(fg + we - mw, -100)) : 0.f;
+            if (!FULL) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = mul2(x[e], pair(scale, scale));
+              scale = scale_w;
+            }
           }
         }
-        qe_s[c & 3][th] = bad ? 0x7fffffff : qe;
-        uq_s[c & 3][th] = n2 > 0.f ? norm_exponent(n2) : 0;
+        if (pass < mid) continue;
+        if (__any_sync(0xffffffffu, zero)) {
+          if (zero) {
+#pragma unroll
+            for (int d = 0; d < 32; ++d) x[d] = 0;
+          }
+        }
+        // one row of a hi and a lo tile (128-byte swizzle), or of q's columns of tensor memory
+        const bool weighted = is_v && (!FULL || pass == 1);
+        const uint32_t tile = stage + (is_v ? (uint32_t)(2 * KT + (weighted ? 2 : 0)) * kTileB : (uint32_t)half * kTileB) +
+                              (uint32_t)(j * 128);
+        const uint32_t lo_at = is_v ? kTileB : KT * kTileB;
+        const uint32_t tq = trow + S_::q + half * 32;
+        if (FULL && weighted) scale = scale_w;
+        const uint64_t sc = pair(scale, scale);
+#pragma unroll
+        for (int q8 = 0; q8 < 8; ++q8) {
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[4 * q8 + e] = mul2(x[4 * q8 + e], sc);       // v's weights come on top of its scale
+            split2(x[4 * q8 + e], &h[e], &l[e]);
+          }
+          if (is_q) {
+            tmem_st4(tq + q8 * 4, h[0], h[1], h[2], h[3]);
+            tmem_st4(tq + 32 * KT + q8 * 4, l[0], l[1], l[2], l[3]);
+          } else {
+            const uint32_t to = tile + (uint32_t)((q8 ^ (j & 7)) << 4);
+            sts128(to, h[0], h[1], h[2], h[3]);
+            sts128(to + lo_at, l[0], l[1], l[2], l[3]);
+          }
+        }
+      }
+      if (is_q) {
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(bar_q);
+      } else {
+        fence_proxy_async();
+        mbar_arrive((is_k ? bar_k : bar_v) + 8 * (c % NS));
       }
     }
   } else if (role == 3) {
     // ---------------- scores -> P: thread = row i ----------------
-    if constexpr (Regs<KT>::p > 80) regs_inc<Regs<KT>::p>();
+    if constexpr (Regs<KT>::p < 80) regs_dec<Regs<KT>::p>();
     if constexpr (FULL) {
       const int l = th;
 #pragma unroll 1
@@ -484,43 +486,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         wait_or_dead(bar_sp + 8 * (c % NSP), (uint32_t)(c / NSP) & 1u, dead);
         wait_or_dead(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);    // the columns' factors
         tc_fence_after();
-        // P is held as its multiple of 2^(m + uq - 15): at most 2^15
-        const float rowf = p2(max(-126, min(mc_s[c & 1] - (m_s[c & 3][l] + uq_s[c & 3][l] - 15), 127)));
+        // |q_i . k_j| <= 2^score of the scaled vectors: P is held as its multiple of 2^(m + score - 15)
+        const float rowf = p2(max(-126, min(mc_s[c & 1] - m_s[c & 3][l] - (S_::score - 15), 127)));
+        const uint64_t rf = pair(rowf, rowf);
+        const float* pw = &pow_pad[32 + l];      // r^(i - j), zero for j > i: the mask
+        const float* col = col_s[c & 1];
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
-          uint32_t hi[16], lo[16];
-          if (g > tw) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) hi[x] = lo[x] = 0u;
-          } else {
-            uint32_t r[32];
-            tmem_ld32(sp + g * 32, r);
+        for (int g = 0; g < 128; g += 16, pw -= 16, col += 16) {
+          uint32_t hi[8], lo[8];
+          if (g < tw * 32 + 32) {
+            uint32_t r[16];
+            tmem_ld16(sp + g, r);
             tmem_ld_wait();
-            if (g < tw) {
-              // r^(i - j) = r^(i - 32 (g + 1)) r^(32 - j % 32)
-              const float rf = rowf * pow_pad[l - g * 32];
 #pragma unroll
-              for (int jj = 0; jj < 32; jj += 4) {
-                const float4 cf = *reinterpret_cast<const float4*>(&colr_s[c & 1][g * 32 + jj]);
-                split2(__uint_as_float(r[jj]) * cf.x * rf, __uint_as_float(r[jj + 1]) * cf.y * rf, &hi[jj / 2],
-                       &lo[jj / 2]);
-                split2(__uint_as_float(r[jj + 2]) * cf.z * rf, __uint_as_float(r[jj + 3]) * cf.w * rf, &hi[jj / 2 + 1],
-                       &lo[jj / 2 + 1]);
-              }
-            } else {
-              const float* pw = &pow_pad[32 + lane];    // the power first: its zeros are the mask
-#pragma unroll
-              for (int jj = 0; jj < 32; jj += 4) {
-                const float4 cf = *reinterpret_cast<const float4*>(&col_s[c & 1][g * 32 + jj]);
-                split2(__uint_as_float(r[jj]) * pw[-jj] * cf.x * rowf,
-                       __uint_as_float(r[jj + 1]) * pw[-jj - 1] * cf.y * rowf, &hi[jj / 2], &lo[jj / 2]);
-                split2(__uint_as_float(r[jj + 2]) * pw[-jj - 2] * cf.z * rowf,
-                       __uint_as_float(r[jj + 3]) * pw[-jj - 3] * cf.w * rowf, &hi[jj / 2 + 1], &lo[jj / 2 + 1]);
-              }
+            for (int jj = 0; jj < 16; jj += 4) {
+              const float4 cf = *reinterpret_cast<const float4*>(col + jj);
+              // the power first: its zeros take whatever the steps after i hold
+              const uint64_t x = mul2(pair(__uint_as_float(r[jj]), __uint_as_float(r[jj + 1])), pair(pw[-jj], pw[-jj - 1]));
+              const uint64_t y = mul2(pair(__uint_as_float(r[jj + 2]), __uint_as_float(r[jj + 3])), pair(pw[-jj - 2], pw[-jj - 3]));
+              split2(mul2(mul2(x, pair(cf.x, cf.y)), rf), &hi[jj / 2], &lo[jj / 2]);
+              split2(mul2(mul2(y, pair(cf.z, cf.w)), rf), &hi[jj / 2 + 1], &lo[jj / 2 + 1]);
             }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) hi[x] = lo[x] = 0u;
           }
-          tmem_st16(sp + g * 32, hi);
-          tmem_st16(sp + g * 32 + 16, lo);
+          tmem_st8(sp + g, hi);
+          tmem_st8(sp + g + 8, lo);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -556,14 +548,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       bar_sync(2, 128);
       top = fmaxf(top, top_s[l ^ 64]);
       const int se = min(fit_exponent(top), 113);
-      const float s = p2(-se);
+      const uint64_t ss = pair(p2(-se), p2(-se));
       if (half == 0) scale_s[slot][e] = p2(se);
       const uint32_t tile = sbase + (KT == 2 ? half * 8192 : 0);
 #pragma unroll
       for (int c = 0; c < NSt / 8; ++c) {
         uint32_t h[4], lo[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) split2(St[8 * c + 2 * x] * s, St[8 * c + 2 * x + 1] * s, &h[x], &lo[x]);
+        for (int x = 0; x < 4; ++x) split2(mul2(pair(St[8 * c + 2 * x], St[8 * c + 2 * x + 1]), ss), &h[x], &lo[x]);
         const int chunk = (KT == 1 ? half * 4 : 0) + c;
         const uint32_t at = tile + (uint32_t)(e * 128 + ((chunk ^ (e & 7)) << 4));
         sts128(at, h[0], h[1], h[2], h[3]);
@@ -607,9 +599,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                          : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3])
                          : "r"(my_row + (uint32_t)(((b / 4 + x) ^ (l & 7)) << 4)));
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              St[b + 4 * x + u] = fmaf(carry, St[b + 4 * x + u],
-                                       (__uint_as_float(r[4 * x + u]) + y[u]) * mw.a * mw.b);
+            for (int u = 0; u < 4; u += 2) {
+              const uint64_t grown = add2(pair(__uint_as_float(r[4 * x + u]), __uint_as_float(r[4 * x + u + 1])), pair(y[u], y[u + 1]));
+              const float2 v = unpair(fma2(pair(carry, carry), pair(St[b + 4 * x + u], St[b + 4 * x + u + 1]),
+                                           mul2(mul2(grown, pair(mw.a, mw.a)), pair(mw.b, mw.b))));
+              St[b + 4 * x + u] = v.x;
+              St[b + 4 * x + u + 1] = v.y;
+            }
           }
         }
         tc_fence_before();
@@ -624,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const bool live = t < T, plain = (c0 + c + 1) * kL <= T && ne == 64;
         wait_or_dead(bar_o, (uint32_t)c & 1u, dead);
         tc_fence_after();
-        const int qe = qe_s[c & 3][l], m = m_s[c & 3][l] + uq_s[c & 3][l] - 15;
+        const int qe = qe_s[c & 3][l], m = m_s[c & 3][l] + S_::score - 15;
         const bool bad = qe == 0x7fffffff;
         const Factors fi = p2_wide((bad ? 0 : qe) + m), fx = p2_wide(bad ? 0 : qe);
         const float nan = __int_as_float(0x7fffffff);
@@ -643,8 +639,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           const float* sc = &scale_s[c & 1][b];
           float y[16];
 #pragma unroll
-          for (int x = 0; x < 16; ++x)
-            y[x] = __uint_as_float(ri[x]) * ia * ib + __uint_as_float(rx[x]) * xa * (xb * sc[x]);
+          for (int x = 0; x < 16; x += 2) {
+            const uint64_t inter = mul2(mul2(pair(__uint_as_float(rx[x]), __uint_as_float(rx[x + 1])), pair(xa, xa)),
+                                        mul2(pair(sc[x], sc[x + 1]), pair(xb, xb)));
+            const float2 v = unpair(fma2(mul2(pair(__uint_as_float(ri[x]), __uint_as_float(ri[x + 1])), pair(ia, ia)),
+                                         pair(ib, ib), inter));
+            y[x] = v.x;
+            y[x + 1] = v.y;
+          }
           if (poisoned) {
 #pragma unroll
             for (int x = 0; x < 16; ++x)
@@ -753,9 +755,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const uint32_t sp = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
 #pragma unroll 1
         for (int s = 0; s < 8; ++s) {
-          const uint32_t p_hi = sp + (uint32_t)((s >> 1) * 32 + (s & 1) * 8), bh = desc_mn(v_hi + s * 2048);
+          const uint32_t p_hi = sp + (uint32_t)(s * 16), bh = desc_mn(v_hi + s * 2048);
           mma_f16_ts(toi, p_hi, bh, id_intra, s > 0);
-          mma_f16_ts(toi, p_hi + 16, bh, id_intra, 1u);
+          mma_f16_ts(toi, p_hi + 8, bh, id_intra, 1u);
           mma_f16_ts(toi, p_hi, bh + (kTileB >> 4), id_intra, 1u);
         }
         umma_commit(bar_o);
