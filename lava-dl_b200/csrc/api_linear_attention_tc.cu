@@ -41,10 +41,16 @@
 // A head with T steps is one CTA, or several when there are fewer heads than SMs: the axis is then cut
 // into segments, a first launch takes each segment's growth from zero, a small one joins them, and the
 // walk starts every segment from its own state.
+#include <string.h>
+
 #include "linear_attention.cuh"
 #include "tc.cuh"
 
 namespace sb {
+
+int make_map_5d(CUtensorMap* out, const void* base, const uint64_t (&dims)[5], const uint64_t (&strides)[4],
+                const uint32_t (&box)[5], int swizzle);
+
 namespace la {
 namespace {
 
@@ -55,18 +61,20 @@ constexpr int kThreads = 768;
 // the vectors live.  Each row adds up to 6 * 80.
 template <int KT>
 struct Regs {
-  static constexpr int load = KT == 1 ? 96 : 88, p = KT == 1 ? 80 : 72, s = KT == 1 ? 88 : 112, mma = 24;
+  static constexpr int load = KT == 1 ? 96 : 88, p = KT == 1 ? 72 : 64, s = KT == 1 ? 80 : 112, mma = 40;
   static_assert(3 * load + p + s + mma <= 480, "more registers than the block was launched with");
 };
 constexpr int kMaxSub = 6;
 
 struct TcArgs {
+  CUtensorMap map[3][3];   // q, k, v of each walk in boxes of 64 rows and 128 steps, when `boxes`
   Walk w[3];
   float* seg[3];        // [nseg][heads][Dk * Dv]: states after each segment
   int nsub;             // CTAs per head and segment: (walk, 64 columns of v)
   int sub_walk[kMaxSub], sub_e0[kMaxSub];
   int64_t heads;
   int nseg, seg_chunks;
+  int boxes;            // TMA can describe the tensors: 16-byte bases, T % 4 == 0
   unsigned int* status;
 };
 
@@ -74,10 +82,12 @@ template <int KT>
 struct Shape {
   static constexpr int stages = KT == 1 ? 2 : 1;      // KT = 2 has room for one
   static constexpr int nsp = KT == 1 ? 2 : 1;         // score accumulators
-  static constexpr int stage_bytes = (2 * KT + 4) * kTileB;
-  static constexpr int state_bytes = 2 * KT * 64 * 128;
-  static constexpr int score = KT == 1 ? 34 : 35;     // 2^14 2^14 Dk
-  static constexpr int smem = 1024 + stages * stage_bytes + state_bytes;
+  static constexpr int score = KT == 1 ? 34 : 35;     // scores of the scaled vectors are below 2^score: 2^14 2^14 Dk
+  // shared memory: k, v (hi and lo tiles; the raw fp32 tile they are converted from lies in the same
+  // place), weighted v, raw q (KT = 1), state
+  static constexpr int k_bytes = 2 * KT * kTileB, v_at = stages * k_bytes, v_bytes = 2 * kTileB,
+                       vw_at = v_at + stages * v_bytes, q_at = vw_at + v_bytes, s_at = q_at + (KT == 1 ? v_bytes : 0);
+  static constexpr int smem = 1024 + s_at + 2 * KT * 64 * 128;
   // tensor memory columns
   static constexpr uint32_t q = 0, sp = 64 * KT, oi = sp + 128 * nsp, ox = oi + 64, ds = ox + 64;
 };
@@ -141,11 +151,6 @@ __device__ __forceinline__ void split2(uint64_t x, uint32_t* hi, uint32_t* lo) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(*lo) : "f"(d.y), "f"(d.x));
   *hi = h;
 }
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
-               ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
 // D (+)= A B^T, fp16 operands, fp32 accumulator: A in tensor memory or shared memory, B in shared memory
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -207,6 +212,22 @@ __device__ __forceinline__ void load64(uint64_t (&x)[32], const float* p, int64_
     }
   }
 }
+// the same out of a raw tile [64][128] in shared memory (rows and steps outside the tensor are zeros)
+__device__ __forceinline__ void load64_shared(uint64_t (&x)[32], uint32_t p) {
+#pragma unroll
+  for (int d = 0; d < 32; ++d) {
+    float a, b;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(p + d * 1024));
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(p + d * 1024 + 512));
+    x[d] = pair(a, b);
+  }
+}
+__device__ __forceinline__ void tma_load_box(uint32_t dst, const CUtensorMap* map, int t, int row, int head, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %5}], [%6];"
+      ::"r"(dst), "l"(map), "r"(t), "r"(row), "r"(head), "r"(0), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ float top64(const uint64_t (&x)[32], float m = 0.f) {
 #pragma unroll
   for (int d = 0; d < 32; ++d) {
@@ -245,22 +266,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   __shared__ float scan_s[2][4];
   __shared__ int kmax_s[2][8];
   __shared__ float pow_pad[32 + kL + 1];       // r^n at 32 + n; zeros before it are the causal mask
-  __shared__ float scale_s[2][64];
+  __shared__ __align__(16) float scale_s[2][64];
   __shared__ float top_s[kL];
   __shared__ int poison_s[64];
   __shared__ int any_poison_s, dead_s;
   __shared__ uint32_t tmem_s;
-  __shared__ __align__(8) uint64_t bars[20];
+  __shared__ __align__(8) uint64_t bars[26];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = tid >> 7, th = tid & 127, tw = warp & 3;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t sbase = base + NS * S_::stage_bytes;
+  const uint32_t sbase = base + S_::s_at;
   volatile int* dead = &dead_s;
   volatile int* any_poison = &any_poison_s;
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t bar_k = bar0, bar_v = bar0 + 16, bar_free = bar0 + 32, bar_sp = bar0 + 48, bar_kx = bar0 + 64;   // two each
   const uint32_t bar_q = bar0 + 80, bar_qfree = bar0 + 88, bar_p = bar0 + 96, bar_ds = bar0 + 104, bar_s = bar0 + 112,
-                 bar_o = bar0 + 120, bar_ofree = bar0 + 128, bar_end = bar0 + 136;
+                 bar_o = bar0 + 120, bar_ofree = bar0 + 128, bar_end = bar0 + 144;
+  const uint32_t bar_kraw = bar0 + 152, bar_vraw = bar0 + 168, bar_qraw = bar0 + 184, bar_qread = bar0 + 192;   // k, v: two
 
   // which head, segment, walk and columns
   const int64_t bid = blockIdx.x;
@@ -274,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   const int64_t c0 = (int64_t)seg * args.seg_chunks;
   const int nc = (int)min((int64_t)args.seg_chunks, (T + kL - 1) / kL - c0);
   const int after = w.after;
+  const bool boxes = KT == 1 && args.boxes != 0;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -282,9 +305,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mbar_init(bar_free + 8 * i, 1);
       mbar_init(bar_sp + 8 * i, 2);
       mbar_init(bar_kx + 8 * i, 128);
+      mbar_init(bar_kraw + 8 * i, 1);
+      mbar_init(bar_vraw + 8 * i, 1);
     }
+    mbar_init(bar_qraw, 1);
+    mbar_init(bar_qread, 128);
     mbar_init(bar_q, 128);
-    mbar_init(bar_qfree, 1);
+    mbar_init(bar_qfree, 2);
     mbar_init(bar_p, 128);
     mbar_init(bar_ds, 2);
     mbar_init(bar_s, 128);
@@ -318,9 +345,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   const uint32_t trow = tmem + ((uint32_t)(tw * 32) << 16);   // this warp's lanes of tensor memory
 
   if (role < 3) {
-    // ---------------- k, v, q: load, convert, hand on; the same instructions for the three ----------------
+    // ---------------- k, v, q: load, convert, hand on ----------------
     regs_inc<Regs<KT>::load>();
     const int j = th;
+    // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
+    const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
     const bool is_k = role == 0, is_v = role == 1, is_q = role == 2;
     const float* src = is_k ? w.k + head * (int64_t)Dk * T
                             : (is_v ? w.v + (head * (int64_t)w.Dv + e0) * T : w.q + head * (int64_t)Dk * T);
@@ -329,22 +358,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     // is converted while it is there, then the first half again.  v: as it is, and weighted.
     const int passes = is_v ? (FULL ? 2 : 1) : (KT == 2 ? 3 : 1);
     const int mid = is_v ? 0 : KT - 1;           // the pass after whose load the exponent is known
-    // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
-    const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
-    uint64_t x[32];
 #pragma unroll 1
     for (int c = (FULL || !is_q) ? 0 : nc; c < nc; ++c) {
-      const uint32_t stage = base + (uint32_t)(c % NS) * S_::stage_bytes;
+      const uint32_t slot = base + (is_k ? (uint32_t)(c % NS) * S_::k_bytes
+                                         : (is_v ? S_::v_at + (uint32_t)(c % NS) * S_::v_bytes : S_::q_at));
       const int64_t t = (c0 + c) * kL + j;
       const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
       const bool in = j < len, whole = len == kL;
       const float* at = src + (w.reverse ? T - 1 - t : t);
+      uint64_t x[32];
       float top = 0.f, scale = 0.f, scale_w = 0.f;
       bool zero = false;                         // the whole vector is left out
 #pragma unroll 1
       for (int pass = 0; pass < passes; ++pass) {
         const int half = (KT == 2 && !is_v && pass == 1) ? 1 : 0;
-        if (!is_v || pass == 0) load64(x, at + (int64_t)half * 64 * T, T, rows - half * 64, in, whole);
+        if (!is_v || pass == 0) {
+          if (boxes) {
+            // the raw tile, a step earlier or later in memory by direction; its place is free to be written
+            // (k, v) or to receive the next tile (q) once the whole warpgroup has read it
+            wait_or_dead(is_q ? bar_qraw : (is_k ? bar_kraw : bar_vraw) + 8 * (c % NS),
+                         is_q ? (uint32_t)c & 1u : (uint32_t)(c / NS) & 1u, dead);
+            load64_shared(x, slot + (uint32_t)(w.reverse ? kL - 1 - j : j) * 4);
+            if (is_q) mbar_arrive(bar_qread);
+            else bar_sync(3 + role, 128);
+          } else {
+            load64(x, at + (int64_t)half * 64 * T, T, rows - half * 64, in, whole);
+          }
+        }
         if (pass <= mid) top = top64(x, top);
         if (pass == mid) {
           const bool bad = not_finite(top);
@@ -356,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
             const int f = fit_exponent(bad ? 0.f : top);
             scale = p2(-f);
-            if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+            if (!boxes && c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
             f_s[c & 1][j] = bad ? kNoTerm - 1 : (top > 0.f ? f : kNoTerm);
             mbar_arrive(bar_kx + 8 * (c & 1));
           } else if (is_q) {
@@ -414,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
               mw = max(mw, kmax_s[c & 1][i]);
               mc = max(mc, kmax_s[c & 1][4 + i]);
             }
-            if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+            if (!boxes && c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
             if (FULL) {
               col_s[c & 1][j] = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
               m_s[c & 3][j] = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
@@ -440,14 +480,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             for (int d = 0; d < 32; ++d) x[d] = 0;
           }
         }
-        // one row of a hi and a lo tile (128-byte swizzle), or of q's columns of tensor memory
         const bool weighted = is_v && (!FULL || pass == 1);
-        const uint32_t tile = stage + (is_v ? (uint32_t)(2 * KT + (weighted ? 2 : 0)) * kTileB : (uint32_t)half * kTileB) +
-                              (uint32_t)(j * 128);
-        const uint32_t lo_at = is_v ? kTileB : KT * kTileB;
-        const uint32_t tq = trow + S_::q + half * 32;
         if (FULL && weighted) scale = scale_w;
         const uint64_t sc = pair(scale, scale);
+        if (is_q) {
+          // 16 channels of q (one step of an MMA) are 8 columns of hi and 8 of lo, side by side: one store
+#pragma unroll
+          for (int b = 0; b < 32; b += 8) {
+            uint32_t r[16];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) split2(mul2(x[b + e], sc), &r[e], &r[8 + e]);
+            tmem_st16(trow + S_::q + half * 64 + 2 * b, r);
+          }
+          if constexpr (KT == 1) break;          // (x is not carried on)
+          continue;
+        }
+        // one row of a hi and a lo tile (128-byte swizzle)
+        if (weighted && c >= 1) wait_or_dead(bar_ds, (uint32_t)(c - 1) & 1u, dead);    // read by the growth before
+        const uint32_t tile = (weighted ? base + S_::vw_at : slot + (uint32_t)half * kTileB) + (uint32_t)(j * 128);
+        const uint32_t lo_at = is_v ? kTileB : KT * kTileB;
 #pragma unroll
         for (int q8 = 0; q8 < 8; ++q8) {
           uint32_t h[4], l[4];
@@ -456,24 +507,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             x[4 * q8 + e] = mul2(x[4 * q8 + e], sc);       // v's weights come on top of its scale
             split2(x[4 * q8 + e], &h[e], &l[e]);
           }
-          if (is_q) {
-            tmem_st4(tq + q8 * 4, h[0], h[1], h[2], h[3]);
-            tmem_st4(tq + 32 * KT + q8 * 4, l[0], l[1], l[2], l[3]);
-          } else {
-            const uint32_t to = tile + (uint32_t)((q8 ^ (j & 7)) << 4);
-            sts128(to, h[0], h[1], h[2], h[3]);
-            sts128(to + lo_at, l[0], l[1], l[2], l[3]);
-          }
+          const uint32_t to = tile + (uint32_t)((q8 ^ (j & 7)) << 4);
+          sts128(to, h[0], h[1], h[2], h[3]);
+          sts128(to + lo_at, l[0], l[1], l[2], l[3]);
         }
       }
-      if (is_q) {
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(bar_q);
-      } else {
+      if (is_k || is_v) {
         fence_proxy_async();
         mbar_arrive((is_k ? bar_k : bar_v) + 8 * (c % NS));
+        continue;
       }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(bar_q);
     }
   } else if (role == 3) {
     // ---------------- scores -> P: thread = row i ----------------
@@ -492,27 +538,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const float* pw = &pow_pad[32 + l];      // r^(i - j), zero for j > i: the mask
         const float* col = col_s[c & 1];
 #pragma unroll 1
-        for (int g = 0; g < 128; g += 16, pw -= 16, col += 16) {
-          uint32_t hi[8], lo[8];
-          if (g < tw * 32 + 32) {
-            uint32_t r[16];
-            tmem_ld16(sp + g, r);
+        for (int g = 0; g < 128; g += 32, pw -= 32, col += 32) {
+          uint32_t s[32];                        // 16 columns of hi and 16 of lo, in the place of 32 scores
+          if (g <= tw * 32) {
+            uint32_t r[32];
+            tmem_ld32(sp + g, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int jj = 0; jj < 16; jj += 4) {
+            for (int jj = 0; jj < 32; jj += 4) {
               const float4 cf = *reinterpret_cast<const float4*>(col + jj);
               // the power first: its zeros take whatever the steps after i hold
               const uint64_t x = mul2(pair(__uint_as_float(r[jj]), __uint_as_float(r[jj + 1])), pair(pw[-jj], pw[-jj - 1]));
               const uint64_t y = mul2(pair(__uint_as_float(r[jj + 2]), __uint_as_float(r[jj + 3])), pair(pw[-jj - 2], pw[-jj - 3]));
-              split2(mul2(mul2(x, pair(cf.x, cf.y)), rf), &hi[jj / 2], &lo[jj / 2]);
-              split2(mul2(mul2(y, pair(cf.z, cf.w)), rf), &hi[jj / 2 + 1], &lo[jj / 2 + 1]);
+              split2(mul2(mul2(x, pair(cf.x, cf.y)), rf), &s[jj / 2], &s[16 + jj / 2]);
+              split2(mul2(mul2(y, pair(cf.z, cf.w)), rf), &s[jj / 2 + 1], &s[17 + jj / 2]);
             }
           } else {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) hi[x] = lo[x] = 0u;
+            for (int x = 0; x < 32; ++x) s[x] = 0u;
           }
-          tmem_st8(sp + g, hi);
-          tmem_st8(sp + g + 8, lo);
+          tmem_st32(sp + g, s);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -520,8 +565,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
     }
   } else if (role == 4) {
-    // ---------------- state (column e, half of Dk) and output (step i) ----------------
-    regs_inc<Regs<KT>::s>();
+    // ---------------- state (thread = column e, half of Dk) and output (thread = step i) ----------------
+    if constexpr (Regs<KT>::s > 80) regs_inc<Regs<KT>::s>();
     const int l = th, e = l & 63, half = l >> 6;
     constexpr int NSt = 32 * KT;                 // state elements per thread: d = half * NSt ...
     float St[NSt];
@@ -563,13 +608,69 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       fence_proxy_async();
     };
-    // two call sites in one: c = -1 publishes the state the walk starts from
+    // Trip c writes the output of chunk c - 1, then takes the state over chunk c: the published state is
+    // replaced once the MMAs of chunk c have read it.  Trip -1 publishes what the walk starts from.
 #pragma unroll 1
-    for (int c = -1; c < nc; ++c) {
+    for (int c = -1; c <= (FULL ? nc : nc - 1); ++c) {
+      if (FULL && c >= 1) {
+        const int p = c - 1;                     // the chunk whose output this is
+        const int64_t t = (c0 + p) * kL + l;
+        float* out = w.o + (head * (int64_t)w.Dv + e0) * T + (w.reverse ? T - 1 - t : t);
+        const bool live = t < T, plain = (c0 + p + 1) * kL <= T && ne == 64;
+        wait_or_dead(bar_o, (uint32_t)p & 1u, dead);
+        tc_fence_after();
+        const int qe = qe_s[p & 3][l], m = m_s[p & 3][l] + S_::score - 15;
+        const bool bad = qe == 0x7fffffff;
+        const Factors fi = p2_wide((bad ? 0 : qe) + m), fx = p2_wide(bad ? 0 : qe);
+        const float nan = __int_as_float(0x7fffffff), rowx = fx.b * pow_pad[32 + l + after];
+        const uint64_t ia = pair(bad ? nan : fi.a, bad ? nan : fi.a), ib = pair(fi.b, fi.b), xa = pair(fx.a, fx.a),
+                       xb = pair(rowx, rowx);
+#pragma unroll 1
+        for (int b = 0; b < 64; b += 16) {
+          uint32_t ri[16], rx[16];
+          tmem_ld16(trow + S_::oi + b, ri);
+          tmem_ld16(trow + S_::ox + b, rx);
+          tmem_ld_wait();
+          if (b == 48) {
+            tc_fence_before();
+            mbar_arrive(bar_ofree);
+          }
+          const float* sc = &scale_s[p & 1][b];
+          float y[16];
+#pragma unroll
+          for (int x = 0; x < 16; x += 2) {
+            const uint64_t inter = mul2(mul2(pair(__uint_as_float(rx[x]), __uint_as_float(rx[x + 1])), xa),
+                                        mul2(pair(sc[x], sc[x + 1]), xb));
+            const float2 v = unpair(fma2(mul2(pair(__uint_as_float(ri[x]), __uint_as_float(ri[x + 1])), ia), ib, inter));
+            y[x] = v.x;
+            y[x + 1] = v.y;
+          }
+          if (plain) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              *out = y[x];
+              out += T;
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              if (live && b + x < ne) *out = y[x];
+              out += T;
+            }
+          }
+        }
+        if (*any_poison != 0 && live) {          // spoilt columns
+          out -= 64 * T;
+          for (int x = 0; x < ne; ++x)
+            if (poison_s[x] <= (int)t) out[(int64_t)x * T] = nan;
+        }
+      }
+      if (c == nc) break;
       if (c >= 0) {
         // the state after chunk c
         const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
         wait_or_dead(bar_ds, (uint32_t)c & 1u, dead);
+        if (FULL) wait_or_dead(bar_qfree, (uint32_t)c & 1u, dead);     // the published state has been read
         tc_fence_after();
         const Factors mw = p2_wide(mw_s[c & 3]);
         const float carry = pow_pad[32 + len];
@@ -613,60 +714,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       if (FULL && c + 1 < nc) publish((c + 1) & 1);      // its barrier also ends the exchange
       else bar_sync(2, 128);
       mbar_arrive(bar_s);
-      if (FULL && c >= 0) {
-        const int64_t t = (c0 + c) * kL + l;
-        const int64_t tt = w.reverse ? T - 1 - t : t;
-        float* out = w.o + (head * (int64_t)w.Dv + e0) * T + tt;
-        const bool live = t < T, plain = (c0 + c + 1) * kL <= T && ne == 64;
-        wait_or_dead(bar_o, (uint32_t)c & 1u, dead);
-        tc_fence_after();
-        const int qe = qe_s[c & 3][l], m = m_s[c & 3][l] + S_::score - 15;
-        const bool bad = qe == 0x7fffffff;
-        const Factors fi = p2_wide((bad ? 0 : qe) + m), fx = p2_wide(bad ? 0 : qe);
-        const float nan = __int_as_float(0x7fffffff);
-        const float ia = bad ? nan : fi.a, ib = fi.b, xa = fx.a, xb = fx.b * pow_pad[32 + l + after];
-        const bool poisoned = *any_poison != 0;
-#pragma unroll 1
-        for (int b = 0; b < 64; b += 16) {
-          uint32_t ri[16], rx[16];
-          tmem_ld16(trow + S_::oi + b, ri);
-          tmem_ld16(trow + S_::ox + b, rx);
-          tmem_ld_wait();
-          if (b == 48) {
-            tc_fence_before();
-            mbar_arrive(bar_ofree);
-          }
-          const float* sc = &scale_s[c & 1][b];
-          float y[16];
-#pragma unroll
-          for (int x = 0; x < 16; x += 2) {
-            const uint64_t inter = mul2(mul2(pair(__uint_as_float(rx[x]), __uint_as_float(rx[x + 1])), pair(xa, xa)),
-                                        mul2(pair(sc[x], sc[x + 1]), pair(xb, xb)));
-            const float2 v = unpair(fma2(mul2(pair(__uint_as_float(ri[x]), __uint_as_float(ri[x + 1])), pair(ia, ia)),
-                                         pair(ib, ib), inter));
-            y[x] = v.x;
-            y[x + 1] = v.y;
-          }
-          if (poisoned) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-              if (poison_s[b + x] <= (int)t) y[x] = nan;
-          }
-          if (plain) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              *out = y[x];
-              out += T;
-            }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              if (live && b + x < ne) *out = y[x];
-              out += T;
-            }
-          }
-        }
-      }
     }
     // the state after the last chunk
     float* dst = nullptr;
@@ -699,40 +746,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         ok = wait_or_dead(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         if (!ok) return;
         tc_fence_after();
-        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::stage_bytes, d = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
+        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes, d = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
 #pragma unroll 1
         for (int s = 0; s < 4 * KT; ++s) {
           const uint32_t bh = desc_lo(k_hi + (uint32_t)((s >> 2) * kTileB + (s & 3) * 32));
-          mma_f16_ts(d, tq + s * 8, bh, id_scores, s > 0);
-          mma_f16_ts(d, tq + 32 * KT + s * 8, bh, id_scores, 1u);
-          mma_f16_ts(d, tq + s * 8, bh + (KT * kTileB >> 4), id_scores, 1u);
+          const uint32_t q_hi = tq + (uint32_t)s * 16;
+          mma_f16_ts(d, q_hi, bh, id_scores, s > 0);
+          mma_f16_ts(d, q_hi + 8, bh, id_scores, 1u);
+          mma_f16_ts(d, q_hi, bh + (KT * kTileB >> 4), id_scores, 1u);
         }
         umma_commit(bar_sp + 8 * (c % NSP));
         mbar_arrive(bar_sp + 8 * (c % NSP));
       };
       if (FULL) scores(0);
+      // Growth first, it waits for nothing but the state's warps; then the state's part of the output, for
+      // which the output before has to be taken away; with two score accumulators the next scores run ahead
+      // of the read-out, so that P is made while the MMAs go on.
 #pragma unroll 1
       for (int c = 0; c < nc && ok; ++c) {
-        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::stage_bytes, v_hi = k_hi + 2 * KT * kTileB,
-                       vw_hi = v_hi + 2 * kTileB;
+        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes,
+                       v_hi = base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, vw_hi = base + S_::vw_at;
         ok = wait_or_dead(bar_s, (uint32_t)c & 1u, dead) && ok;
-        if (FULL) {
-          if (c >= 1) ok = wait_or_dead(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
-        } else {
-          ok = wait_or_dead(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
-        }
-        if (!ok) break;
-        tc_fence_after();
-        if (FULL) {
-#pragma unroll 1
-          for (int s = 0; s < 4 * KT; ++s) {
-            const uint32_t bh = desc_lo(sbase + (uint32_t)((s >> 2) * 8192 + (s & 3) * 32));
-            mma_f16_ts(tox, tq + s * 8, bh, id_inter, s > 0);
-            mma_f16_ts(tox, tq + 32 * KT + s * 8, bh, id_inter, 1u);
-            mma_f16_ts(tox, tq + s * 8, bh + (KT * 8192 >> 4), id_inter, 1u);
-          }
-          umma_commit(bar_qfree);
-        }
+        if (!FULL) ok = wait_or_dead(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         ok = wait_or_dead(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();
@@ -748,6 +783,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           umma_commit(bar_free + 8 * (c % NS));
           continue;
         }
+        if (c >= 1) ok = wait_or_dead(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int s = 0; s < 4 * KT; ++s) {
+          const uint32_t bh = desc_lo(sbase + (uint32_t)((s >> 2) * 8192 + (s & 3) * 32));
+          const uint32_t q_hi = tq + (uint32_t)s * 16;
+          mma_f16_ts(tox, q_hi, bh, id_inter, s > 0);
+          mma_f16_ts(tox, q_hi + 8, bh, id_inter, 1u);
+          mma_f16_ts(tox, q_hi, bh + (KT * 8192 >> 4), id_inter, 1u);
+        }
+        umma_commit(bar_qfree);
+        mbar_arrive(bar_qfree);
         if (NSP == 2 && c + 1 < nc) scores(c + 1);
         ok = wait_or_dead(bar_p, (uint32_t)c & 1u, dead) && ok;
         if (!ok) break;
@@ -755,9 +803,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const uint32_t sp = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
 #pragma unroll 1
         for (int s = 0; s < 8; ++s) {
-          const uint32_t p_hi = sp + (uint32_t)(s * 16), bh = desc_mn(v_hi + s * 2048);
+          const uint32_t p_hi = sp + (uint32_t)((s >> 1) * 32 + (s & 1) * 8), bh = desc_mn(v_hi + s * 2048);
           mma_f16_ts(toi, p_hi, bh, id_intra, s > 0);
-          mma_f16_ts(toi, p_hi + 8, bh, id_intra, 1u);
+          mma_f16_ts(toi, p_hi + 16, bh, id_intra, 1u);
           mma_f16_ts(toi, p_hi, bh + (kTileB >> 4), id_intra, 1u);
         }
         umma_commit(bar_o);
@@ -767,6 +815,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       umma_commit(bar_end);          // everything issued has landed before tensor memory is given back
       if (!mbar_wait(bar_end, 0)) *dead = 1;
+    } else if (KT == 1 && th == 32 && boxes) {
+      // ---------------- raw tiles, one TMA box each ----------------
+      const CUtensorMap* maps = args.map[wi];
+      int issued[3] = {0, 0, 0};
+#pragma unroll 1
+      for (int c = 0; c < nc; ++c) {
+        const int64_t t = (c0 + c) * kL;
+        const int from = (int)(w.reverse ? T - t - kL : t);      // walking back, the last box may start before 0
+        if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+        if (*dead) break;
+        const uint32_t bk = bar_kraw + 8 * (c % NS), bv = bar_vraw + 8 * (c % NS);
+        mbar_expect_tx(bk, 2 * kTileB);
+        tma_load_box(base + (uint32_t)(c % NS) * S_::k_bytes, &maps[1], from, 0, (int)head, bk);
+        issued[0] = c + 1;
+        mbar_expect_tx(bv, 2 * kTileB);
+        tma_load_box(base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, &maps[2], from, e0, (int)head, bv);
+        issued[1] = c + 1;
+        if (FULL) {
+          if (c >= 1) wait_or_dead(bar_qread, (uint32_t)(c - 1) & 1u, dead);
+          if (*dead) break;
+          mbar_expect_tx(bar_qraw, 2 * kTileB);
+          tma_load_box(base + S_::q_at, &maps[0], from, 0, (int)head, bar_qraw);
+          issued[2] = c + 1;
+        }
+      }
+      if (*dead) {   // nobody may have waited for the boxes in flight: not before they have landed
+        for (int c = max(issued[0] - 2, 0); c < issued[0]; ++c) mbar_wait(bar_kraw + 8 * (c % NS), (uint32_t)(c / NS) & 1u);
+        for (int c = max(issued[1] - 2, 0); c < issued[1]; ++c) mbar_wait(bar_vraw + 8 * (c % NS), (uint32_t)(c / NS) & 1u);
+        if (issued[2] > 0) mbar_wait(bar_qraw, (uint32_t)(issued[2] - 1) & 1u);
+      }
     }
     __syncwarp();
   }
@@ -848,7 +926,8 @@ static int go(const TcArgs& a, cudaStream_t s) {
 
 // Walks of one launch: the same heads and T, Dk on the same side of 64.
 int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
-  TcArgs a{};
+  TcArgs a;
+  memset(&a, 0, sizeof(a));
   int64_t ctas = 0;
   a.nsub = 0;
   for (int i = 0; i < n; ++i) {
@@ -868,6 +947,19 @@ int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
     for (int i = 0; i < n; ++i) {
       a.seg[i] = p;
       p += (int64_t)(a.nseg - 1) * a.heads * walks[i].Dk * walks[i].Dv;
+    }
+  }
+  uintptr_t bits = 0;
+  for (int i = 0; i < n; ++i) bits |= (uintptr_t)walks[i].q | (uintptr_t)walks[i].k | (uintptr_t)walks[i].v;
+  a.boxes = walks[0].Dk <= 64 && (bits & 15u) == 0 && walks[0].T % 4 == 0;
+  for (int i = 0; i < n && a.boxes; ++i) {
+    const Walk& w = walks[i];
+    const float* base[3] = {w.q, w.k, w.v};
+    for (int x = 0; x < 3; ++x) {
+      const uint64_t D = (uint64_t)(x == 2 ? w.Dv : w.Dk), row = (uint64_t)w.T * 4, all = row * D * (uint64_t)w.heads;
+      const uint64_t dims[5] = {(uint64_t)w.T, D, (uint64_t)w.heads, 1, 1}, strides[4] = {row, row * D, all, all};
+      const uint32_t box[5] = {kL, 64, 1, 1, 1};
+      SB_TRY(make_map_5d(&a.map[i][x], base[x], dims, strides, box, 0));
     }
   }
   a.status = status_ptr();
