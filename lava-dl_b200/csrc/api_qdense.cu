@@ -9,6 +9,7 @@
 // the product is then the float synapse's, bit for bit.  A time step with a value that is not finite
 // gives NaN for all of its outputs.
 #include "api_util.cuh"
+#include "tc.cuh"
 
 using namespace sb;
 
@@ -112,13 +113,238 @@ int launch_few(const float* x, const int8_t* w, const float* ws, float* y, int64
   return SB_OK;
 }
 
+
+// ---------------------------------------------------------------------------
+// Many tokens, first pass: x [n][k][t] -> xq [token][k] (rows of Kp bytes, zeros past K) and the steps.
+// A block owns 32 consecutive time steps of a sample and walks all of their inputs twice, once for the
+// largest magnitude and once to round; the second walk reads what the first has left in L2 (the blocks in
+// flight hold 32 K floats each, 78 MB at K = 2048).  A lane is a time step: loads of 128 contiguous bytes,
+// and 32 neighbouring inputs of a step packed in its registers to one whole sector.
+// ---------------------------------------------------------------------------
+constexpr int kQThreads = 512, kQWarps = kQThreads / 32;
+
+__global__ void __launch_bounds__(kQThreads, 2)
+qdense_quantize_kernel(const float* __restrict__ x, int8_t* __restrict__ xq, float* __restrict__ steps, int K, int Kp,
+                       int64_t T, int64_t tiles_t) {
+  __shared__ uint32_t top_s[kQWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n = blockIdx.x / tiles_t, t = (blockIdx.x - n * tiles_t) * 32 + lane;
+  const bool in = t < T;
+  const float* src = x + n * K * T + (in ? t : 0);
+  uint32_t top = 0;
+#pragma unroll 1
+  for (int k0 = warp * 32; k0 < K; k0 += kQWarps * 32) {
+    float v[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = k0 + e < K ? __ldg(src + (int64_t)(k0 + e) * T) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+  }
+  top_s[warp][lane] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQWarps; ++w) top = max(top, top_s[w][lane]);
+  float step, inv;
+  step_of(top, &step, &inv);
+  const int64_t token = n * T + t;
+  if (warp == 0 && in) steps[token] = step;
+#pragma unroll 1
+  for (int k0 = warp * 32; k0 < Kp; k0 += kQWarps * 32) {
+    float v[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = k0 + e < K ? __ldg(src + (int64_t)(k0 + e) * T) : 0.f;
+    uint32_t p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int a = __float2int_rn(v[4 * e] * inv), b = __float2int_rn(v[4 * e + 1] * inv),
+                c = __float2int_rn(v[4 * e + 2] * inv), d = __float2int_rn(v[4 * e + 3] * inv);
+      p[e] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    }
+    if (in) {
+      uint4* dst = reinterpret_cast<uint4*>(xq + token * Kp + k0);
+      dst[0] = make_uint4(p[0], p[1], p[2], p[3]);
+      if (k0 + 16 < Kp) dst[1] = make_uint4(p[4], p[5], p[6], p[7]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Second pass: D[token][o] = xq w^T on the tensor cores (kind::i8, 32-bit sums in tensor memory).
+// Tokens are the rows of a tile, so that a warp's 32 lanes write 32 neighbouring time steps of one output
+// neuron.  One persistent CTA per SM: a thread fetches 128-byte-wide boxes of both operands into a ring of
+// stages, a thread issues the MMAs (32 inputs each), eight warps take a finished tile out of one half of
+// tensor memory while the next one is summed in the other.
+// ---------------------------------------------------------------------------
+constexpr int kStages = 4, kGThreads = 320, kTM = 128, kTK = 128;
+
+__device__ __forceinline__ void mma_i8(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(acc)
+      : "memory");
+}
+// signed 8-bit operands, both K-major, 32-bit integer accumulator
+__host__ __device__ constexpr uint32_t idesc_i8(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTM >> 4) << 24);
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kGThreads, 1)
+qdense_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                   const float* __restrict__ steps, const float* __restrict__ ws, float* __restrict__ y, int64_t tokens,
+                   int kblocks, int O, int64_t T, int tiles_n, int64_t tiles, unsigned int* status) {
+  constexpr int kStageBytes = (kTM + NT) * kTK;
+  constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
+  __shared__ int dead_s;
+  __shared__ uint32_t tmem_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  volatile int* dead = &dead_s;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, done = empty + 8 * kStages, taken = done + 16;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(done + 8 * i, 1);
+      mbar_init(taken + 8 * i, 256);
+    }
+    fence_mbar_init();
+    dead_s = 0;
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_s)), "r"(kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int64_t tile = blockIdx.x; tile < tiles && !*dead; tile += gridDim.x) {
+        const int m0 = (int)(tile / tiles_n) * kTM, n0 = (int)(tile % tiles_n) * NT;
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const uint32_t s = it % kStages;
+          if (it >= kStages && !wait_or_dead(empty + 8 * s, (it / kStages - 1u) & 1u, dead)) break;
+          mbar_expect_tx(full + 8 * s, kStageBytes);
+          tma_load_2d(base + s * kStageBytes, &amap, kb * (kTK / 4), m0, full + 8 * s);
+          tma_load_2d(base + s * kStageBytes + kTM * kTK, &bmap, kb * (kTK / 4), n0, full + 8 * s);
+        }
+      }
+      if (*dead)   // boxes in flight land before the memory is given back
+        for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j) mbar_wait(full + 8 * (j % kStages), (j / kStages) & 1u);
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      uint32_t it = 0, nt = 0;
+      bool ok = true;
+      for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++nt) {
+        const uint32_t acc = nt & 1u, d = tmem + acc * NT;
+        if (nt >= 2) ok = wait_or_dead(taken + 8 * acc, (nt / 2 - 1u) & 1u, dead);
+        tc_fence_after();
+        for (int kb = 0; kb < kblocks && ok; ++kb, ++it) {
+          const uint32_t s = it % kStages;
+          ok = wait_or_dead(full + 8 * s, (it / kStages) & 1u, dead);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a = desc_lo(base + s * kStageBytes), b = desc_lo(base + s * kStageBytes + kTM * kTK);
+#pragma unroll
+          for (uint32_t k = 0; k < kTK / 32; ++k) mma_i8(d, a + 2 * k, b + 2 * k, idesc_i8(NT), (uint32_t)(kb > 0 || k > 0));
+          umma_commit(empty + 8 * s);
+        }
+        umma_commit(done + 8 * acc);
+      }
+      if (nt > 0) mbar_wait(done + 8 * ((nt - 1) & 1u), ((nt - 1) / 2) & 1u);
+    }
+  } else {
+    // eight warps: lanes 32 (warp % 4) ... of the tile, columns by halves
+    const int quarter = warp & 3, half = warp >> 2;
+    constexpr int kMine = NT / 2;                        // columns of this warp
+    uint32_t nt = 0;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++nt) {
+      const uint32_t acc = nt & 1u;
+      const int64_t m = (tile / tiles_n) * kTM + quarter * 32 + lane;
+      const int n0 = (int)(tile % tiles_n) * NT + half * kMine;
+      const bool live = m < tokens;
+      const int64_t n = live ? m / T : 0;
+      float* out = y + (n * O + n0) * T + (live ? m - n * T : 0);
+      const float step = live ? __ldg(steps + m) : 0.f;
+      const bool ok = wait_or_dead(done + 8 * acc, (nt / 2) & 1u, dead);
+      tc_fence_after();
+      const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + acc * NT + half * kMine;
+#pragma unroll 1
+      for (int c = 0; c < kMine; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(src + c, r);
+        tmem_ld_wait();
+        if (c + 32 >= kMine) {
+          tc_fence_before();
+          mbar_arrive(taken + 8 * acc);
+        }
+        if (!ok || !live) continue;
+        const int left = O - (n0 + c);
+        if (left >= 32) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) out[(int64_t)(c + e) * T] = (float)(int)r[e] * __ldg(ws + n0 + c + e) * step;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (e < left) out[(int64_t)(c + e) * T] = (float)(int)r[e] * __ldg(ws + n0 + c + e) * step;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*dead && tid == 0) dev_flag(status, SB_DEV_TMA_TIMEOUT);
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+  }
+}
+
+template <int NT>
+int launch_gemm(const int8_t* xq, const float* steps, const int8_t* w, const float* ws, float* y, int64_t tokens, int Kp,
+                int O, int64_t T, cudaStream_t s) {
+  CUtensorMap amap, bmap;
+  SB_TRY(make_row_map_box(&amap, xq, tokens, Kp / 4, 32, kTM));
+  SB_TRY(make_row_map_box(&bmap, w, O, Kp / 4, 32, NT));
+  unsigned int* status = status_ptr();
+  if (!status) return SB_ERR_CUDA;
+  const int tiles_n = (O + NT - 1) / NT;
+  const int64_t tiles = (tokens + kTM - 1) / kTM * tiles_n;
+  constexpr int smem = 1024 + kStages * (kTM + NT) * kTK;
+  SB_CUDA(cudaFuncSetAttribute(qdense_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t grid = tiles < sm_count() ? tiles : sm_count();
+  qdense_gemm_kernel<NT><<<(unsigned)grid, kGThreads, smem, s>>>(amap, bmap, steps, ws, y, tokens, (Kp + kTK - 1) / kTK, O,
+                                                                T, tiles_n, tiles, status);
+  SB_CUDA(cudaGetLastError());
+  return SB_OK;
+}
+
+// From this many tokens on the two passes are ahead of the kernel that keeps its tokens in shared memory.
+constexpr int64_t kManyTokens = 9;
+
+int64_t steps_at(int64_t tokens, int64_t Kp) { return (tokens * Kp + 127) / 128 * 128; }
+
 }  // namespace
 
 extern "C" {
 
 int64_t sb_qdense_scratch_bytes(int64_t tokens, int64_t Kp) {
-  (void)tokens; (void)Kp;
-  return 0;
+  if (tokens < kManyTokens || Kp < 16 || tokens > (1LL << 40) || Kp > kMaxK) return 0;
+  return steps_at(tokens, Kp) + tokens * (int64_t)sizeof(float);
 }
 
 int sb_qdense_fwd(const float* x, const signed char* w, const float* w_scale, float* y, int64_t N, int64_t K,
@@ -130,11 +356,25 @@ int sb_qdense_fwd(const float* x, const signed char* w, const float* w_scale, fl
   if (N * O * T == 0) return SB_OK;
   SB_REQUIRE(x && w && w_scale && y, "null tensor pointer");
   SB_REQUIRE(((uintptr_t)w & 15u) == 0, "weights must be 16-byte aligned");
-  (void)scratch;
   const cudaStream_t s = (cudaStream_t)stream;
   const int64_t tokens = N * T;
   const int8_t* w8 = (const int8_t*)w;
   const int k = (int)K, kp = (int)Kp, o = (int)O;
+  if (tokens >= kManyTokens) {
+    SB_REQUIRE(scratch && ((uintptr_t)scratch & 15u) == 0, "scratch must be given and 16-byte aligned");
+    SB_REQUIRE(tokens < (1LL << 31) - kTM, "geometry too large");
+    int8_t* xq = (int8_t*)scratch;
+    float* steps = (float*)(xq + steps_at(tokens, Kp));
+    const int64_t tiles_t = (T + 31) / 32;
+    SB_REQUIRE(N * tiles_t < (1LL << 31), "geometry too large");
+    qdense_quantize_kernel<<<(unsigned)(N * tiles_t), kQThreads, 0, s>>>(x, xq, steps, k, kp, T, tiles_t);
+    SB_CUDA(cudaGetLastError());
+    // the widest tile that still gives every SM one
+    const int64_t rows = (tokens + kTM - 1) / kTM, sms = sm_count();
+    if (rows * ((O + 255) / 256) >= sms) return launch_gemm<256>(xq, steps, w8, w_scale, y, tokens, kp, o, T, s);
+    if (rows * ((O + 127) / 128) >= sms) return launch_gemm<128>(xq, steps, w8, w_scale, y, tokens, kp, o, T, s);
+    return launch_gemm<64>(xq, steps, w8, w_scale, y, tokens, kp, o, T, s);
+  }
   if (tokens > 4 && 8 * Kp <= 200 * 1024) return launch_few<8>(x, w8, w_scale, y, tokens, k, kp, o, T, s);
   if (tokens > 2 && 4 * Kp <= 200 * 1024) return launch_few<4>(x, w8, w_scale, y, tokens, k, kp, o, T, s);
   if (tokens > 1 && 2 * Kp <= 200 * 1024) return launch_few<2>(x, w8, w_scale, y, tokens, k, kp, o, T, s);
