@@ -37,83 +37,111 @@ __device__ __forceinline__ Words philox(uint64_t counter, uint64_t offset, uint6
   return Words{{c0, c1, c2, c3}};
 }
 
-constexpr int kThreads = 256;
+// A block takes spans of 4096 values: four groups of four consecutive ones per thread, all loaded before
+// the first is used (262 M values: 0.33 ms, 6.3 TB/s; with one group in flight per thread 0.39 ms).
+constexpr int kThreads = 256, kGroups = 4, kSpan = kThreads * kGroups * 4;
 
-// Four consecutive values per thread and trip: exactly one counter.  VEC needs 16-byte bases.
+struct Group {
+  float v[4];
+};
+// n: values of the tensor from `at` on (4 or more: a whole group)
+template <bool VEC>
+__device__ __forceinline__ Group load_group(const float* x, int64_t n) {
+  Group g{{0.f, 0.f, 0.f, 0.f}};
+  if (VEC && n >= 4) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(x));
+    g.v[0] = a.x; g.v[1] = a.y; g.v[2] = a.z; g.v[3] = a.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) g.v[e] = __ldcs(x + e);
+  }
+  return g;
+}
+template <bool VEC>
+__device__ __forceinline__ void store_group(float* y, int64_t n, const Group& g) {
+  if (VEC && n >= 4) {
+    __stcs(reinterpret_cast<float4*>(y), make_float4(g.v[0], g.v[1], g.v[2], g.v[3]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) __stcs(y + e, g.v[e]);
+  }
+}
+
+// Each value for itself: a group is exactly one counter.  VEC needs 16-byte bases.
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads)
 dropout_values_kernel(const float* __restrict__ x, float* __restrict__ y, const int64_t* __restrict__ key, int64_t n,
                       uint32_t threshold, float scale) {
   const uint64_t seed = (uint64_t)key[0], offset = (uint64_t)key[1];
-  const int64_t quads = (n + 3) / 4;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < quads; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t base = i * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool whole = VEC && base + 4 <= n;
-    if (whole) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(x + base));
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    } else {
+  for (int64_t span = (int64_t)blockIdx.x * kSpan; span < n; span += (int64_t)gridDim.x * kSpan) {
+    const int64_t first = span + threadIdx.x * 4;
+    Group g[kGroups];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (base + e < n) v[e] = __ldg(x + base + e);
-    }
-    const Words w = philox((uint64_t)i, offset, seed);
+    for (int i = 0; i < kGroups; ++i) g[i] = load_group<VEC>(x + first + i * kThreads * 4, n - (first + i * kThreads * 4));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = w.w[e] >= threshold ? v[e] * scale : 0.f;   // a select: NaN does not pass a drop
-    if (whole) {
-      *reinterpret_cast<float4*>(y + base) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
+    for (int i = 0; i < kGroups; ++i) {
+      const int64_t at = first + i * kThreads * 4;
+      const Words w = philox((uint64_t)at / 4, offset, seed);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (base + e < n) y[base + e] = v[e];
+      for (int e = 0; e < 4; ++e) g[i].v[e] = w.w[e] >= threshold ? g[i].v[e] * scale : 0.f;   // a select: NaN does not pass
+      store_group<VEC>(y + at, n - at, g[i]);
     }
   }
 }
 
-// Whole rows of T values: a thread's four values lie in one row or straddle rows.
+// Whole rows of T values.  The rows a span touches are drawn once, into shared memory.
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads)
 dropout_rows_kernel(const float* __restrict__ x, float* __restrict__ y, const int64_t* __restrict__ key, int64_t n,
                     int64_t T, uint32_t threshold, float scale) {
+  __shared__ uint8_t keep_s[kSpan + 8];
+  __shared__ int64_t row_s;
   const uint64_t seed = (uint64_t)key[0], offset = (uint64_t)key[1];
-  const int64_t quads = (n + 3) / 4;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < quads; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t base = i * 4;
-    int64_t row = base / T, pos = base - row * T, have = -1;
-    Words w{};
-    bool keep[4];
+  const float inv = 1.0f / (float)T;
+  for (int64_t span = (int64_t)blockIdx.x * kSpan; span < n; span += (int64_t)gridDim.x * kSpan) {
+    if (threadIdx.x == 0) row_s = span / T;
+    __syncthreads();
+    const int64_t row0 = row_s;
+    const int64_t pos0 = span - row0 * T;                        // within the first row
+    const int64_t left = n - span < kSpan ? n - span : kSpan;
+    // rows of the span behind the first (T < 4096 only: a longer row ends at most once in it)
+    auto row_of = [&](int i) {
+      if (T >= kSpan) return pos0 + i >= T ? 1 : 0;
+      // whole numbers below 8192: half a unit from the next multiple is more than the rounding of the product
+      return (int)(((float)((int)pos0 + i) + 0.5f) * inv);
+    };
+    const int rows = row_of((int)left - 1) + 1, head = (int)(row0 & 3);
+    for (int r = threadIdx.x * 4; r < rows + head; r += kThreads * 4) {
+      const Words w = philox((uint64_t)((row0 - head + r) >> 2), offset, seed);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (pos >= T) { ++row; pos = 0; }
-      if (row / 4 != have) { have = row / 4; w = philox((uint64_t)have, offset, seed); }
-      const int s = (int)(row & 3);
-      const uint32_t word = s == 0 ? w.w[0] : s == 1 ? w.w[1] : s == 2 ? w.w[2] : w.w[3];
-      keep[e] = word >= threshold;
-      ++pos;
+      for (int e = 0; e < 4; ++e) keep_s[r + e] = w.w[e] >= threshold ? 1 : 0;
     }
-    const bool any = keep[0] || keep[1] || keep[2] || keep[3];
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool whole = VEC && base + 4 <= n;
-    if (whole) {
-      if (any) {   // a dropped row is not read at all
-        const float4 a = __ldg(reinterpret_cast<const float4*>(x + base));
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    __syncthreads();
+    Group g[kGroups];
+    uint32_t keep[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int at = (threadIdx.x + i * kThreads) * 4;
+      keep[i] = 0;
+      if (at < left) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at + e < left) keep[i] |= (uint32_t)keep_s[head + row_of(at + e)] << e;
+        if (keep[i]) g[i] = load_group<VEC>(x + span + at, left - at);   // a dropped row is not read at all
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (keep[e] && base + e < n) v[e] = __ldg(x + base + e);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = keep[e] ? v[e] * scale : 0.f;
-    if (whole) {
-      *reinterpret_cast<float4*>(y + base) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
+    for (int i = 0; i < kGroups; ++i) {
+      const int at = (threadIdx.x + i * kThreads) * 4;
+      if (at < left) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (base + e < n) y[base + e] = v[e];
+        for (int e = 0; e < 4; ++e) g[i].v[e] = (keep[i] >> e & 1) ? g[i].v[e] * scale : 0.f;
+        store_group<VEC>(y + span + at, left - at, g[i]);
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -144,8 +172,8 @@ int sb_dropout(const float* x, float* y, const int64_t* key, int64_t rows, int64
   const uint32_t threshold = (uint32_t)(uint64_t)(p * 4294967296.0);
   const float scale = (float)(1.0 / (1.0 - p));
   const bool vec = ((((uintptr_t)x) | ((uintptr_t)y)) & 15u) == 0;
-  const int64_t blocks = (n + 4 * kThreads - 1) / (4 * kThreads);
-  const int64_t most = (int64_t)sm_count() * 16;
+  const int64_t blocks = (n + kSpan - 1) / kSpan;
+  const int64_t most = (int64_t)sm_count() * 32;
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
   if (per_step) {
     if (vec) dropout_values_kernel<true><<<grid, kThreads, 0, s>>>(x, y, key, n, threshold, scale);

@@ -147,7 +147,8 @@ def ptr(t):
 
 
 def stream_of(t):
-    return c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    # the raw handle: a Stream object costs as much host time as the launch itself
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def require_cuda(*tensors):
@@ -166,10 +167,15 @@ def require_cuda(*tensors):
 
 def call(name, device_tensor, *args):
     """Invoke an entry point with ``device_tensor``'s device current."""
-    lib = load()
-    with torch.cuda.device(device_tensor.device):
-        rc = getattr(lib, name)(*args)
-    check(rc, name)
+    fn = getattr(_lib or load(), name)
+    index = device_tensor.device.index
+    if index == torch._C._cuda_getDevice():   # entering the device's context costs several us of host time
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc != 0:
+        check(rc, name)
 
 
 def device_status():

@@ -53,6 +53,8 @@ def _c(t):
 
 def _param(p, like):
     """Flatten a decay-like parameter to contiguous fp32 on the input's device."""
+    if p.dtype == torch.float32 and p.device == like.device and p.dim() == 1 and p.is_contiguous():
+        return p
     p = p.detach().to(device=like.device, dtype=torch.float32).reshape(-1)
     return _c(p)
 
@@ -790,20 +792,24 @@ def _written(t):
 
 def _attention_check(q, k, v, decay, state, time):
     """Argument checks of the linear attention; returns (samples, H, Dk, Dv)."""
-    N.require_cuda(q, k, v, decay, state)
-    _same_device(q, key=k, value=v, decay=decay, state=state)
+    device, f32 = q.device, torch.float32
+    for name, t in (('query', q), ('key', k), ('value', v), ('decay', decay), ('state', state)):
+        if t is not None and (t.dtype is not f32 or t.device != device or not t.is_cuda):
+            N.require_cuda(t)
+            _same_device(q, **{name: t})
+    shape, vshape = q.shape, v.shape
     dims = 4 if time else 3
-    if q.dim() != dims or k.shape != q.shape:
+    if len(shape) != dims or k.shape != shape:
         raise ValueError(f'query and key must have one shape [batch, heads, width{", time" if time else ""}], '
-                         f'found {tuple(q.shape)} and {tuple(k.shape)}')
-    if v.dim() != dims or v.shape[:2] != q.shape[:2] or (time and v.shape[3] != q.shape[3]):
-        raise ValueError(f'value of shape {tuple(v.shape)} does not match query of shape {tuple(q.shape)}')
-    n, h, dk, dv = q.shape[0], q.shape[1], q.shape[2], v.shape[2]
+                         f'found {tuple(shape)} and {tuple(k.shape)}')
+    if len(vshape) != dims or vshape[:2] != shape[:2] or (time and vshape[3] != shape[3]):
+        raise ValueError(f'value of shape {tuple(vshape)} does not match query of shape {tuple(shape)}')
+    n, h, dk, dv = shape[0], shape[1], shape[2], vshape[2]
     if not (1 <= dk <= 128 and 1 <= dv <= 128):
         raise ValueError(f'head widths of 1 to 128 are supported, found {dk} (query, key) and {dv} (value)')
     if decay.numel() not in (1, h):
         raise ValueError(f'decay must have 1 or {h} elements, found {decay.numel()}')
-    if state is not None and tuple(state.shape) != (n, h, dk, dv):
+    if state is not None and state.shape != (n, h, dk, dv):
         raise ValueError(f'state must have shape {(n, h, dk, dv)}, found {tuple(state.shape)}')
     return n, h, dk, dv
 
@@ -849,8 +855,8 @@ def linear_attention_step(q, k, v, decay, state):
         raise ValueError('state is updated in place and must be contiguous')
     q, k, v, decay = _c(q), _c(k), _c(v), _param(decay, q)
     out = torch.empty_like(v)
-    N.call('sb_linear_attention_step', q, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(), N.ptr(state),
-           N.ptr(out), n * h, max(h, 1), dk, dv, N.stream_of(q))
+    N.call('sb_linear_attention_step', q, q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), decay.numel(),
+           state.data_ptr(), out.data_ptr(), n * h, h or 1, dk, dv, N.stream_of(q))
     _written(state)
     return out
 

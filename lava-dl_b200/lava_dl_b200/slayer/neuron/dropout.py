@@ -27,6 +27,8 @@ def dropout(input, p, key, per_step=False):
     torch tensor
         shaped like ``input``.
     """
+    if not torch.is_grad_enabled():
+        return _ops.dropout(input, p, key, per_step)
     return _Dropout.apply(input, key, p, per_step)
 
 

@@ -37,9 +37,12 @@ def dynamics(query, key, value, decay, state=None, return_state=False):
     torch tensor or pair of torch tensors
         output, shaped like ``value`` (and the state).
     """
-    if torch.is_grad_enabled() and decay.requires_grad:
+    if not torch.is_grad_enabled():
+        output, final = _ops.linear_attention_fwd(query, key, value, decay, state, return_state)
+    elif decay.requires_grad:
         raise RuntimeError('linear attention has no gradient for its decay; pass decay.detach()')
-    output, final = _LinearAttention.apply(query, key, value, decay, state, return_state)
+    else:
+        output, final = _LinearAttention.apply(query, key, value, decay, state, return_state)
     return (output, final) if return_state else output
 
 
@@ -62,8 +65,8 @@ def step(query, key, value, decay, state):
     torch tensor
         output, shaped like ``value``.
     """
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (query, key, value, decay, state)):
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad
+                                    or decay.requires_grad or (state is not None and state.requires_grad)):
         raise RuntimeError('linear attention steps update their state in place and have no gradient; use dynamics(), '
                            'or call step() under torch.no_grad()')
     return _ops.linear_attention_step(query, key, value, decay, state)
