@@ -81,7 +81,7 @@ struct TcArgs {
 template <int KT>
 struct Shape {
   static constexpr int stages = KT == 1 ? 2 : 1;      // KT = 2 has room for one
-  static constexpr int nsp = KT == 1 ? 2 : 1;         // score accumulators
+  static constexpr int nq = KT == 1 ? 2 : 1;          // q's of chunks in tensor memory
   static constexpr int score = KT == 1 ? 34 : 35;     // scores of the scaled vectors are below 2^score: 2^14 2^14 Dk
   // shared memory: k, v (hi and lo tiles; the raw fp32 tile they are converted from lies in the same
   // place), weighted v, raw q (KT = 1), state
@@ -89,8 +89,32 @@ struct Shape {
                        vw_at = v_at + stages * v_bytes, q_at = vw_at + v_bytes, s_at = q_at + (KT == 1 ? v_bytes : 0);
   static constexpr int smem = 1024 + s_at + 2 * KT * 64 * 128;
   // tensor memory columns
-  static constexpr uint32_t q = 0, sp = 64 * KT, oi = sp + 128 * nsp, ox = oi + 64, ds = ox + 64;
+  static constexpr uint32_t q = 0, sp = 128, oi = sp + 128, ox = oi + 64, ds = ox + 64;
 };
+
+// Bounded wait of this kernel.  The hardware holds the warp until the phase completes or the hinted time is
+// over, so that waiting warps do not fetch and issue polls between the instructions of the working ones.
+// Gives up after two seconds, or when another thread has.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* dead) {
+  uint64_t start = 0;
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+    if (ok) return true;
+    uint64_t now;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+    if (start == 0) start = now;
+    if (*dead) return false;
+    if (now - start > 2000000000ull) {
+      *dead = 1;
+      return false;
+    }
+  }
+}
 
 __device__ __forceinline__ float p2(int n) { return __int_as_float((n + 127) << 23); }   // -126 <= n <= 127
 struct Factors {
@@ -256,7 +280,7 @@ __device__ __forceinline__ void regs_dec() {
 template <int KT, bool FULL>
 __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ TcArgs args) {
   using S_ = Shape<KT>;
-  constexpr int NS = S_::stages, NSP = S_::nsp;
+  constexpr int NS = S_::stages;
   extern __shared__ uint8_t raw[];
   // What travels beside the mantissas.  A slot of two is rewritten for chunk c + 2 once the read-out of
   // chunk c has ended, a slot of four once the output of chunk c + 1 has been written.
@@ -271,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   __shared__ int poison_s[64];
   __shared__ int any_poison_s, dead_s;
   __shared__ uint32_t tmem_s;
-  __shared__ __align__(8) uint64_t bars[26];
+  __shared__ __align__(8) uint64_t bars[28];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = tid >> 7, th = tid & 127, tw = warp & 3;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -279,10 +303,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   volatile int* dead = &dead_s;
   volatile int* any_poison = &any_poison_s;
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t bar_k = bar0, bar_v = bar0 + 16, bar_free = bar0 + 32, bar_sp = bar0 + 48, bar_kx = bar0 + 64;   // two each
-  const uint32_t bar_q = bar0 + 80, bar_qfree = bar0 + 88, bar_p = bar0 + 96, bar_ds = bar0 + 104, bar_s = bar0 + 112,
-                 bar_o = bar0 + 120, bar_ofree = bar0 + 128, bar_end = bar0 + 144;
-  const uint32_t bar_kraw = bar0 + 152, bar_vraw = bar0 + 168, bar_qraw = bar0 + 184, bar_qread = bar0 + 192;   // k, v: two
+  auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+  // by stage or chunk parity: two each
+  const uint32_t bar_k = bar(0), bar_v = bar(2), bar_free = bar(4), bar_kx = bar(6), bar_kraw = bar(8), bar_vraw = bar(10),
+                 bar_q = bar(12), bar_qfree = bar(14);
+  const uint32_t bar_sp = bar(16), bar_p = bar(17), bar_ds = bar(18), bar_s = bar(19), bar_o = bar(20), bar_ofree = bar(21),
+                 bar_qraw = bar(22), bar_qread = bar(23), bar_end = bar(24);
 
   // which head, segment, walk and columns
   const int64_t bid = blockIdx.x;
@@ -303,15 +329,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mbar_init(bar_k + 8 * i, 128);
       mbar_init(bar_v + 8 * i, 128);
       mbar_init(bar_free + 8 * i, 1);
-      mbar_init(bar_sp + 8 * i, 2);
+      mbar_init(bar_q + 8 * i, 128);
+      mbar_init(bar_qfree + 8 * i, 2);
       mbar_init(bar_kx + 8 * i, 128);
       mbar_init(bar_kraw + 8 * i, 1);
       mbar_init(bar_vraw + 8 * i, 1);
     }
     mbar_init(bar_qraw, 1);
     mbar_init(bar_qread, 128);
-    mbar_init(bar_q, 128);
-    mbar_init(bar_qfree, 2);
+    mbar_init(bar_sp, 2);
     mbar_init(bar_p, 128);
     mbar_init(bar_ds, 2);
     mbar_init(bar_s, 128);
@@ -376,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           if (boxes) {
             // the raw tile, a step earlier or later in memory by direction; its place is free to be written
             // (k, v) or to receive the next tile (q) once the whole warpgroup has read it
-            wait_or_dead(is_q ? bar_qraw : (is_k ? bar_kraw : bar_vraw) + 8 * (c % NS),
+            wait_phase(is_q ? bar_qraw : (is_k ? bar_kraw : bar_vraw) + 8 * (c % NS),
                          is_q ? (uint32_t)c & 1u : (uint32_t)(c / NS) & 1u, dead);
             load64_shared(x, slot + (uint32_t)(w.reverse ? kL - 1 - j : j) * 4);
             if (is_q) mbar_arrive(bar_qread);
@@ -396,19 +422,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
             const int f = fit_exponent(bad ? 0.f : top);
             scale = p2(-f);
-            if (!boxes && c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+            if (!boxes && c >= NS) wait_phase(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
             f_s[c & 1][j] = bad ? kNoTerm - 1 : (top > 0.f ? f : kNoTerm);
             mbar_arrive(bar_kx + 8 * (c & 1));
           } else if (is_q) {
             zero = bad;
             const int qe = bad ? 0 : fit_exponent(top);
             scale = p2(-qe);
-            if (c >= 1) wait_or_dead(bar_qfree, (uint32_t)(c - 1) & 1u, dead);
+            if (c >= S_::nq)
+              wait_phase(bar_qfree + 8 * ((c - S_::nq) & 1), (uint32_t)((c - S_::nq) >> 1) & 1u, dead);
             tc_fence_after();
             qe_s[c & 3][j] = bad ? 0x7fffffff : qe;
           } else {
             // v, and what P and the growth need to know of the steps
-            wait_or_dead(bar_kx + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
+            wait_phase(bar_kx + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
             const int f = f_s[c & 1][j];
             zero = f == kNoTerm - 1;
             if (bad && !zero) {                  // single columns are spoilt; the rest of the vector counts
@@ -454,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
               mw = max(mw, kmax_s[c & 1][i]);
               mc = max(mc, kmax_s[c & 1][4 + i]);
             }
-            if (!boxes && c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+            if (!boxes && c >= NS) wait_phase(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
             if (FULL) {
               col_s[c & 1][j] = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
               m_s[c & 3][j] = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
@@ -490,13 +517,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             uint32_t r[16];
 #pragma unroll
             for (int e = 0; e < 8; ++e) split2(mul2(x[b + e], sc), &r[e], &r[8 + e]);
-            tmem_st16(trow + S_::q + half * 64 + 2 * b, r);
+            tmem_st16(trow + S_::q + (uint32_t)(c % S_::nq) * 64 + half * 64 + 2 * b, r);
           }
           if constexpr (KT == 1) break;          // (x is not carried on)
           continue;
         }
         // one row of a hi and a lo tile (128-byte swizzle)
-        if (weighted && c >= 1) wait_or_dead(bar_ds, (uint32_t)(c - 1) & 1u, dead);    // read by the growth before
+        if (weighted && c >= 1) wait_phase(bar_ds, (uint32_t)(c - 1) & 1u, dead);    // read by the growth before
         const uint32_t tile = (weighted ? base + S_::vw_at : slot + (uint32_t)half * kTileB) + (uint32_t)(j * 128);
         const uint32_t lo_at = is_v ? kTileB : KT * kTileB;
 #pragma unroll
@@ -519,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(bar_q);
+      mbar_arrive(bar_q + 8 * (c & 1));
     }
   } else if (role == 3) {
     // ---------------- scores -> P: thread = row i ----------------
@@ -528,9 +555,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       const int l = th;
 #pragma unroll 1
       for (int c = 0; c < nc; ++c) {
-        const uint32_t sp = trow + S_::sp + (uint32_t)(c % NSP) * 128u;
-        wait_or_dead(bar_sp + 8 * (c % NSP), (uint32_t)(c / NSP) & 1u, dead);
-        wait_or_dead(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);    // the columns' factors
+        const uint32_t sp = trow + S_::sp;
+        wait_phase(bar_sp, (uint32_t)c & 1u, dead);
+        wait_phase(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);    // the columns' factors
         tc_fence_after();
         // |q_i . k_j| <= 2^score of the scaled vectors: P is held as its multiple of 2^(m + score - 15)
         const float rowf = p2(max(-126, min(mc_s[c & 1] - m_s[c & 3][l] - (S_::score - 15), 127)));
@@ -617,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const int64_t t = (c0 + p) * kL + l;
         float* out = w.o + (head * (int64_t)w.Dv + e0) * T + (w.reverse ? T - 1 - t : t);
         const bool live = t < T, plain = (c0 + p + 1) * kL <= T && ne == 64;
-        wait_or_dead(bar_o, (uint32_t)p & 1u, dead);
+        wait_phase(bar_o, (uint32_t)p & 1u, dead);
         tc_fence_after();
         const int qe = qe_s[p & 3][l], m = m_s[p & 3][l] + S_::score - 15;
         const bool bad = qe == 0x7fffffff;
@@ -669,8 +696,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       if (c >= 0) {
         // the state after chunk c
         const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
-        wait_or_dead(bar_ds, (uint32_t)c & 1u, dead);
-        if (FULL) wait_or_dead(bar_qfree, (uint32_t)c & 1u, dead);     // the published state has been read
+        wait_phase(bar_ds, (uint32_t)c & 1u, dead);
+        if (FULL) wait_phase(bar_qfree + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);   // the published state has been read
         tc_fence_after();
         const Factors mw = p2_wide(mw_s[c & 3]);
         const float carry = pow_pad[32 + len];
@@ -742,33 +769,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       // The barriers that count to two take an arrival of this thread beside the commit: it hands on what
       // the loaders wrote beside the operands.
       auto scores = [&](int c) {
-        ok = wait_or_dead(bar_q, (uint32_t)c & 1u, dead) && ok;
-        ok = wait_or_dead(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        ok = wait_phase(bar_q + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead) && ok;
+        ok = wait_phase(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         if (!ok) return;
         tc_fence_after();
-        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes, d = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
+        const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes, d = tmem + S_::sp;
 #pragma unroll 1
         for (int s = 0; s < 4 * KT; ++s) {
           const uint32_t bh = desc_lo(k_hi + (uint32_t)((s >> 2) * kTileB + (s & 3) * 32));
-          const uint32_t q_hi = tq + (uint32_t)s * 16;
+          const uint32_t q_hi = tq + (uint32_t)(c % S_::nq) * 64 + (uint32_t)s * 16;
           mma_f16_ts(d, q_hi, bh, id_scores, s > 0);
           mma_f16_ts(d, q_hi + 8, bh, id_scores, 1u);
           mma_f16_ts(d, q_hi, bh + (KT * kTileB >> 4), id_scores, 1u);
         }
-        umma_commit(bar_sp + 8 * (c % NSP));
-        mbar_arrive(bar_sp + 8 * (c % NSP));
+        umma_commit(bar_sp);
+        mbar_arrive(bar_sp);
       };
       if (FULL) scores(0);
       // Growth first, it waits for nothing but the state's warps; then the state's part of the output, for
-      // which the output before has to be taken away; with two score accumulators the next scores run ahead
-      // of the read-out, so that P is made while the MMAs go on.
+      // which the output before has to be taken away, the read-out, and the next chunk's scores.
 #pragma unroll 1
       for (int c = 0; c < nc && ok; ++c) {
         const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes,
                        v_hi = base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, vw_hi = base + S_::vw_at;
-        ok = wait_or_dead(bar_s, (uint32_t)c & 1u, dead) && ok;
-        if (!FULL) ok = wait_or_dead(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
-        ok = wait_or_dead(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        ok = wait_phase(bar_s, (uint32_t)c & 1u, dead) && ok;
+        if (!FULL) ok = wait_phase(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        ok = wait_phase(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
@@ -783,24 +809,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           umma_commit(bar_free + 8 * (c % NS));
           continue;
         }
-        if (c >= 1) ok = wait_or_dead(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
+        if (c >= 1) ok = wait_phase(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
         for (int s = 0; s < 4 * KT; ++s) {
           const uint32_t bh = desc_lo(sbase + (uint32_t)((s >> 2) * 8192 + (s & 3) * 32));
-          const uint32_t q_hi = tq + (uint32_t)s * 16;
+          const uint32_t q_hi = tq + (uint32_t)(c % S_::nq) * 64 + (uint32_t)s * 16;
           mma_f16_ts(tox, q_hi, bh, id_inter, s > 0);
           mma_f16_ts(tox, q_hi + 8, bh, id_inter, 1u);
           mma_f16_ts(tox, q_hi, bh + (KT * 8192 >> 4), id_inter, 1u);
         }
-        umma_commit(bar_qfree);
-        mbar_arrive(bar_qfree);
-        if (NSP == 2 && c + 1 < nc) scores(c + 1);
-        ok = wait_or_dead(bar_p, (uint32_t)c & 1u, dead) && ok;
+        umma_commit(bar_qfree + 8 * (c & 1));
+        mbar_arrive(bar_qfree + 8 * (c & 1));
+        ok = wait_phase(bar_p, (uint32_t)c & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();
-        const uint32_t sp = tmem + S_::sp + (uint32_t)(c % NSP) * 128u;
+        const uint32_t sp = tmem + S_::sp;
 #pragma unroll 1
         for (int s = 0; s < 8; ++s) {
           const uint32_t p_hi = sp + (uint32_t)((s >> 1) * 32 + (s & 1) * 8), bh = desc_mn(v_hi + s * 2048);
@@ -811,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         umma_commit(bar_o);
         mbar_arrive(bar_o);
         umma_commit(bar_free + 8 * (c % NS));
-        if (NSP == 1 && c + 1 < nc) scores(c + 1);
+        if (c + 1 < nc) scores(c + 1);
       }
       umma_commit(bar_end);          // everything issued has landed before tensor memory is given back
       if (!mbar_wait(bar_end, 0)) *dead = 1;
@@ -823,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       for (int c = 0; c < nc; ++c) {
         const int64_t t = (c0 + c) * kL;
         const int from = (int)(w.reverse ? T - t - kL : t);      // walking back, the last box may start before 0
-        if (c >= NS) wait_or_dead(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+        if (c >= NS) wait_phase(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
         if (*dead) break;
         const uint32_t bk = bar_kraw + 8 * (c % NS), bv = bar_vraw + 8 * (c % NS);
         mbar_expect_tx(bk, 2 * kTileB);
@@ -833,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         tma_load_box(base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, &maps[2], from, e0, (int)head, bv);
         issued[1] = c + 1;
         if (FULL) {
-          if (c >= 1) wait_or_dead(bar_qread, (uint32_t)(c - 1) & 1u, dead);
+          if (c >= 1) wait_phase(bar_qread, (uint32_t)(c - 1) & 1u, dead);
           if (*dead) break;
           mbar_expect_tx(bar_qraw, 2 * kTileB);
           tma_load_box(base + S_::q_at, &maps[0], from, 0, (int)head, bar_qraw);
