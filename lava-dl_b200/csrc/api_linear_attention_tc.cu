@@ -26,8 +26,8 @@
 // loads and holds that step's whole vector: its exponent needs no exchange, and its hi and lo halves are
 // written as one 128-byte row of a [step][channel] tile each.  That one tile of k is the K-major B
 // operand of the scores and the MN-major B operand of the growth; v is MN-major in the read-out, and a
-// copy weighted by r^(L-a-j) is the MN-major A operand of the growth (hi and lo stacked to M = 128, so
-// two MMAs cover the three products).  q goes to tensor memory (it is A of two products) and so does P,
+// copy weighted by r^(L-a-j) is the MN-major A operand of the growth (64 rows, repeated to M = 128: each
+// half of the lanes keeps half of the columns).  q goes to tensor memory (it is A of two products) and so does P,
 // converted in place of the scores.
 //
 // Roles of a CTA (one per SM, six warpgroups): k, v and q are each loaded and converted by a warpgroup
@@ -147,11 +147,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
@@ -205,6 +200,9 @@ constexpr uint32_t kAMajorMN = 1u << 15, kBMajorMN = 1u << 16;
 __device__ __forceinline__ uint32_t desc_mn(uint32_t saddr) {
   return ((saddr & 0x3ffffu) >> 4) | ((uint32_t)(kTileB >> 4) << 16);
 }
+
+// MN-major, the rows 64-127 a repetition of the rows 0-63
+__device__ __forceinline__ uint32_t desc_twice(uint32_t saddr) { return (saddr & 0x3ffffu) >> 4; }
 
 // 64 rows of one step.  volatile: the loads stay where they are issued, in one batch ahead of the waits
 // and conversions (left to itself the compiler sinks them to their use).
@@ -308,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   const uint32_t bar_k = bar(0), bar_v = bar(2), bar_free = bar(4), bar_kx = bar(6), bar_kraw = bar(8), bar_vraw = bar(10),
                  bar_q = bar(12), bar_qfree = bar(14);
   const uint32_t bar_sp = bar(16), bar_p = bar(17), bar_ds = bar(18), bar_s = bar(19), bar_o = bar(20), bar_ofree = bar(21),
-                 bar_qraw = bar(22), bar_qread = bar(23), bar_end = bar(24);
+                 bar_qraw = bar(22), bar_qread = bar(23), bar_end = bar(24), bar_dsfree = bar(25);
 
   // which head, segment, walk and columns
   const int64_t bid = blockIdx.x;
@@ -341,6 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     mbar_init(bar_p, 128);
     mbar_init(bar_ds, 2);
     mbar_init(bar_s, 128);
+    mbar_init(bar_dsfree, 128);
     mbar_init(bar_o, 2);
     mbar_init(bar_ofree, 128);
     mbar_init(bar_end, 1);
@@ -635,8 +634,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       fence_proxy_async();
     };
-    // Trip c writes the output of chunk c - 1, then takes the state over chunk c: the published state is
-    // replaced once the MMAs of chunk c have read it.  Trip -1 publishes what the walk starts from.
+    // Trip c writes the output of chunk c - 1, then takes the state over chunk c.  Trip -1 publishes what the
+    // walk starts from.
 #pragma unroll 1
     for (int c = -1; c <= (FULL ? nc : nc - 1); ++c) {
       if (FULL && c >= 1) {
@@ -697,50 +696,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         // the state after chunk c
         const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
         wait_phase(bar_ds, (uint32_t)c & 1u, dead);
-        if (FULL) wait_phase(bar_qfree + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);   // the published state has been read
         tc_fence_after();
         const Factors mw = p2_wide(mw_s[c & 3]);
         const float carry = pow_pad[32 + len];
-        // rows 0-63 of the accumulator come from the hi half of v, rows 64-127 from the lo half: each
-        // thread adds the other's to its own half of the columns (exchanged where the published state lay)
-        const uint32_t mine = trow + S_::ds + (uint32_t)half * NSt, other = trow + S_::ds + (uint32_t)(half ^ 1) * NSt;
-        const uint32_t ex_row = sbase + (uint32_t)(l ^ 64) * (NSt * 4), my_row = sbase + (uint32_t)l * (NSt * 4);
+        const uint64_t ma = pair(mw.a, mw.a), mb = pair(mw.b, mw.b), cy = pair(carry, carry);
+        // (rows 64-127 of the accumulator repeat rows 0-63)
 #pragma unroll
         for (int b = 0; b < NSt; b += 32) {
           uint32_t r[32];
-          tmem_ld32(other + b, r);
+          tmem_ld32(trow + S_::ds + (uint32_t)(half * NSt + b), r);
           tmem_ld_wait();
+          if (b + 32 == NSt) {
+            tc_fence_before();
+            mbar_arrive(bar_dsfree);
+          }
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            sts128(ex_row + (uint32_t)(((b / 4 + x) ^ (l & 7)) << 4), r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]);
-        }
-        bar_sync(2, 128);
-#pragma unroll
-        for (int b = 0; b < NSt; b += 32) {
-          uint32_t r[32];
-          tmem_ld32(mine + b, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            float y[4];
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3])
-                         : "r"(my_row + (uint32_t)(((b / 4 + x) ^ (l & 7)) << 4)));
-#pragma unroll
-            for (int u = 0; u < 4; u += 2) {
-              const uint64_t grown = add2(pair(__uint_as_float(r[4 * x + u]), __uint_as_float(r[4 * x + u + 1])), pair(y[u], y[u + 1]));
-              const float2 v = unpair(fma2(pair(carry, carry), pair(St[b + 4 * x + u], St[b + 4 * x + u + 1]),
-                                           mul2(mul2(grown, pair(mw.a, mw.a)), pair(mw.b, mw.b))));
-              St[b + 4 * x + u] = v.x;
-              St[b + 4 * x + u + 1] = v.y;
-            }
+          for (int x = 0; x < 32; x += 2) {
+            const uint64_t grown = mul2(mul2(pair(__uint_as_float(r[x]), __uint_as_float(r[x + 1])), ma), mb);
+            const float2 v = unpair(fma2(cy, pair(St[b + x], St[b + x + 1]), grown));
+            St[b + x] = v.x;
+            St[b + x + 1] = v.y;
           }
         }
-        tc_fence_before();
       }
-      if (FULL && c + 1 < nc) publish((c + 1) & 1);      // its barrier also ends the exchange
-      else bar_sync(2, 128);
-      mbar_arrive(bar_s);
+      if (FULL && c + 1 < nc) {
+        // the published state is replaced once the MMAs of the chunk have read it
+        if (c >= 0) wait_phase(bar_qfree + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
+        publish((c + 1) & 1);
+        mbar_arrive(bar_s);
+      }
     }
     // the state after the last chunk
     float* dst = nullptr;
@@ -792,15 +776,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       for (int c = 0; c < nc && ok; ++c) {
         const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes,
                        v_hi = base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, vw_hi = base + S_::vw_at;
-        ok = wait_phase(bar_s, (uint32_t)c & 1u, dead) && ok;
         if (!FULL) ok = wait_phase(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         ok = wait_phase(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        if (c >= 1) ok = wait_phase(bar_dsfree, (uint32_t)(c - 1) & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
         for (int s = 0; s < 8; ++s) {
-          const uint32_t a = desc_mn(vw_hi + s * 2048), b = desc_mn(k_hi + s * 2048);
+          const uint32_t a = desc_twice(vw_hi + s * 2048), b = desc_mn(k_hi + s * 2048);
           mma_f16_ss(tds, a, b, id_grow, s > 0);
+          mma_f16_ss(tds, a + (kTileB >> 4), b, id_grow, 1u);
           mma_f16_ss(tds, a, b + (KT * kTileB >> 4), id_grow, 1u);
         }
         umma_commit(bar_ds);
@@ -809,6 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           umma_commit(bar_free + 8 * (c % NS));
           continue;
         }
+        ok = wait_phase(bar_s, (uint32_t)c & 1u, dead) && ok;
         if (c >= 1) ok = wait_phase(bar_ofree, (uint32_t)(c - 1) & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();
