@@ -83,10 +83,10 @@ struct Shape {
   static constexpr int stages = KT == 1 ? 2 : 1;      // KT = 2 has room for one
   static constexpr int nq = KT == 1 ? 2 : 1;          // q's of chunks in tensor memory
   static constexpr int score = KT == 1 ? 34 : 35;     // scores of the scaled vectors are below 2^score: 2^14 2^14 Dk
-  // shared memory: k, v (hi and lo tiles; the raw fp32 tile they are converted from lies in the same
-  // place), weighted v, raw q (KT = 1), state
+  // shared memory: k, v (hi and lo tile of each 64 channels; the raw fp32 tile they are converted from lies
+  // in the same 32 KB), weighted v, raw q (64 channels at a time), state
   static constexpr int k_bytes = 2 * KT * kTileB, v_at = stages * k_bytes, v_bytes = 2 * kTileB,
-                       vw_at = v_at + stages * v_bytes, q_at = vw_at + v_bytes, s_at = q_at + (KT == 1 ? v_bytes : 0);
+                       vw_at = v_at + stages * v_bytes, q_at = vw_at + v_bytes, s_at = q_at + v_bytes;
   static constexpr int smem = 1024 + s_at + 2 * KT * 64 * 128;
   // tensor memory columns
   static constexpr uint32_t q = 0, sp = 128, oi = sp + 128, ox = oi + 64, ds = ox + 64;
@@ -196,9 +196,9 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n) {
 }
 constexpr uint32_t kAMajorMN = 1u << 15, kBMajorMN = 1u << 16;
 // Low descriptor word: K-major (the leading offset is unused with the 128-byte swizzle), or MN-major
-// with the next 64 channels one tile further on; groups of eight rows lie 1024 bytes apart either way.
+// with the next 64 channels two tiles further on; groups of eight rows lie 1024 bytes apart either way.
 __device__ __forceinline__ uint32_t desc_mn(uint32_t saddr) {
-  return ((saddr & 0x3ffffu) >> 4) | ((uint32_t)(kTileB >> 4) << 16);
+  return ((saddr & 0x3ffffu) >> 4) | ((uint32_t)(2 * kTileB >> 4) << 16);
 }
 
 // MN-major, the rows 64-127 a repetition of the rows 0-63
@@ -243,6 +243,16 @@ __device__ __forceinline__ void load64_shared(uint64_t (&x)[32], uint32_t p) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(p + d * 1024 + 512));
     x[d] = pair(a, b);
   }
+}
+__device__ __forceinline__ float top64_shared(uint32_t p, float m) {
+#pragma unroll
+  for (int d = 0; d < 32; ++d) {
+    float a, b;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(p + d * 1024));
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(p + d * 1024 + 512));
+    m = max_abs3(m, a, b);
+  }
+  return m;
 }
 __device__ __forceinline__ void tma_load_box(uint32_t dst, const CUtensorMap* map, int t, int row, int head, uint32_t bar) {
   asm volatile(
@@ -307,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                  bar_q = bar(12), bar_qfree = bar(14);
   const uint32_t bar_sp = bar(16), bar_p = bar(17), bar_ds = bar(18), bar_s = bar(19), bar_o = bar(20), bar_ofree = bar(21),
                  bar_qraw = bar(22), bar_qread = bar(23), bar_end = bar(24), bar_dsfree = bar(25);
+  const uint32_t bar_kfree = bar(26);           // two
 
   // which head, segment, walk and columns
   const int64_t bid = blockIdx.x;
@@ -320,13 +331,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   const int64_t c0 = (int64_t)seg * args.seg_chunks;
   const int nc = (int)min((int64_t)args.seg_chunks, (T + kL - 1) / kL - c0);
   const int after = w.after;
-  const bool boxes = KT == 1 && args.boxes != 0;
+  const bool boxes = args.boxes != 0;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_k + 8 * i, 128);
       mbar_init(bar_v + 8 * i, 128);
       mbar_init(bar_free + 8 * i, 1);
+      mbar_init(bar_kfree + 8 * i, 1);
       mbar_init(bar_q + 8 * i, 128);
       mbar_init(bar_qfree + 8 * i, 2);
       mbar_init(bar_kx + 8 * i, 128);
@@ -379,10 +391,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     const float* src = is_k ? w.k + head * (int64_t)Dk * T
                             : (is_v ? w.v + (head * (int64_t)w.Dv + e0) * T : w.q + head * (int64_t)Dk * T);
     const int rows = is_v ? ne : Dk;
-    // Passes over an operand.  Dk > 64: the largest magnitude of the first half, then of the second, which
-    // is converted while it is there, then the first half again.  v: as it is, and weighted.
-    const int passes = is_v ? (FULL ? 2 : 1) : (KT == 2 ? 3 : 1);
-    const int mid = is_v ? 0 : KT - 1;           // the pass after whose load the exponent is known
+    // Passes over an operand.  Dk > 64 needs the largest magnitude of both halves before either is converted:
+    // k's raw tiles are looked through first; otherwise the first half is loaded, the second, which is
+    // converted while it is there, and the first again.  v: as it is, and weighted.
+    const bool ahead = KT == 2 && is_k && boxes;
+    const int passes = is_v ? (FULL ? 2 : 1) : (KT == 1 ? 1 : (ahead ? 2 : 3));
+    const int mid = is_v || ahead ? 0 : KT - 1;  // the pass after whose load the exponent is known
 #pragma unroll 1
     for (int c = (FULL || !is_q) ? 0 : nc; c < nc; ++c) {
       const uint32_t slot = base + (is_k ? (uint32_t)(c % NS) * S_::k_bytes
@@ -401,9 +415,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           if (boxes) {
             // the raw tile, a step earlier or later in memory by direction; its place is free to be written
             // (k, v) or to receive the next tile (q) once the whole warpgroup has read it
-            wait_phase(is_q ? bar_qraw : (is_k ? bar_kraw : bar_vraw) + 8 * (c % NS),
-                         is_q ? (uint32_t)c & 1u : (uint32_t)(c / NS) & 1u, dead);
-            load64_shared(x, slot + (uint32_t)(w.reverse ? kL - 1 - j : j) * 4);
+            const uint32_t raw_at = slot + (uint32_t)(w.reverse ? kL - 1 - j : j) * 4;
+            if (is_q) {
+              const uint32_t n = (uint32_t)(KT == 1 ? c : 3 * c + pass);
+              wait_phase(bar_qraw, n & 1u, dead);
+            } else if (pass == 0) {
+              wait_phase((is_k ? bar_kraw : bar_vraw) + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);
+              if (ahead) top = top64_shared(raw_at + 2 * kTileB, top);
+            }
+            load64_shared(x, raw_at + (is_k ? (uint32_t)half * 2 * kTileB : 0u));
             if (is_q) mbar_arrive(bar_qread);
             else bar_sync(3 + role, 128);
           } else {
@@ -421,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
             const int f = fit_exponent(bad ? 0.f : top);
             scale = p2(-f);
-            if (!boxes && c >= NS) wait_phase(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+            if (!boxes && c >= NS) wait_phase(bar_kfree + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
             f_s[c & 1][j] = bad ? kNoTerm - 1 : (top > 0.f ? f : kNoTerm);
             mbar_arrive(bar_kx + 8 * (c & 1));
           } else if (is_q) {
@@ -523,8 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
         // one row of a hi and a lo tile (128-byte swizzle)
         if (weighted && c >= 1) wait_phase(bar_ds, (uint32_t)(c - 1) & 1u, dead);    // read by the growth before
-        const uint32_t tile = (weighted ? base + S_::vw_at : slot + (uint32_t)half * kTileB) + (uint32_t)(j * 128);
-        const uint32_t lo_at = is_v ? kTileB : KT * kTileB;
+        const uint32_t tile = (weighted ? base + S_::vw_at : slot + (uint32_t)half * 2 * kTileB) + (uint32_t)(j * 128);
 #pragma unroll
         for (int q8 = 0; q8 < 8; ++q8) {
           uint32_t h[4], l[4];
@@ -535,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
           const uint32_t to = tile + (uint32_t)((q8 ^ (j & 7)) << 4);
           sts128(to, h[0], h[1], h[2], h[3]);
-          sts128(to + lo_at, l[0], l[1], l[2], l[3]);
+          sts128(to + kTileB, l[0], l[1], l[2], l[3]);
         }
       }
       if (is_k || is_v) {
@@ -760,11 +779,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes, d = tmem + S_::sp;
 #pragma unroll 1
         for (int s = 0; s < 4 * KT; ++s) {
-          const uint32_t bh = desc_lo(k_hi + (uint32_t)((s >> 2) * kTileB + (s & 3) * 32));
+          const uint32_t bh = desc_lo(k_hi + (uint32_t)((s >> 2) * 2 * kTileB + (s & 3) * 32));
           const uint32_t q_hi = tq + (uint32_t)(c % S_::nq) * 64 + (uint32_t)s * 16;
           mma_f16_ts(d, q_hi, bh, id_scores, s > 0);
           mma_f16_ts(d, q_hi + 8, bh, id_scores, 1u);
-          mma_f16_ts(d, q_hi, bh + (KT * kTileB >> 4), id_scores, 1u);
+          mma_f16_ts(d, q_hi, bh + (kTileB >> 4), id_scores, 1u);
         }
         umma_commit(bar_sp);
         mbar_arrive(bar_sp);
@@ -786,10 +805,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           const uint32_t a = desc_twice(vw_hi + s * 2048), b = desc_mn(k_hi + s * 2048);
           mma_f16_ss(tds, a, b, id_grow, s > 0);
           mma_f16_ss(tds, a + (kTileB >> 4), b, id_grow, 1u);
-          mma_f16_ss(tds, a, b + (KT * kTileB >> 4), id_grow, 1u);
+          mma_f16_ss(tds, a, b + (kTileB >> 4), id_grow, 1u);
         }
         umma_commit(bar_ds);
         mbar_arrive(bar_ds);
+        umma_commit(bar_kfree + 8 * (c % NS));
         if (!FULL) {
           umma_commit(bar_free + 8 * (c % NS));
           continue;
@@ -826,36 +846,45 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       umma_commit(bar_end);          // everything issued has landed before tensor memory is given back
       if (!mbar_wait(bar_end, 0)) *dead = 1;
-    } else if (KT == 1 && th == 32 && boxes) {
-      // ---------------- raw tiles, one TMA box each ----------------
+    } else if (th == 32 && boxes) {
+      // ---------------- raw k and v, a TMA box for 64 channels ----------------
       const CUtensorMap* maps = args.map[wi];
-      int issued[3] = {0, 0, 0};
+      int k_issued = 0, v_issued = 0;
 #pragma unroll 1
       for (int c = 0; c < nc; ++c) {
         const int64_t t = (c0 + c) * kL;
         const int from = (int)(w.reverse ? T - t - kL : t);      // walking back, the last box may start before 0
-        if (c >= NS) wait_phase(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
+        const uint32_t bk = bar_kraw + 8 * (c % NS), bv = bar_vraw + 8 * (c % NS), again = (uint32_t)(c / NS - 1) & 1u;
+        if (c >= NS) wait_phase(bar_kfree + 8 * (c % NS), again, dead);
         if (*dead) break;
-        const uint32_t bk = bar_kraw + 8 * (c % NS), bv = bar_vraw + 8 * (c % NS);
-        mbar_expect_tx(bk, 2 * kTileB);
-        tma_load_box(base + (uint32_t)(c % NS) * S_::k_bytes, &maps[1], from, 0, (int)head, bk);
-        issued[0] = c + 1;
-        mbar_expect_tx(bv, 2 * kTileB);
+        mbar_expect_tx(bk, S_::k_bytes);
+        for (int h = 0; h < KT; ++h)
+          tma_load_box(base + (uint32_t)(c % NS) * S_::k_bytes + h * 2 * kTileB, &maps[1], from, 64 * h, (int)head, bk);
+        k_issued = c + 1;
+        if (c >= NS) wait_phase(bar_free + 8 * (c % NS), again, dead);
+        if (*dead) break;
+        mbar_expect_tx(bv, S_::v_bytes);
         tma_load_box(base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, &maps[2], from, e0, (int)head, bv);
-        issued[1] = c + 1;
-        if (FULL) {
-          if (c >= 1) wait_phase(bar_qread, (uint32_t)(c - 1) & 1u, dead);
-          if (*dead) break;
-          mbar_expect_tx(bar_qraw, 2 * kTileB);
-          tma_load_box(base + S_::q_at, &maps[0], from, 0, (int)head, bar_qraw);
-          issued[2] = c + 1;
-        }
+        v_issued = c + 1;
       }
       if (*dead) {   // nobody may have waited for the boxes in flight: not before they have landed
-        for (int c = max(issued[0] - 2, 0); c < issued[0]; ++c) mbar_wait(bar_kraw + 8 * (c % NS), (uint32_t)(c / NS) & 1u);
-        for (int c = max(issued[1] - 2, 0); c < issued[1]; ++c) mbar_wait(bar_vraw + 8 * (c % NS), (uint32_t)(c / NS) & 1u);
-        if (issued[2] > 0) mbar_wait(bar_qraw, (uint32_t)(issued[2] - 1) & 1u);
+        for (int c = max(k_issued - NS, 0); c < k_issued; ++c) mbar_wait(bar_kraw + 8 * (c % NS), (uint32_t)(c / NS) & 1u);
+        for (int c = max(v_issued - NS, 0); c < v_issued; ++c) mbar_wait(bar_vraw + 8 * (c % NS), (uint32_t)(c / NS) & 1u);
       }
+    } else if (FULL && th == 64 && boxes) {
+      // ---------------- raw q, 64 channels at a time ----------------
+      constexpr int per = KT == 1 ? 1 : 3;       // the halves in the order they are asked for: 0, 1, 0
+      int n = 0;
+#pragma unroll 1
+      for (; n < per * nc; ++n) {
+        const int64_t t = (c0 + n / per) * kL;
+        if (n >= 1) wait_phase(bar_qread, (uint32_t)(n - 1) & 1u, dead);
+        if (*dead) break;
+        mbar_expect_tx(bar_qraw, 2 * kTileB);
+        tma_load_box(base + S_::q_at, &args.map[wi][0], (int)(w.reverse ? T - t - kL : t), n % per == 1 ? 64 : 0,
+                     (int)head, bar_qraw);
+      }
+      if (*dead && n > 0) mbar_wait(bar_qraw, (uint32_t)(n - 1) & 1u);
     }
     __syncwarp();
   }
@@ -962,7 +991,7 @@ int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
   }
   uintptr_t bits = 0;
   for (int i = 0; i < n; ++i) bits |= (uintptr_t)walks[i].q | (uintptr_t)walks[i].k | (uintptr_t)walks[i].v;
-  a.boxes = walks[0].Dk <= 64 && (bits & 15u) == 0 && walks[0].T % 4 == 0;
+  a.boxes = (bits & 15u) == 0 && walks[0].T % 4 == 0;
   for (int i = 0; i < n && a.boxes; ++i) {
     const Walk& w = walks[i];
     const float* base[3] = {w.q, w.k, w.v};
