@@ -30,13 +30,18 @@
 // half of the lanes keeps half of the columns).  q goes to tensor memory (it is A of two products) and so does P,
 // converted in place of the scores.
 //
-// Roles of a CTA (one per SM, six warpgroups): k, v and q are each loaded and converted by a warpgroup
-// (one step per thread), one turns scores into P, one keeps the state (32 elements per thread and 64 of
-// Dk in registers, fp32) and writes the output, and one thread issues the MMAs.  What decides the speed
-// is the instruction cache: a first form (one loading warpgroup with two operands in 232 registers) ran at
-// 15.3 us per chunk of [128 x 64], separate code for k, v and q at 8.4 us with 41 % of the fetches missing.
-// So the three loaders run the same instructions, the branches between them are uniform, and loops over
-// columns stay rolled where registers allow.
+// Roles of a CTA (one per SM, six warpgroups): k, v and q are each converted by a warpgroup (one step per
+// thread) out of raw tiles that TMA has landed, in place for k and v; one turns scores into P, one keeps the
+// state (32 elements per thread and 64 of Dk in registers, fp32) and writes the output; of the last, three
+// single threads issue the MMAs and the TMA loads.  Tensors that TMA cannot describe (T % 4 != 0, unaligned)
+// are loaded by the converting threads themselves.
+//
+// What bounds it is the instruction stream.  A chunk of 128 steps and 64 channels a side (131 KB, 3.0 us of
+// an SM's share of copy bandwidth; 0.65 us of MMA time at the bf16 rate) takes 6.5 us, 12,000 cycles, in which
+// a scheduler issues 4,500 instructions, mostly the splitting into fp16 pairs, at 0.38 per cycle with a
+// sixth of the fetches missing the instruction cache.  Steps on the way: one loading warpgroup with two
+// operands in registers 15.3 us, a warpgroup per operand 8.9, the same code for the three 7.7, TMA with
+// raw tiles 7.7, waits that hold the warp in hardware instead of polling 6.4.
 //
 // A head with T steps is one CTA, or several when there are fewer heads than SMs: the axis is then cut
 // into segments, a first launch takes each segment's growth from zero, a small one joins them, and the
@@ -293,17 +298,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   // What travels beside the mantissas.  A slot of two is rewritten for chunk c + 2 once the read-out of
   // chunk c has ended, a slot of four once the output of chunk c + 1 has been written.
   __shared__ int f_s[2][kL];                                        // k's exponent
-  __shared__ __align__(16) float col_s[2][kL];                      // of a column of P: 2^(fg - mc)
-  __shared__ int mc_s[2], m_s[4][kL], qe_s[4][kL], mw_s[4];
-  __shared__ float scan_s[2][4];
-  __shared__ int kmax_s[2][8];
+  __shared__ int fg_s[2][kL];                                       // k's and v's exponents together
+  __shared__ __align__(16) float col_s[kL];                         // of a column of P: 2^(fg - largest fg)
+  __shared__ int m_s[4][kL], qe_s[4][kL], mw_s[4];
+  __shared__ float scan_s[4];
+  __shared__ int fmax_s[4], kmax_s[2][4];
   __shared__ float pow_pad[32 + kL + 1];       // r^n at 32 + n; zeros before it are the causal mask
   __shared__ __align__(16) float scale_s[2][64];
   __shared__ float top_s[kL];
   __shared__ int poison_s[64];
   __shared__ int any_poison_s, dead_s;
   __shared__ uint32_t tmem_s;
-  __shared__ __align__(8) uint64_t bars[28];
+  __shared__ __align__(8) uint64_t bars[30];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = tid >> 7, th = tid & 127, tw = warp & 3;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                  bar_q = bar(12), bar_qfree = bar(14);
   const uint32_t bar_sp = bar(16), bar_p = bar(17), bar_ds = bar(18), bar_s = bar(19), bar_o = bar(20), bar_ofree = bar(21),
                  bar_qraw = bar(22), bar_qread = bar(23), bar_end = bar(24), bar_dsfree = bar(25);
-  const uint32_t bar_kfree = bar(26);           // two
+  const uint32_t bar_kfree = bar(26), bar_vw = bar(28);    // two each
 
   // which head, segment, walk and columns
   const int64_t bid = blockIdx.x;
@@ -339,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mbar_init(bar_v + 8 * i, 128);
       mbar_init(bar_free + 8 * i, 1);
       mbar_init(bar_kfree + 8 * i, 1);
+      mbar_init(bar_vw + 8 * i, 128);
       mbar_init(bar_q + 8 * i, 128);
       mbar_init(bar_qfree + 8 * i, 2);
       mbar_init(bar_kx + 8 * i, 128);
@@ -385,15 +392,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     // ---------------- k, v, q: load, convert, hand on ----------------
     regs_inc<Regs<KT>::load>();
     const int j = th;
-    // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
-    const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
     const bool is_k = role == 0, is_v = role == 1, is_q = role == 2;
     const float* src = is_k ? w.k + head * (int64_t)Dk * T
                             : (is_v ? w.v + (head * (int64_t)w.Dv + e0) * T : w.q + head * (int64_t)Dk * T);
     const int rows = is_v ? ne : Dk;
     // Passes over an operand.  Dk > 64 needs the largest magnitude of both halves before either is converted:
     // k's raw tiles are looked through first; otherwise the first half is loaded, the second, which is
-    // converted while it is there, and the first again.  v: as it is, and weighted.
+    // converted while it is there, and the first again.  v: weighted, and as it is.
     const bool ahead = KT == 2 && is_k && boxes;
     const int passes = is_v ? (FULL ? 2 : 1) : (KT == 1 ? 1 : (ahead ? 2 : 3));
     const int mid = is_v || ahead ? 0 : KT - 1;  // the pass after whose load the exponent is known
@@ -475,48 +480,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
             const int g = fit_exponent(top);
             const int fg = (top > 0.f && f > kNoTerm) ? f + g : kNoTerm;
-            // weight of the step in the state, and the largest exponents: of all steps, of the weighted ones
+            // weight of the step in the state, and the largest exponent of the weighted steps
             const float wt = in ? pow_pad[32 + len - after - j] : 0.f;
             const int we = (int)((__float_as_uint(wt) >> 23) & 0xff) - 127;
             const int key = wt != 0.f && fg != kNoTerm ? fg + we : kNoTerm;
-            // running maximum of fg_j + (i - j) log2 r: the scan runs on that less i log2 r
-            float mk = fg == kNoTerm ? -1e30f : (float)fg - (float)j * slope;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const float up = __shfl_up_sync(0xffffffffu, mk, o);
-              if (lane >= o) mk = fmaxf(mk, up);
-            }
-            const int kmax = __reduce_max_sync(0xffffffffu, key), fmax = __reduce_max_sync(0xffffffffu, fg);
-            if (lane == 31) {
-              scan_s[c & 1][tw] = mk;
-              kmax_s[c & 1][tw] = kmax;
-              kmax_s[c & 1][4 + tw] = fmax;
-            }
+            const int kmax = __reduce_max_sync(0xffffffffu, key);
+            if (lane == 0) kmax_s[c & 1][tw] = kmax;
             bar_sync(1, 128);
-            int mw = kNoTerm, mc = kNoTerm;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (i < tw) mk = fmaxf(mk, scan_s[c & 1][i]);
-              mw = max(mw, kmax_s[c & 1][i]);
-              mc = max(mc, kmax_s[c & 1][4 + i]);
-            }
+            const int mw = max(max(kmax_s[c & 1][0], kmax_s[c & 1][1]), max(kmax_s[c & 1][2], kmax_s[c & 1][3]));
             if (!boxes && c >= NS) wait_phase(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
-            if (FULL) {
-              col_s[c & 1][j] = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
-              m_s[c & 3][j] = max(kNoTerm, (int)floorf(fmaxf(mk + (float)j * slope, (float)kNoTerm)) + 1);
-            }
-            if (j == 0) {
-              mc_s[c & 1] = mc;
-              mw_s[c & 3] = mw;
-            }
+            if (FULL) fg_s[c & 1][j] = fg;
+            if (j == 0) mw_s[c & 3] = mw;
             scale = p2(-g);
-            // r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa first
-            scale_w = key != kNoTerm ? (wt * p2(max(-we, -126))) * p2(max(fg + we - mw, -100)) : 0.f;
-            if (!FULL) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = mul2(x[e], pair(scale, scale));
-              scale = scale_w;
-            }
+            // 2^-g r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa first.  What this
+            // takes below a float's range is nothing in fp16 either.
+            scale_w = key != kNoTerm ? (wt * p2(max(-we, -126))) * p2(max(fg + we - mw, -100)) * scale : 0.f;
           }
         }
         if (pass < mid) continue;
@@ -526,9 +504,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             for (int d = 0; d < 32; ++d) x[d] = 0;
           }
         }
-        const bool weighted = is_v && (!FULL || pass == 1);
-        if (FULL && weighted) scale = scale_w;
-        const uint64_t sc = pair(scale, scale);
+        // the weighted rows first where the growth waits for them (Dk > 64: 18.2 against 20.2 us per chunk of both
+        // halves of v; Dk <= 64: 6.9 against 6.5)
+        const bool weighted = is_v && (!FULL || pass == (KT == 2 ? 0 : 1));
+        const float by = weighted ? scale_w : scale;
+        const uint64_t sc = pair(by, by);
         if (is_q) {
           // 16 channels of q (one step of an MMA) are 8 columns of hi and 8 of lo, side by side: one store
 #pragma unroll
@@ -549,39 +529,63 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           uint32_t h[4], l[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[4 * q8 + e] = mul2(x[4 * q8 + e], sc);       // v's weights come on top of its scale
-            split2(x[4 * q8 + e], &h[e], &l[e]);
+            split2(mul2(x[4 * q8 + e], sc), &h[e], &l[e]);
           }
           const uint32_t to = tile + (uint32_t)((q8 ^ (j & 7)) << 4);
           sts128(to, h[0], h[1], h[2], h[3]);
           sts128(to + kTileB, l[0], l[1], l[2], l[3]);
         }
+        if (is_v || pass == passes - 1) {
+          fence_proxy_async();
+          mbar_arrive((is_k ? bar_k : (weighted ? bar_vw : bar_v)) + 8 * (c % NS));
+        }
       }
-      if (is_k || is_v) {
-        fence_proxy_async();
-        mbar_arrive((is_k ? bar_k : bar_v) + 8 * (c % NS));
-        continue;
+      if (is_q) {
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar_q + 8 * (c & 1));
       }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(bar_q + 8 * (c & 1));
     }
   } else if (role == 3) {
     // ---------------- scores -> P: thread = row i ----------------
     if constexpr (Regs<KT>::p < 80) regs_dec<Regs<KT>::p>();
     if constexpr (FULL) {
       const int l = th;
+      // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
+      const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
 #pragma unroll 1
       for (int c = 0; c < nc; ++c) {
         const uint32_t sp = trow + S_::sp;
+        wait_phase(bar_vw + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);     // the steps' exponents
+        // running maximum of fg_j + (i - j) log2 r: the scan runs on that less i log2 r
+        const int fg = fg_s[c & 1][l];
+        float mk = fg == kNoTerm ? -1e30f : (float)fg - (float)l * slope;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float up = __shfl_up_sync(0xffffffffu, mk, o);
+          if (lane >= o) mk = fmaxf(mk, up);
+        }
+        const int fmax = __reduce_max_sync(0xffffffffu, fg);
+        if (lane == 31) {
+          scan_s[tw] = mk;
+          fmax_s[tw] = fmax;
+        }
+        bar_sync(6, 128);
+        const int mc = max(max(fmax_s[0], fmax_s[1]), max(fmax_s[2], fmax_s[3]));
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (i < tw) mk = fmaxf(mk, scan_s[i]);
+        const int m = max(kNoTerm, (int)floorf(fmaxf(mk + (float)l * slope, (float)kNoTerm)) + 1);
+        m_s[c & 3][l] = m;
+        col_s[l] = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
+        bar_sync(6, 128);
         wait_phase(bar_sp, (uint32_t)c & 1u, dead);
-        wait_phase(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);    // the columns' factors
         tc_fence_after();
         // |q_i . k_j| <= 2^score of the scaled vectors: P is held as its multiple of 2^(m + score - 15)
-        const float rowf = p2(max(-126, min(mc_s[c & 1] - m_s[c & 3][l] - (S_::score - 15), 127)));
+        const float rowf = p2(max(-126, min(mc - m - (S_::score - 15), 127)));
         const uint64_t rf = pair(rowf, rowf);
         const float* pw = &pow_pad[32 + l];      // r^(i - j), zero for j > i: the mask
-        const float* col = col_s[c & 1];
+        const float* col = col_s;
 #pragma unroll 1
         for (int g = 0; g < 128; g += 32, pw -= 32, col += 32) {
           uint32_t s[32];                        // 16 columns of hi and 16 of lo, in the place of 32 scores
@@ -796,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes,
                        v_hi = base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, vw_hi = base + S_::vw_at;
         if (!FULL) ok = wait_phase(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
-        ok = wait_phase(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
+        ok = wait_phase(bar_vw + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         if (c >= 1) ok = wait_phase(bar_dsfree, (uint32_t)(c - 1) & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();
@@ -828,6 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
         umma_commit(bar_qfree + 8 * (c & 1));
         mbar_arrive(bar_qfree + 8 * (c & 1));
+        ok = wait_phase(bar_v + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
         ok = wait_phase(bar_p, (uint32_t)c & 1u, dead) && ok;
         if (!ok) break;
         tc_fence_after();

@@ -44,7 +44,8 @@ def check_walk(arrays, out, final, T):
 SHAPES = [   # n, h, dk, dv, T
     (1, 1, 1, 1, 1), (2, 3, 5, 7, 2), (1, 2, 64, 64, 31), (2, 2, 64, 64, 128), (1, 2, 64, 64, 129), (3, 2, 16, 48, 300),
     (1, 3, 40, 72, 277), (2, 1, 128, 128, 257), (1, 2, 65, 33, 130), (1, 1, 128, 1, 200), (1, 1, 1, 128, 200),
-    (2, 2, 64, 64, 1000), (5, 4, 63, 64, 515), (1, 2, 100, 96, 2049)]
+    (2, 2, 64, 64, 1000), (5, 4, 63, 64, 515), (1, 2, 100, 96, 2049),
+    (1, 2, 128, 96, 260), (2, 1, 70, 128, 1284), (1, 3, 64, 64, 48), (3, 1, 64, 20, 47), (1, 2, 9, 33, 124)]
 
 
 @pytest.mark.parametrize('spikes', [False, True])
