@@ -175,49 +175,57 @@ int shape_walks(int64_t heads, int dk, int dv, int64_t T, bool backward, Walk* w
 
 // ---------------------------------------------------------------------------
 // One step on a kept state: reads and writes the state once, Dk x Dv floats each way.
-// Threads lie over the columns of a state row (four each) and over groups of rows.
+// Threads lie over the columns of a state row (four each) and over groups of rows; a thread's NI rows are
+// all loaded before the first is written back (they are the same memory, so the compiler would wait for one
+// after the other).
 // ---------------------------------------------------------------------------
-template <bool VEC>
+template <bool VEC, int NI>
 __global__ void __launch_bounds__(256)
 step_kernel(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
-            const float* __restrict__ decay, int n_decay, float* __restrict__ state, float* __restrict__ o, int Dk,
-            int Dv, int lanes) {
-  __shared__ float qs[kMaxDim], ks[kMaxDim];
+            const float* __restrict__ decay, int n_decay, float* state, float* __restrict__ o, int Dk, int Dv, int lanes) {
   __shared__ float part[256 * 4];
   const int64_t head = blockIdx.x;
   const int tid = threadIdx.x, col = (tid % lanes) * 4, group = tid / lanes, groups = 256 / lanes;
-  if (tid < Dk) {
-    qs[tid] = q[head * Dk + tid];
-    ks[tid] = k[head * Dk + tid];
+  float* S = state + head * Dk * Dv + col;
+  float x[NI][4], kd[NI], qd[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int d = group + i * groups;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+    kd[i] = qd[i] = 0.f;
+    if (d < Dk && col < Dv) {
+      if (VEC) {
+        const float4 a = *reinterpret_cast<const float4*>(S + (int64_t)d * Dv);
+        x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < Dv) x[i][e] = S[(int64_t)d * Dv + e];
+      }
+      kd[i] = __ldg(k + head * Dk + d);
+      qd[i] = __ldg(q + head * Dk + d);
+    }
   }
   const float r = 1.0f - decay[n_decay > 1 ? head % n_decay : 0] * (1.0f / 4096.0f);
   float ve[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) ve[e] = col + e < Dv ? v[head * Dv + col + e] : 0.f;
-  __syncthreads();
-  float* S = state + head * Dk * Dv + col;
-  if (col < Dv) {
-#pragma unroll 8
-    for (int d = group; d < Dk; d += groups) {
-      float x[4];
-      if (VEC) {
-        const float4 a = *reinterpret_cast<const float4*>(S + (int64_t)d * Dv);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      } else {
+  for (int e = 0; e < 4; ++e) ve[e] = col + e < Dv ? __ldg(v + head * Dv + col + e) : 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = col + e < Dv ? S[(int64_t)d * Dv + e] : 0.f;
-      }
+  for (int i = 0; i < NI; ++i) {
+    const int d = group + i * groups;
+    if (d < Dk && col < Dv) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = fmaf(r, x[e], ks[d] * ve[e]);
-        acc[e] = fmaf(qs[d], x[e], acc[e]);
+        x[i][e] = fmaf(r, x[i][e], kd[i] * ve[e]);
+        acc[e] = fmaf(qd[i], x[i][e], acc[e]);
       }
       if (VEC) {
-        *reinterpret_cast<float4*>(S + (int64_t)d * Dv) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(S + (int64_t)d * Dv) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (col + e < Dv) S[(int64_t)d * Dv + e] = x[e];
+          if (col + e < Dv) S[(int64_t)d * Dv + e] = x[i][e];
       }
     }
   }
@@ -228,6 +236,20 @@ step_kernel(const float* __restrict__ q, const float* __restrict__ k, const floa
     for (int g = 0; g < groups; ++g) sum += part[g * lanes * 4 + tid];
     o[head * Dv + tid] = sum;
   }
+}
+
+template <bool VEC>
+void launch_step(const float* q, const float* k, const float* v, const float* decay, int n_decay, float* state, float* o,
+                 int64_t heads, int Dk, int Dv, cudaStream_t s) {
+  int lanes = 1;
+  while (lanes * 4 < Dv) lanes *= 2;
+  const int rows = (Dk * lanes + 255) / 256;             // per thread: 1 to 16
+  const unsigned g = (unsigned)heads;
+  if (rows <= 1) step_kernel<VEC, 1><<<g, 256, 0, s>>>(q, k, v, decay, n_decay, state, o, Dk, Dv, lanes);
+  else if (rows <= 2) step_kernel<VEC, 2><<<g, 256, 0, s>>>(q, k, v, decay, n_decay, state, o, Dk, Dv, lanes);
+  else if (rows <= 4) step_kernel<VEC, 4><<<g, 256, 0, s>>>(q, k, v, decay, n_decay, state, o, Dk, Dv, lanes);
+  else if (rows <= 8) step_kernel<VEC, 8><<<g, 256, 0, s>>>(q, k, v, decay, n_decay, state, o, Dk, Dv, lanes);
+  else step_kernel<VEC, 16><<<g, 256, 0, s>>>(q, k, v, decay, n_decay, state, o, Dk, Dv, lanes);
 }
 
 int check_shape(int64_t heads, int64_t H, int64_t n_decay, int64_t Dk, int64_t Dv, int64_t T) {
@@ -286,14 +308,10 @@ int sb_linear_attention_step(const float* q, const float* k, const float* v, con
   SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, 1));
   if (heads == 0) return SB_OK;
   SB_REQUIRE(q && k && v && decay && state && out, "null tensor pointer");
-  int lanes = 1;
-  while (lanes * 4 < Dv) lanes *= 2;
   const bool vec = Dv % 4 == 0 && ((uintptr_t)state & 15u) == 0;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (vec)
-    step_kernel<true><<<(unsigned)heads, 256, 0, s>>>(q, k, v, decay, (int)n_decay, state, out, (int)Dk, (int)Dv, lanes);
-  else
-    step_kernel<false><<<(unsigned)heads, 256, 0, s>>>(q, k, v, decay, (int)n_decay, state, out, (int)Dk, (int)Dv, lanes);
+  const auto launch = vec ? launch_step<true> : launch_step<false>;
+  launch(q, k, v, decay, (int)n_decay, state, out, heads, (int)Dk, (int)Dv, s);
   SB_CUDA(cudaGetLastError());
   return SB_OK;
 }
