@@ -96,7 +96,7 @@ template <bool VEC>
 __global__ void __launch_bounds__(kThreads)
 dropout_rows_kernel(const float* __restrict__ x, float* __restrict__ y, const int64_t* __restrict__ key, int64_t n,
                     int64_t T, uint32_t threshold, float scale) {
-  __shared__ uint8_t keep_s[kSpan + 8];
+  __shared__ uint8_t keep_s[kSpan + 12];
   __shared__ int64_t row_s;
   const uint64_t seed = (uint64_t)key[0], offset = (uint64_t)key[1];
   const float inv = 1.0f / (float)T;
@@ -112,7 +112,8 @@ dropout_rows_kernel(const float* __restrict__ x, float* __restrict__ y, const in
       // whole numbers below 8192: half a unit from the next multiple is more than the rounding of the product
       return (int)(((float)((int)pos0 + i) + 0.5f) * inv);
     };
-    const int rows = row_of((int)left - 1) + 1, head = (int)(row0 & 3);
+    // (one row more than the span has: a group that ends with the span may look at it)
+    const int rows = row_of((int)left - 1) + 2, head = (int)(row0 & 3);
     for (int r = threadIdx.x * 4; r < rows + head; r += kThreads * 4) {
       const Words w = philox((uint64_t)((row0 - head + r) >> 2), offset, seed);
 #pragma unroll
@@ -126,9 +127,17 @@ dropout_rows_kernel(const float* __restrict__ x, float* __restrict__ y, const in
       const int at = (threadIdx.x + i * kThreads) * 4;
       keep[i] = 0;
       if (at < left) {
+        if (T >= 4) {                            // the group ends in its first row or in the next
+          const int r = row_of(at);
+          const int64_t here = T - (pos0 + at - r * T);           // values of the first row, 1 or more
+          const uint32_t first = here >= 4 ? 15u : (1u << here) - 1u;
+          keep[i] = keep_s[head + r] ? first : 0u;
+          if (here < 4 && keep_s[head + r + 1]) keep[i] |= 15u & ~first;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (at + e < left) keep[i] |= (uint32_t)keep_s[head + row_of(at + e)] << e;
+          for (int e = 0; e < 4; ++e)
+            if (at + e < left) keep[i] |= (uint32_t)keep_s[head + row_of(at + e)] << e;
+        }
         if (keep[i]) g[i] = load_group<VEC>(x + span + at, left - at);   // a dropped row is not read at all
       }
     }
