@@ -786,8 +786,7 @@ def _same_device(first, **others):
 
 def _written(t):
     """Tell autograd that a kernel wrote to ``t``: a graph that saved it must not use the new values."""
-    if not t.is_inference():
-        torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version(t)
 
 
 def _attention_check(q, k, v, decay, state, time):
@@ -853,7 +852,8 @@ def linear_attention_step(q, k, v, decay, state):
     n, h, dk, dv = _attention_check(q, k, v, decay, state, False)
     if not state.is_contiguous():
         raise ValueError('state is updated in place and must be contiguous')
-    q, k, v, decay = _c(q), _c(k), _c(v), _param(decay, q)
+    q, k, v = _c(q), _c(k), _c(v)
+    decay = _param(decay, q)
     out = torch.empty_like(v)
     N.call('sb_linear_attention_step', q, q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), decay.numel(),
            state.data_ptr(), out.data_ptr(), n * h, h or 1, dk, dv, N.stream_of(q))
@@ -866,20 +866,23 @@ def linear_attention_step(q, k, v, decay, state):
 # --------------------------------------------------------------------------
 def qdense_fwd(x, weight, weight_scale, in_neurons):
     """``[N, K, T]`` fp32 times int8 rows ``[O, Kp]`` (zero-padded) -> ``[N, O, T]`` fp32."""
-    N.require_cuda(x, weight_scale)
-    if weight.dtype != torch.int8:
+    device = x.device
+    if not x.is_cuda or x.dtype is not torch.float32 or weight_scale.dtype is not torch.float32:
+        N.require_cuda(x, weight_scale)
+    if weight.dtype is not torch.int8:
         raise TypeError(f'expected int8 weights, got {weight.dtype}')
-    _same_device(x, weight=weight, weight_scale=weight_scale)
+    if weight.device != device or weight_scale.device != device:
+        _same_device(x, weight=weight, weight_scale=weight_scale)
     n, k, T = x.shape
     if k != in_neurons:
         raise ValueError(f'expected {in_neurons} input neurons, found {k}')
     x, weight, weight_scale = _c(x), _c(weight), _c(weight_scale)
     o, kp = weight.shape
-    y = torch.empty(n, o, T, device=x.device, dtype=torch.float32)
-    nbytes = N.load().sb_qdense_scratch_bytes(n * T, kp)
+    y = torch.empty((n, o, T), device=x.device, dtype=torch.float32)
+    nbytes = (N._lib or N.load()).sb_qdense_scratch_bytes(n * T, kp)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes > 0 else None
-    N.call('sb_qdense_fwd', x, N.ptr(x), N.ptr(weight), N.ptr(weight_scale), N.ptr(y), n, k, kp, o, T,
-           N.ptr(scratch), N.stream_of(x))
+    N.call('sb_qdense_fwd', x, x.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), y.data_ptr(), n, k, kp, o, T,
+           None if scratch is None else scratch.data_ptr(), N.stream_of(x))
     return y
 
 
