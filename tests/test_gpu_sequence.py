@@ -233,6 +233,32 @@ def test_attention_strides_streams_and_repeats(cuda):
     assert torch.equal(*(torch.autograd.grad(attention.dynamics(q, full, v, decay, s), full, go)[0] for _ in range(2)))
 
 
+@pytest.mark.parametrize('shape', [(2, 2, 64, 64, 300), (1, 2, 128, 72, 200), (1, 2, 16, 16, 20)])
+def test_attention_unaligned(cuda, shape):
+    """Contiguous tensors that start between 16-byte boundaries: other loads, the same values."""
+    arrays, rng = make(15, *shape)
+    aligned = [dev(a) for a in arrays]
+
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, device='cuda')
+        return flat[1:].view(t.shape).copy_(t)
+
+    odd = [moved(t) for t in aligned]
+    with torch.no_grad():
+        for a, b in zip(attention.dynamics(*aligned, return_state=True), attention.dynamics(*odd, return_state=True)):
+            assert torch.equal(a, b)
+    go = moved(dev(rng.normal(size=arrays[2].shape).astype(np.float32)))
+    grads = []
+    for args in (aligned, odd):
+        leaves = [t.detach().requires_grad_() for t in args[:3]]
+        grads.append(torch.autograd.grad(attention.dynamics(*leaves, args[3], args[4]), leaves, go))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    q, k, v = (moved(t[..., 0].contiguous()) for t in aligned[:3])
+    kept, want = moved(aligned[4]), aligned[4].clone()
+    assert torch.equal(attention.step(q, k, v, odd[3], kept), attention.step(q, k, v, aligned[3], want))
+    assert torch.equal(kept, want)
+
+
 def test_attention_empty(cuda):
     z = torch.zeros(2, 3, 8, 0, device='cuda')
     s = torch.randn(2, 3, 8, 8, device='cuda')
@@ -472,6 +498,40 @@ def test_attention_block_training(cuda):
     for name in ('query', 'key', 'value'):
         assert getattr(b, name + '_synapse').weight.grad.abs().max() > 0, name
     assert b.neuron.drop.generator.tolist()[1] == 4
+
+
+def test_attention_block_training_captured(cuda):
+    """A captured training step: the gradients of the eager one under the same masks, new masks at each replay."""
+    x = (torch.rand(3, 24, 200, generator=torch.Generator().manual_seed(2)) < 0.3).float().cuda()
+    b = block(drop=slayer.neuron.Dropout(0.2, seed=1))
+
+    def step(module):
+        weights = [p for p in module.parameters() if p.requires_grad]
+        return torch.autograd.grad(module(x).sum(), weights, allow_unused=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(b)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step(b)
+    start = int(b.neuron.drop.generator[1])
+    seen = []
+    for i in range(2):
+        graph.replay()
+        got = [g.clone() for g in grads if g is not None]
+        fresh = block(drop=slayer.neuron.Dropout(0.2, seed=1))
+        fresh.load_state_dict(b.state_dict())
+        fresh.neuron.drop.generator.copy_(torch.tensor([1, start + 4 * i]))
+        want = [g for g in step(fresh) if g is not None]
+        # (the synapses' own gradients are library sums, whose order may differ)
+        for g, w in zip(got, want):
+            assert torch.allclose(g, w, rtol=1e-4, atol=1e-4 * float(w.abs().max()))
+        seen.append(got)
+    assert any(not torch.equal(a, c) for a, c in zip(*seen))
 
 
 def test_attention_block_quantized(cuda):
