@@ -29,13 +29,23 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int kTile = 8;
 
-template <int NI>
-__global__ void __launch_bounds__(128) walk_kernel(Walk w) {
+struct Walks {
+  Walk w[3];
+};
+
+// MANY: one walk per blockIdx.z, copied out of the parameters (indexed, they would be read in the loops);
+// a single walk reads them as constants, which saves the registers (66 against 94 us at [64, 16, 64, 48]).
+template <int NI, bool MANY>
+__global__ void __launch_bounds__(128) walk_kernel(const __grid_constant__ Walks walks) {
+  Walk copy;
+  if (MANY) copy = walks.w[blockIdx.z];
+  const Walk& w = MANY ? copy : walks.w[0];
   __shared__ float qs[kTile][8 * NI], ks[kTile][8 * NI], vs[kTile][64];
   __shared__ float part[kTile][8][64];
   const int tid = threadIdx.x, ec = (tid & 15) * 4, dg = tid >> 4;
   const int64_t head = blockIdx.x;
   const int e0 = blockIdx.y * 64;
+  if (e0 >= w.Dv) return;
   const int ne = min(64, w.Dv - e0);
   const float delta = w.decay[w.n_decay > 1 ? head % w.n_decay : 0] * (1.0f / 4096.0f);
   const float r = __fsub_rn(1.0f, delta), r_lo = __fsub_rn(__fsub_rn(1.0f, r), delta);
@@ -117,16 +127,50 @@ __global__ void __launch_bounds__(128) walk_kernel(Walk w) {
   }
 }
 
-int launch_walk(const Walk& w, cudaStream_t s) {
-  const dim3 grid((unsigned)w.heads, (unsigned)((w.Dv + 63) / 64));
-  if (w.Dk <= 64) walk_kernel<8><<<grid, 128, 0, s>>>(w);
-  else walk_kernel<16><<<grid, 128, 0, s>>>(w);
-  SB_CUDA(cudaGetLastError());
+int launch_walks(const Walk* walks, int n, cudaStream_t s) {
+  Walks a{};
+  int dk = 0, dv = 0;
+  for (int i = 0; i < n; ++i) {
+    a.w[i] = walks[i];
+    dk = walks[i].Dk > dk ? walks[i].Dk : dk;
+    dv = walks[i].Dv > dv ? walks[i].Dv : dv;
+  }
+  const unsigned heads = (unsigned)walks[0].heads, tiles = (unsigned)((dv + 63) / 64);
+  if (n > 1 && walks[0].heads * tiles <= sm_count()) {      // few heads: side by side in one launch
+    const dim3 grid(heads, tiles, (unsigned)n);
+    if (dk <= 64) walk_kernel<8, true><<<grid, 128, 0, s>>>(a);
+    else walk_kernel<16, true><<<grid, 128, 0, s>>>(a);
+    SB_CUDA(cudaGetLastError());
+    return SB_OK;
+  }
+  for (int i = 0; i < n; ++i) {
+    a.w[0] = walks[i];
+    const dim3 grid(heads, (unsigned)((walks[i].Dv + 63) / 64));
+    if (walks[i].Dk <= 64) walk_kernel<8, false><<<grid, 128, 0, s>>>(a);
+    else walk_kernel<16, false><<<grid, 128, 0, s>>>(a);
+    SB_CUDA(cudaGetLastError());
+  }
   return SB_OK;
 }
 
-// Short sequences walk step by step; from kMinSteps on the chunked kernel is ahead.
-constexpr int64_t kMinSteps = 48;
+// Whether sequences shorter than a chunk walk step by step.  The chunked kernel takes 12.5 us (Dk > 64: 15.5)
+// for every wave of CTAs whatever their length; the walk 4 us and for each step 0.45 us (twice that for
+// Dk > 64) or, with many heads, 1.3 ns for each of its blocks.  [1, 8, 64, T]: 9.0 against 12.5 us at T = 16,
+// 16.5 at 32; [64, 16, 64, T]: 66 against 89 at T = 48, 135 at 96.
+bool walks_by_steps(const Walk* w, int n) {
+  const int64_t T = w[0].T;
+  if (T >= 128) return false;
+  int64_t blocks = 0;
+  bool wide = false;
+  for (int i = 0; i < n; ++i) {
+    blocks += w[i].heads * ((w[i].Dv + 63) / 64);
+    wide = wide || w[i].Dk > 64;
+  }
+  const double per_step = 1.3e-3 * (double)blocks > 0.45 ? 1.3e-3 * (double)blocks : 0.45;
+  const double steps = 4.0 + (double)T * per_step * (wide ? 2.0 : 1.0);
+  const double chunk = (wide ? 15.5 : 12.5) * (double)((blocks + sm_count() - 1) / sm_count());
+  return steps < chunk;
+}
 
 // Splits walks into the two widths of the chunked kernel; returns how many come first.
 int by_width(const Walk* in, int n, Walk* out) {
@@ -140,10 +184,7 @@ int by_width(const Walk* in, int n, Walk* out) {
 }
 
 int run_walks(const Walk* walks, int n, void* scratch, cudaStream_t s) {
-  if (walks[0].T < kMinSteps) {
-    for (int i = 0; i < n; ++i) SB_TRY(launch_walk(walks[i], s));
-    return SB_OK;
-  }
+  if (walks_by_steps(walks, n)) return launch_walks(walks, n, s);
   Walk w[3];
   const int narrow = by_width(walks, n, w);
   float* f = static_cast<float*>(scratch);
@@ -268,7 +309,7 @@ int check_shape(int64_t heads, int64_t H, int64_t n_decay, int64_t Dk, int64_t D
 extern "C" {
 
 int64_t sb_linear_attention_scratch_bytes(int64_t heads, int64_t Dk, int64_t Dv, int64_t T, int backward) {
-  if (check_shape(heads, 1, 1, Dk, Dv, T) != SB_OK || heads == 0 || T < kMinSteps) return 0;
+  if (check_shape(heads, 1, 1, Dk, Dv, T) != SB_OK || heads == 0 || T < 128) return 0;   // (one chunk is not cut)
   Walk all[3], w[3];
   const int n = shape_walks(heads, (int)Dk, (int)Dv, T, backward != 0, all);
   const int narrow = by_width(all, n, w);

@@ -280,7 +280,6 @@ __device__ __forceinline__ int fit_exponent(float top) {
   return max(e, -113) - 13;
 }
 __device__ __forceinline__ bool not_finite(float top) { return __float_as_uint(top) >= 0x7f800000u; }
-// KT: 64-wide tiles of Dk.  FULL: the walk itself; otherwise only the state after each segment but the last.
 template <int R>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
@@ -290,6 +289,7 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 
+// KT: 64-wide tiles of Dk.  FULL: the walk itself; otherwise only the state after each segment but the last.
 template <int KT, bool FULL>
 __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ TcArgs args) {
   using S_ = Shape<KT>;

@@ -791,11 +791,12 @@ def _written(t):
 
 def _attention_check(q, k, v, decay, state, time):
     """Argument checks of the linear attention; returns (samples, H, Dk, Dv)."""
-    device, f32 = q.device, torch.float32
-    for name, t in (('query', q), ('key', k), ('value', v), ('decay', decay), ('state', state)):
-        if t is not None and (t.dtype is not f32 or t.device != device or not t.is_cuda):
-            N.require_cuda(t)
-            _same_device(q, **{name: t})
+    f32, device = torch.float32, q.get_device()
+    if not (device >= 0 and k.get_device() == v.get_device() == decay.get_device() == device
+            and q.dtype is f32 and k.dtype is f32 and v.dtype is f32 and decay.dtype is f32
+            and (state is None or (state.get_device() == device and state.dtype is f32))):
+        N.require_cuda(q, k, v, decay, state)
+        _same_device(q, key=k, value=v, decay=decay, state=state)
     shape, vshape = q.shape, v.shape
     dims = 4 if time else 3
     if len(shape) != dims or k.shape != shape:
