@@ -153,23 +153,29 @@ int launch_walks(const Walk* walks, int n, cudaStream_t s) {
   return SB_OK;
 }
 
-// Whether sequences shorter than a chunk walk step by step.  The chunked kernel takes 12.5 us (Dk > 64: 15.5)
-// for every wave of CTAs whatever their length; the walk 4 us and for each step 0.45 us (twice that for
-// Dk > 64) or, with many heads, 1.3 ns for each of its blocks.  [1, 8, 64, T]: 9.0 against 12.5 us at T = 16,
-// 16.5 at 32; [64, 16, 64, T]: 66 against 89 at T = 48, 135 at 96.
+// Whether sequences shorter than a chunk walk step by step, in us.  The chunked kernel takes 1.5 and 9.6 (Dk > 64:
+// 13.2) for every wave of items whatever their length; a launch of walks takes 3 and for each step 0.48 or, with
+// many blocks, 1.3 ns for each of them (twice that for Dk > 64).  Steps against chunks: [1, 8, 64, T] 9.4 and 10.9
+// at T = 16, 17.2 and 11.2 at 32; [64, 16, 64, T] 67 and 70 at T = 48, 90 and 68 at 64; their gradients 71 and 202
+// at T = 16, 199 and 203 at 48; [16, 16, 128, T] 49 and 52 at T = 32.
 bool walks_by_steps(const Walk* w, int n) {
   const int64_t T = w[0].T;
   if (T >= 128) return false;
-  int64_t blocks = 0;
-  bool wide = false;
+  int64_t items = 0;
+  bool wide = false, few = n > 1;                // few heads: the walks side by side in one launch
+  double steps = 0.0;
   for (int i = 0; i < n; ++i) {
-    blocks += w[i].heads * ((w[i].Dv + 63) / 64);
+    const int64_t blocks = w[i].heads * ((w[i].Dv + 63) / 64);
+    items += blocks;
     wide = wide || w[i].Dk > 64;
+    few = few && blocks <= sm_count();
   }
-  const double per_step = 1.3e-3 * (double)blocks > 0.45 ? 1.3e-3 * (double)blocks : 0.45;
-  const double steps = 4.0 + (double)T * per_step * (wide ? 2.0 : 1.0);
-  const double chunk = (wide ? 15.5 : 12.5) * (double)((blocks + sm_count() - 1) / sm_count());
-  return steps < chunk;
+  for (int i = 0; i < (few ? 1 : n); ++i) {
+    const double blocks = few ? (double)items : (double)(w[i].heads * ((w[i].Dv + 63) / 64));
+    const double many = (few ? 2.0e-3 : 1.3e-3) * blocks, per_step = many > 0.48 ? many : 0.48;
+    steps += 3.0 + (double)T * per_step * (w[i].Dk > 64 ? 2.0 : 1.0);
+  }
+  return steps < 1.5 + (wide ? 13.2 : 9.6) * (double)((items + sm_count() - 1) / sm_count());
 }
 
 // Splits walks into the two widths of the chunked kernel; returns how many come first.

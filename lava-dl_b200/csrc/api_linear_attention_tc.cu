@@ -79,6 +79,7 @@ struct TcArgs {
   int sub_walk[kMaxSub], sub_e0[kMaxSub];
   int64_t heads;
   int nseg, seg_chunks;
+  int64_t items;        // (segment, head, sub) triples of this launch, sub fastest; a CTA takes every gridDim-th
   int boxes;            // TMA can describe the tensors: 16-byte bases, T % 4 == 0
   unsigned int* status;
 };
@@ -119,6 +120,18 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volati
       return false;
     }
   }
+}
+
+// Barrier of `threads` threads that tells all of them whether one brought `x`.
+__device__ __forceinline__ bool bar_any(int id, int threads, bool x) {
+  int any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(any) : "r"((int)x), "r"(id), "r"(threads) : "memory");
+  return any != 0;
 }
 
 __device__ __forceinline__ float p2(int n) { return __int_as_float((n + 127) << 23); }   // -126 <= n <= 127
@@ -289,6 +302,23 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 
+// What a CTA walks in one go: a segment of a head for one walk and 64 columns of its v.  One thread works the
+// items out; the others read what they need from shared memory, where it costs them no registers.
+struct Item {
+  const float* src[3];       // k, v (from the first column), q
+  float* o;
+  const float* s_from;       // state before the first step, after the last; nullable
+  float* s_to;
+  int64_t from_row, from_col, to_row, to_col;
+  int nc, t0;                // chunks (0: no more items), first step
+  int head, e0, ne, Dk;
+  int wi, reverse, after;
+  int any_poison;
+  int poison[64];            // first spoilt step of each column
+  float pw[32 + kL + 1];     // r^n at 32 + n; zeros before it are the causal mask
+};
+constexpr int kItems = 4;    // in the works
+
 // KT: 64-wide tiles of Dk.  FULL: the walk itself; otherwise only the state after each segment but the last.
 template <int KT, bool FULL>
 __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ TcArgs args) {
@@ -303,19 +333,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   __shared__ int m_s[4][kL], qe_s[4][kL], mw_s[4];
   __shared__ float scan_s[4];
   __shared__ int fmax_s[4], kmax_s[2][4];
-  __shared__ float pow_pad[32 + kL + 1];       // r^n at 32 + n; zeros before it are the causal mask
+  __shared__ Item items_s[kItems];
   __shared__ __align__(16) float scale_s[2][64];
   __shared__ float top_s[kL];
-  __shared__ int poison_s[64];
-  __shared__ int any_poison_s, dead_s;
+  __shared__ int dead_s;
   __shared__ uint32_t tmem_s;
-  __shared__ __align__(8) uint64_t bars[30];
+  __shared__ __align__(8) uint64_t bars[42];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = tid >> 7, th = tid & 127, tw = warp & 3;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t sbase = base + S_::s_at;
   volatile int* dead = &dead_s;
-  volatile int* any_poison = &any_poison_s;
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
   // by stage or chunk parity: two each
@@ -323,21 +351,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                  bar_q = bar(12), bar_qfree = bar(14);
   const uint32_t bar_sp = bar(16), bar_p = bar(17), bar_ds = bar(18), bar_s = bar(19), bar_o = bar(20), bar_ofree = bar(21),
                  bar_qraw = bar(22), bar_qread = bar(23), bar_end = bar(24), bar_dsfree = bar(25);
-  const uint32_t bar_kfree = bar(26), bar_vw = bar(28);    // two each
+  const uint32_t bar_kfree = bar(26), bar_vw = bar(28);
+  const uint32_t bar_item = bar(30), bar_itemfree = bar(34), bar_powers = bar(38);   // kItems each
 
-  // which head, segment, walk and columns
-  const int64_t bid = blockIdx.x;
-  const int sub = (int)(bid % args.nsub);
-  const int64_t head = (bid / args.nsub) % args.heads;
-  const int seg = (int)(bid / args.nsub / args.heads);
-  const int wi = args.sub_walk[sub], e0 = args.sub_e0[sub];
-  const Walk& w = args.w[wi];
-  const int64_t T = w.T;
-  const int Dk = w.Dk, ne = min(64, w.Dv - e0);
-  const int64_t c0 = (int64_t)seg * args.seg_chunks;
-  const int nc = (int)min((int64_t)args.seg_chunks, (T + kL - 1) / kL - c0);
-  const int after = w.after;
+  // Every role goes through the CTA's items, and through the chunks of each; barriers and slots follow the
+  // chunk count over all of them (g), so the next item is loaded and converted under the end of the last.
+  const int T = (int)args.w[0].T;
   const bool boxes = args.boxes != 0;
+  // the n-th item, once it is there; null when there are no more
+  auto item_at = [&](int n) -> Item* {
+    Item* item = &items_s[n % kItems];
+    if (!wait_phase(bar_item + 8 * (n % kItems), (uint32_t)(n / kItems) & 1u, dead) || *dead) return nullptr;
+    return *(volatile int*)&item->nc ? item : nullptr;
+  };
+  // the same for a warpgroup, with or without the powers: all of it goes on, or none
+  auto group_item = [&](int n, bool powers) -> Item* {
+    Item* item = item_at(n);
+    if (item && powers) wait_phase(bar_powers + 8 * (n % kItems), (uint32_t)(n / kItems) & 1u, dead);
+    return bar_any(7 + role, 128, item == nullptr) ? nullptr : item;
+  };
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -352,6 +384,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mbar_init(bar_kraw + 8 * i, 1);
       mbar_init(bar_vraw + 8 * i, 1);
     }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(bar_item + 8 * i, 1);
+      mbar_init(bar_powers + 8 * i, 32);
+      mbar_init(bar_itemfree + 8 * i, 128);
+    }
     mbar_init(bar_qraw, 1);
     mbar_init(bar_qread, 128);
     mbar_init(bar_sp, 2);
@@ -364,19 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     mbar_init(bar_end, 1);
     fence_mbar_init();
     dead_s = 0;
-    any_poison_s = 0;
   }
-  if (tid < 64) poison_s[tid] = 0x7fffffff;
-  if (tid < 32) pow_pad[tid] = 0.f;
-  if (tid <= kL) {
-    // r^n by squaring in 64 bits: r itself does not fit 32 (a slow head multiplies it a thousandfold)
-    double b = 1.0 - (double)w.decay[w.n_decay > 1 ? head % w.n_decay : 0] / 4096.0, p = 1.0;
-    for (int n = tid; n; n >>= 1) {
-      if (n & 1) p *= b;
-      b *= b;
-    }
-    pow_pad[32 + tid] = (float)p;
-  }
+  if (tid < 32 * kItems) items_s[tid >> 5].pw[tid & 31] = 0.f;
   if (role == 5 && tw == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
@@ -393,23 +419,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     regs_inc<Regs<KT>::load>();
     const int j = th;
     const bool is_k = role == 0, is_v = role == 1, is_q = role == 2;
-    const float* src = is_k ? w.k + head * (int64_t)Dk * T
-                            : (is_v ? w.v + (head * (int64_t)w.Dv + e0) * T : w.q + head * (int64_t)Dk * T);
-    const int rows = is_v ? ne : Dk;
     // Passes over an operand.  Dk > 64 needs the largest magnitude of both halves before either is converted:
     // k's raw tiles are looked through first; otherwise the first half is loaded, the second, which is
     // converted while it is there, and the first again.  v: weighted, and as it is.
     const bool ahead = KT == 2 && is_k && boxes;
     const int passes = is_v ? (FULL ? 2 : 1) : (KT == 1 ? 1 : (ahead ? 2 : 3));
     const int mid = is_v || ahead ? 0 : KT - 1;  // the pass after whose load the exponent is known
+    int g = 0;
 #pragma unroll 1
-    for (int c = (FULL || !is_q) ? 0 : nc; c < nc; ++c) {
-      const uint32_t slot = base + (is_k ? (uint32_t)(c % NS) * S_::k_bytes
-                                         : (is_v ? S_::v_at + (uint32_t)(c % NS) * S_::v_bytes : S_::q_at));
-      const int64_t t = (c0 + c) * kL + j;
-      const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
-      const bool in = j < len, whole = len == kL;
-      const float* at = src + (w.reverse ? T - 1 - t : t);
+    for (int n = 0; FULL || !is_q; ++n) {
+    Item* const item = group_item(n, is_v);
+    if (!item) break;
+    int t0 = item->t0;
+#pragma unroll 1
+    for (int left = item->nc; left > 0; --left, t0 += kL, ++g) {
+      const uint32_t slot = base + (is_k ? (uint32_t)(g % NS) * S_::k_bytes
+                                         : (is_v ? S_::v_at + (uint32_t)(g % NS) * S_::v_bytes : S_::q_at));
+      const int t = t0 + j;
       uint64_t x[32];
       float top = 0.f, scale = 0.f, scale_w = 0.f;
       bool zero = false;                         // the whole vector is left out
@@ -420,19 +446,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           if (boxes) {
             // the raw tile, a step earlier or later in memory by direction; its place is free to be written
             // (k, v) or to receive the next tile (q) once the whole warpgroup has read it
-            const uint32_t raw_at = slot + (uint32_t)(w.reverse ? kL - 1 - j : j) * 4;
+            const uint32_t raw_at = slot + (uint32_t)(item->reverse ? kL - 1 - j : j) * 4;
             if (is_q) {
-              const uint32_t n = (uint32_t)(KT == 1 ? c : 3 * c + pass);
-              wait_phase(bar_qraw, n & 1u, dead);
+              wait_phase(bar_qraw, (uint32_t)(KT == 1 ? g : 3 * g + pass) & 1u, dead);
             } else if (pass == 0) {
-              wait_phase((is_k ? bar_kraw : bar_vraw) + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);
+              wait_phase((is_k ? bar_kraw : bar_vraw) + 8 * (g % NS), (uint32_t)(g / NS) & 1u, dead);
               if (ahead) top = top64_shared(raw_at + 2 * kTileB, top);
             }
             load64_shared(x, raw_at + (is_k ? (uint32_t)half * 2 * kTileB : 0u));
             if (is_q) mbar_arrive(bar_qread);
             else bar_sync(3 + role, 128);
           } else {
-            load64(x, at + (int64_t)half * 64 * T, T, rows - half * 64, in, whole);
+            const float* at = item->src[role] + (item->reverse ? T - 1 - t : t) + (int64_t)half * 64 * T;
+            const int rows = (is_v ? item->ne : item->Dk) - half * 64;
+            load64(x, at, T, rows, t < T, t0 + kL <= T);
           }
         }
         if (pass <= mid) top = top64(x, top);
@@ -440,32 +467,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           const bool bad = not_finite(top);
           if (is_k) {
             if (bad) {                           // every column of the output is spoilt from this step on
-              for (int e = 0; e < 64; ++e) atomicMin(&poison_s[e], (int)t);
-              any_poison_s = 1;
+              for (int e = 0; e < 64; ++e) atomicMin(&item->poison[e], t);
+              item->any_poison = 1;
               zero = true;
             }
             const int f = fit_exponent(bad ? 0.f : top);
             scale = p2(-f);
-            if (!boxes && c >= NS) wait_phase(bar_kfree + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
-            f_s[c & 1][j] = bad ? kNoTerm - 1 : (top > 0.f ? f : kNoTerm);
-            mbar_arrive(bar_kx + 8 * (c & 1));
+            if (!boxes && g >= NS) wait_phase(bar_kfree + 8 * (g % NS), (uint32_t)(g / NS - 1) & 1u, dead);
+            f_s[g & 1][j] = bad ? kNoTerm - 1 : (top > 0.f ? f : kNoTerm);
+            mbar_arrive(bar_kx + 8 * (g & 1));
           } else if (is_q) {
             zero = bad;
             const int qe = bad ? 0 : fit_exponent(top);
             scale = p2(-qe);
-            if (c >= S_::nq)
-              wait_phase(bar_qfree + 8 * ((c - S_::nq) & 1), (uint32_t)((c - S_::nq) >> 1) & 1u, dead);
+            if (g >= S_::nq)
+              wait_phase(bar_qfree + 8 * ((g - S_::nq) & 1), (uint32_t)((g - S_::nq) >> 1) & 1u, dead);
             tc_fence_after();
-            qe_s[c & 3][j] = bad ? 0x7fffffff : qe;
+            qe_s[g & 3][j] = bad ? 0x7fffffff : qe;
           } else {
             // v, and what P and the growth need to know of the steps
-            wait_phase(bar_kx + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
-            const int f = f_s[c & 1][j];
+            wait_phase(bar_kx + 8 * (g & 1), (uint32_t)(g >> 1) & 1u, dead);
+            const int f = f_s[g & 1][j];
             zero = f == kNoTerm - 1;
             if (bad && !zero) {                  // single columns are spoilt; the rest of the vector counts
-              for (int e = 0; e < ne; ++e)
-                if (not_finite(fabsf(at[(int64_t)e * T]))) atomicMin(&poison_s[e], (int)t);
-              any_poison_s = 1;
+              const float* at = item->src[1] + (item->reverse ? T - 1 - t : t);
+              for (int e = 0; e < item->ne; ++e)
+                if (not_finite(fabsf(at[(int64_t)e * T]))) atomicMin(&item->poison[e], t);
+              item->any_poison = 1;
             }
             if (bad || zero) {
               top = 0.f;
@@ -478,20 +506,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
                 x[e] = pair(v.x, v.y);
               }
             }
-            const int g = fit_exponent(top);
-            const int fg = (top > 0.f && f > kNoTerm) ? f + g : kNoTerm;
+            const int vg = fit_exponent(top);
+            const int fg = (top > 0.f && f > kNoTerm) ? f + vg : kNoTerm;
             // weight of the step in the state, and the largest exponent of the weighted steps
-            const float wt = in ? pow_pad[32 + len - after - j] : 0.f;
+            const float wt = t < T ? item->pw[32 + min(kL, T - t0) - item->after - j] : 0.f;
             const int we = (int)((__float_as_uint(wt) >> 23) & 0xff) - 127;
             const int key = wt != 0.f && fg != kNoTerm ? fg + we : kNoTerm;
             const int kmax = __reduce_max_sync(0xffffffffu, key);
-            if (lane == 0) kmax_s[c & 1][tw] = kmax;
+            if (lane == 0) kmax_s[g & 1][tw] = kmax;
             bar_sync(1, 128);
-            const int mw = max(max(kmax_s[c & 1][0], kmax_s[c & 1][1]), max(kmax_s[c & 1][2], kmax_s[c & 1][3]));
-            if (!boxes && c >= NS) wait_phase(bar_free + 8 * (c % NS), (uint32_t)(c / NS - 1) & 1u, dead);
-            if (FULL) fg_s[c & 1][j] = fg;
-            if (j == 0) mw_s[c & 3] = mw;
-            scale = p2(-g);
+            const int mw = max(max(kmax_s[g & 1][0], kmax_s[g & 1][1]), max(kmax_s[g & 1][2], kmax_s[g & 1][3]));
+            if (!boxes && g >= NS) wait_phase(bar_free + 8 * (g % NS), (uint32_t)(g / NS - 1) & 1u, dead);
+            if (FULL) fg_s[g & 1][j] = fg;
+            if (j == 0) mw_s[g & 3] = mw;
+            scale = p2(-vg);
             // 2^-g r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa first.  What this
             // takes below a float's range is nothing in fp16 either.
             scale_w = key != kNoTerm ? (wt * p2(max(-we, -126))) * p2(max(fg + we - mw, -100)) * scale : 0.f;
@@ -516,13 +544,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             uint32_t r[16];
 #pragma unroll
             for (int e = 0; e < 8; ++e) split2(mul2(x[b + e], sc), &r[e], &r[8 + e]);
-            tmem_st16(trow + S_::q + (uint32_t)(c % S_::nq) * 64 + half * 64 + 2 * b, r);
+            tmem_st16(trow + S_::q + (uint32_t)(g % S_::nq) * 64 + half * 64 + 2 * b, r);
           }
           if constexpr (KT == 1) break;          // (x is not carried on)
           continue;
         }
         // one row of a hi and a lo tile (128-byte swizzle)
-        if (weighted && c >= 1) wait_phase(bar_ds, (uint32_t)(c - 1) & 1u, dead);    // read by the growth before
+        if (weighted && g >= 1) wait_phase(bar_ds, (uint32_t)(g - 1) & 1u, dead);    // read by the growth before
         const uint32_t tile = (weighted ? base + S_::vw_at : slot + (uint32_t)half * 2 * kTileB) + (uint32_t)(j * 128);
 #pragma unroll
         for (int q8 = 0; q8 < 8; ++q8) {
@@ -537,28 +565,34 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
         if (is_v || pass == passes - 1) {
           fence_proxy_async();
-          mbar_arrive((is_k ? bar_k : (weighted ? bar_vw : bar_v)) + 8 * (c % NS));
+          mbar_arrive((is_k ? bar_k : (weighted ? bar_vw : bar_v)) + 8 * (g % NS));
         }
       }
       if (is_q) {
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(bar_q + 8 * (c & 1));
+        mbar_arrive(bar_q + 8 * (g & 1));
       }
+    }
     }
   } else if (role == 3) {
     // ---------------- scores -> P: thread = row i ----------------
     if constexpr (Regs<KT>::p < 80) regs_dec<Regs<KT>::p>();
     if constexpr (FULL) {
       const int l = th;
-      // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
-      const float slope = fminf(fmaxf(log2f(fabsf(pow_pad[33])), -250.f), 250.f);
+      int g = 0;
 #pragma unroll 1
-      for (int c = 0; c < nc; ++c) {
+      for (int n = 0;; ++n) {
+      const Item* const item = group_item(n, true);
+      if (!item) break;
+      // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
+      const float slope = fminf(fmaxf(log2f(fabsf(item->pw[33])), -250.f), 250.f);
+#pragma unroll 1
+      for (int left = item->nc; left > 0; --left, ++g) {
         const uint32_t sp = trow + S_::sp;
-        wait_phase(bar_vw + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead);     // the steps' exponents
+        wait_phase(bar_vw + 8 * (g % NS), (uint32_t)(g / NS) & 1u, dead);     // the steps' exponents
         // running maximum of fg_j + (i - j) log2 r: the scan runs on that less i log2 r
-        const int fg = fg_s[c & 1][l];
+        const int fg = fg_s[g & 1][l];
         float mk = fg == kNoTerm ? -1e30f : (float)fg - (float)l * slope;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -576,22 +610,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         for (int i = 0; i < 3; ++i)
           if (i < tw) mk = fmaxf(mk, scan_s[i]);
         const int m = max(kNoTerm, (int)floorf(fmaxf(mk + (float)l * slope, (float)kNoTerm)) + 1);
-        m_s[c & 3][l] = m;
+        m_s[g & 3][l] = m;
         col_s[l] = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
         bar_sync(6, 128);
-        wait_phase(bar_sp, (uint32_t)c & 1u, dead);
+        wait_phase(bar_sp, (uint32_t)g & 1u, dead);
         tc_fence_after();
         // |q_i . k_j| <= 2^score of the scaled vectors: P is held as its multiple of 2^(m + score - 15)
         const float rowf = p2(max(-126, min(mc - m - (S_::score - 15), 127)));
         const uint64_t rf = pair(rowf, rowf);
-        const float* pw = &pow_pad[32 + l];      // r^(i - j), zero for j > i: the mask
+        const float* pw = &item->pw[32 + l];      // r^(i - j), zero for j > i: the mask
         const float* col = col_s;
 #pragma unroll 1
-        for (int g = 0; g < 128; g += 32, pw -= 32, col += 32) {
+        for (int b = 0; b < 128; b += 32, pw -= 32, col += 32) {
           uint32_t s[32];                        // 16 columns of hi and 16 of lo, in the place of 32 scores
-          if (g <= tw * 32) {
+          if (b <= tw * 32) {
             uint32_t r[32];
-            tmem_ld32(sp + g, r);
+            tmem_ld32(sp + b, r);
             tmem_ld_wait();
 #pragma unroll
             for (int jj = 0; jj < 32; jj += 4) {
@@ -606,11 +640,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 #pragma unroll
             for (int x = 0; x < 32; ++x) s[x] = 0u;
           }
-          tmem_st32(sp + g, s);
+          tmem_st32(sp + b, s);
         }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(bar_p);
+      }
       }
     }
   } else if (role == 4) {
@@ -619,20 +654,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     const int l = th, e = l & 63, half = l >> 6;
     constexpr int NSt = 32 * KT;                 // state elements per thread: d = half * NSt ...
     float St[NSt];
-    {
-      const float* src = nullptr;
-      int64_t rs = 0, cs = 0;
-      if (seg == 0) {
-        if (w.s_in) { src = w.s_in + head * (int64_t)Dk * w.Dv; rs = w.s_row; cs = w.s_col; }
-      } else if (FULL) {
-        src = args.seg[wi] + ((int64_t)(seg - 1) * args.heads + head) * Dk * w.Dv; rs = w.Dv; cs = 1;
-      }
-#pragma unroll
-      for (int i = 0; i < NSt; ++i) {
-        const int d = half * NSt + i;
-        St[i] = (src && d < Dk && e < ne) ? src[d * rs + (int64_t)(e0 + e) * cs] : 0.f;
-      }
-    }
     // the state as the B operand [e][d] of the read-out, one exponent per row
     auto publish = [&](int slot) {
       float top = 0.f;
@@ -657,23 +678,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       fence_proxy_async();
     };
-    // Trip c writes the output of chunk c - 1, then takes the state over chunk c.  Trip -1 publishes what the
-    // walk starts from.
-#pragma unroll 1
-    for (int c = -1; c <= (FULL ? nc : nc - 1); ++c) {
-      if (FULL && c >= 1) {
-        const int p = c - 1;                     // the chunk whose output this is
-        const int64_t t = (c0 + p) * kL + l;
-        float* out = w.o + (head * (int64_t)w.Dv + e0) * T + (w.reverse ? T - 1 - t : t);
-        const bool live = t < T, plain = (c0 + p + 1) * kL <= T && ne == 64;
-        wait_phase(bar_o, (uint32_t)p & 1u, dead);
+    // The output of a chunk is written one chunk later, whichever item that belongs to: what it needs is kept.
+    int out_g = -1, out_n = 0, out_t0 = 0;
+    auto write_output = [&](bool last) {
+        const Item& item = items_s[out_n % kItems];
+        const int out_t = out_t0 + l;
+        wait_phase(bar_o, (uint32_t)out_g & 1u, dead);
         tc_fence_after();
-        const int qe = qe_s[p & 3][l], m = m_s[p & 3][l] + S_::score - 15;
+        const int qe = qe_s[out_g & 3][l], m = m_s[out_g & 3][l] + S_::score - 15;
         const bool bad = qe == 0x7fffffff;
         const Factors fi = p2_wide((bad ? 0 : qe) + m), fx = p2_wide(bad ? 0 : qe);
-        const float nan = __int_as_float(0x7fffffff), rowx = fx.b * pow_pad[32 + l + after];
+        const float nan = __int_as_float(0x7fffffff), rowx = fx.b * item.pw[32 + l + item.after];
         const uint64_t ia = pair(bad ? nan : fi.a, bad ? nan : fi.a), ib = pair(fi.b, fi.b), xa = pair(fx.a, fx.a),
                        xb = pair(rowx, rowx);
+        const int ne = item.ne;
+        const bool plain = out_t0 + kL <= T && ne == 64;
+        const int live = out_t < T ? ne : 0;
+        float* out = item.o + (item.reverse ? T - 1 - out_t : out_t);
 #pragma unroll 1
         for (int b = 0; b < 64; b += 16) {
           uint32_t ri[16], rx[16];
@@ -684,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             tc_fence_before();
             mbar_arrive(bar_ofree);
           }
-          const float* sc = &scale_s[p & 1][b];
+          const float* sc = &scale_s[out_g & 1][b];
           float y[16];
 #pragma unroll
           for (int x = 0; x < 16; x += 2) {
@@ -703,25 +724,47 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           } else {
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-              if (live && b + x < ne) *out = y[x];
+              if (b + x < live) *out = y[x];
               out += T;
             }
           }
         }
-        if (*any_poison != 0 && live) {          // spoilt columns
-          out -= 64 * T;
+        if (*(const volatile int*)&item.any_poison != 0 && live > 0) {          // spoilt columns
+          out -= (int64_t)64 * T;
           for (int x = 0; x < ne; ++x)
-            if (poison_s[x] <= (int)t) out[(int64_t)x * T] = nan;
+            if (item.poison[x] <= out_t) out[(int64_t)x * T] = nan;
         }
+        if (last) mbar_arrive(bar_itemfree + 8 * (out_n % kItems));
+    };
+    int g = 0;
+#pragma unroll 1
+    for (int n = 0;; ++n) {
+      const Item* const item = group_item(n, true);
+      if (!item) break;
+      {
+      const float* src = item->s_from;
+      const int64_t rs = item->from_row, cs = item->from_col;
+#pragma unroll
+      for (int i = 0; i < NSt; ++i) {
+        const int d = half * NSt + i;
+        St[i] = (src && d < item->Dk && e < item->ne) ? src[d * rs + (int64_t)e * cs] : 0.f;
       }
-      if (c == nc) break;
-      if (c >= 0) {
-        // the state after chunk c
-        const int len = (int)min((int64_t)kL, T - (c0 + c) * kL);
-        wait_phase(bar_ds, (uint32_t)c & 1u, dead);
+      }
+      if (FULL) {
+        // the published state is replaced once the MMAs of the chunk have read it
+        if (g >= 1) wait_phase(bar_qfree + 8 * ((g - 1) & 1), (uint32_t)((g - 1) >> 1) & 1u, dead);
+        publish(g & 1);
+        mbar_arrive(bar_s);
+      }
+      int t0 = item->t0;
+#pragma unroll 1
+      for (int left = item->nc; left > 0; --left, t0 += kL, ++g) {
+        if (FULL && out_g >= 0) write_output(out_n != n);
+        // the state after the chunk
+        wait_phase(bar_ds, (uint32_t)g & 1u, dead);
         tc_fence_after();
-        const Factors mw = p2_wide(mw_s[c & 3]);
-        const float carry = pow_pad[32 + len];
+        const Factors mw = p2_wide(mw_s[g & 3]);
+        const float carry = item->pw[32 + min(kL, T - t0)];
         const uint64_t ma = pair(mw.a, mw.a), mb = pair(mw.b, mw.b), cy = pair(carry, carry);
         // (rows 64-127 of the accumulator repeat rows 0-63)
 #pragma unroll
@@ -741,30 +784,31 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             St[b + x + 1] = v.y;
           }
         }
+        if (FULL) {
+          out_g = g;
+          out_n = n;
+          out_t0 = t0;
+          if (left > 1) {
+            wait_phase(bar_qfree + 8 * (g & 1), (uint32_t)(g >> 1) & 1u, dead);
+            publish((g + 1) & 1);
+            mbar_arrive(bar_s);
+          }
+        }
       }
-      if (FULL && c + 1 < nc) {
-        // the published state is replaced once the MMAs of the chunk have read it
-        if (c >= 0) wait_phase(bar_qfree + 8 * (c & 1), (uint32_t)(c >> 1) & 1u, dead);
-        publish((c + 1) & 1);
-        mbar_arrive(bar_s);
-      }
-    }
-    // the state after the last chunk
-    float* dst = nullptr;
-    int64_t rs = 0, cs = 0;
-    if (!FULL) {
-      dst = args.seg[wi] + ((int64_t)seg * args.heads + head) * Dk * w.Dv; rs = w.Dv; cs = 1;
-    } else if (seg == args.nseg - 1 && w.s_out) {
-      dst = w.s_out + head * (int64_t)Dk * w.Dv; rs = w.s_row; cs = w.s_col;
-    }
-    if (dst && e < ne) {
-      const bool bad = poison_s[e] != 0x7fffffff;
+      // the state after the last chunk
+      float* dst = item->s_to;
+      if (dst && e < item->ne) {
+        const int64_t rs = item->to_row, cs = item->to_col;
+        const bool bad = item->poison[e] != 0x7fffffff;
 #pragma unroll
-      for (int i = 0; i < NSt; ++i) {
-        const int d = half * NSt + i;
-        if (d < Dk) dst[d * rs + (int64_t)(e0 + e) * cs] = bad ? __int_as_float(0x7fffffff) : St[i];
+        for (int i = 0; i < NSt; ++i) {
+          const int d = half * NSt + i;
+          if (d < item->Dk) dst[d * rs + (int64_t)e * cs] = bad ? __int_as_float(0x7fffffff) : St[i];
+        }
       }
+      if (!FULL) mbar_arrive(bar_itemfree + 8 * (n % kItems));
     }
+    if (FULL && out_g >= 0) write_output(false);
   } else {
     regs_dec<Regs<KT>::mma>();
     if (th == 0) {
@@ -792,11 +836,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         umma_commit(bar_sp);
         mbar_arrive(bar_sp);
       };
-      if (FULL) scores(0);
+      const Item* item = item_at(0);
+      if (FULL && item) scores(0);
       // Growth first, it waits for nothing but the state's warps; then the state's part of the output, for
       // which the output before has to be taken away, the read-out, and the next chunk's scores.
+      int c = 0;
 #pragma unroll 1
-      for (int c = 0; c < nc && ok; ++c) {
+      for (int n = 0; item && ok; ++n) {
+      const int end = c + *(const volatile int*)&item->nc;
+#pragma unroll 1
+      for (; c < end && ok; ++c) {
+        if (c + 1 == end) item = item_at(n + 1);
         const uint32_t k_hi = base + (uint32_t)(c % NS) * S_::k_bytes,
                        v_hi = base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, vw_hi = base + S_::vw_at;
         if (!FULL) ok = wait_phase(bar_k + 8 * (c % NS), (uint32_t)(c / NS) & 1u, dead) && ok;
@@ -847,30 +897,38 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         umma_commit(bar_o);
         mbar_arrive(bar_o);
         umma_commit(bar_free + 8 * (c % NS));
-        if (c + 1 < nc) scores(c + 1);
+        if (item) scores(c + 1);
+      }
       }
       umma_commit(bar_end);          // everything issued has landed before tensor memory is given back
       if (!mbar_wait(bar_end, 0)) *dead = 1;
     } else if (th == 32 && boxes) {
       // ---------------- raw k and v, a TMA box for 64 channels ----------------
-      const CUtensorMap* maps = args.map[wi];
       int k_issued = 0, v_issued = 0;
 #pragma unroll 1
-      for (int c = 0; c < nc; ++c) {
-        const int64_t t = (c0 + c) * kL;
-        const int from = (int)(w.reverse ? T - t - kL : t);      // walking back, the last box may start before 0
-        const uint32_t bk = bar_kraw + 8 * (c % NS), bv = bar_vraw + 8 * (c % NS), again = (uint32_t)(c / NS - 1) & 1u;
-        if (c >= NS) wait_phase(bar_kfree + 8 * (c % NS), again, dead);
-        if (*dead) break;
-        mbar_expect_tx(bk, S_::k_bytes);
-        for (int h = 0; h < KT; ++h)
-          tma_load_box(base + (uint32_t)(c % NS) * S_::k_bytes + h * 2 * kTileB, &maps[1], from, 64 * h, (int)head, bk);
-        k_issued = c + 1;
-        if (c >= NS) wait_phase(bar_free + 8 * (c % NS), again, dead);
-        if (*dead) break;
-        mbar_expect_tx(bv, S_::v_bytes);
-        tma_load_box(base + S_::v_at + (uint32_t)(c % NS) * S_::v_bytes, &maps[2], from, e0, (int)head, bv);
-        v_issued = c + 1;
+      for (int n = 0; !*dead; ++n) {
+        const Item* const item = item_at(n);
+        if (!item) break;
+        const CUtensorMap* maps = args.map[item->wi];
+        const int head = item->head, e0 = item->e0;
+        int t = item->t0;
+#pragma unroll 1
+        for (int left = item->nc; left > 0; --left, t += kL) {
+          const int g = v_issued;
+          const int from = item->reverse ? T - t - kL : t;       // walking back, the last box may start before 0
+          const uint32_t bk = bar_kraw + 8 * (g % NS), bv = bar_vraw + 8 * (g % NS), again = (uint32_t)(g / NS - 1) & 1u;
+          if (g >= NS) wait_phase(bar_kfree + 8 * (g % NS), again, dead);
+          if (*dead) break;
+          mbar_expect_tx(bk, S_::k_bytes);
+          for (int h = 0; h < KT; ++h)
+            tma_load_box(base + (uint32_t)(g % NS) * S_::k_bytes + h * 2 * kTileB, &maps[1], from, 64 * h, head, bk);
+          k_issued = g + 1;
+          if (g >= NS) wait_phase(bar_free + 8 * (g % NS), again, dead);
+          if (*dead) break;
+          mbar_expect_tx(bv, S_::v_bytes);
+          tma_load_box(base + S_::v_at + (uint32_t)(g % NS) * S_::v_bytes, &maps[2], from, e0, head, bv);
+          v_issued = g + 1;
+        }
       }
       if (*dead) {   // nobody may have waited for the boxes in flight: not before they have landed
         for (int c = max(k_issued - NS, 0); c < k_issued; ++c) mbar_wait(bar_kraw + 8 * (c % NS), (uint32_t)(c / NS) & 1u);
@@ -881,15 +939,91 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       constexpr int per = KT == 1 ? 1 : 3;       // the halves in the order they are asked for: 0, 1, 0
       int n = 0;
 #pragma unroll 1
-      for (; n < per * nc; ++n) {
-        const int64_t t = (c0 + n / per) * kL;
-        if (n >= 1) wait_phase(bar_qread, (uint32_t)(n - 1) & 1u, dead);
-        if (*dead) break;
-        mbar_expect_tx(bar_qraw, 2 * kTileB);
-        tma_load_box(base + S_::q_at, &args.map[wi][0], (int)(w.reverse ? T - t - kL : t), n % per == 1 ? 64 : 0,
-                     (int)head, bar_qraw);
+      for (int i = 0; !*dead; ++i) {
+        const Item* const item = item_at(i);
+        if (!item) break;
+        const CUtensorMap* map = &args.map[item->wi][0];
+        const int head = item->head, reverse = item->reverse, steps = per * item->nc, t0 = item->t0;
+#pragma unroll 1
+        for (int x = 0; x < steps; ++x) {
+          const int t = t0 + x / per * kL;
+          if (n >= 1) wait_phase(bar_qread, (uint32_t)(n - 1) & 1u, dead);
+          if (*dead) break;
+          mbar_expect_tx(bar_qraw, 2 * kTileB);
+          tma_load_box(base + S_::q_at, map, reverse ? T - t - kL : t, x % per == 1 ? 64 : 0, head, bar_qraw);
+          ++n;
+        }
       }
       if (*dead && n > 0) mbar_wait(bar_qraw, (uint32_t)(n - 1) & 1u);
+    } else if (tw == 3) {
+      // ---------------- items, ahead of the others ----------------
+      uint32_t it = blockIdx.x;
+#pragma unroll 1
+      for (int n = 0;; ++n, it += gridDim.x) {
+        Item* const item = &items_s[n % kItems];
+        const uint32_t full = bar_item + 8 * (n % kItems);
+        if (n >= kItems) wait_phase(bar_itemfree + 8 * (n % kItems), (uint32_t)(n / kItems - 1) & 1u, dead);
+        if (__any_sync(0xffffffffu, *dead != 0)) break;          // the others may still be in the items that are there
+        if (it >= (uint32_t)args.items) {
+          if (lane == 0) {
+            *(volatile int*)&item->nc = 0;
+            mbar_arrive(full);
+          }
+          break;
+        }
+        const int sub = (int)(it % (uint32_t)args.nsub), wi = args.sub_walk[sub], e0 = args.sub_e0[sub];
+        const Walk& w = args.w[wi];
+        const uint32_t rest = it / (uint32_t)args.nsub;
+        const int64_t head = rest % (uint32_t)args.heads, state = head * (int64_t)w.Dk * w.Dv;
+        const int seg = (int)(rest / (uint32_t)args.heads);
+        item->poison[lane] = item->poison[32 + lane] = 0x7fffffff;
+        __syncwarp();
+        if (lane == 0) {
+          item->src[0] = w.k + head * (int64_t)w.Dk * T;
+          item->src[1] = w.v + (head * (int64_t)w.Dv + e0) * T;
+          item->src[2] = w.q + head * (int64_t)w.Dk * T;
+          if (FULL) item->o = w.o + (head * (int64_t)w.Dv + e0) * T;
+          const int64_t between = args.heads * (int64_t)w.Dk * w.Dv;       // of args.seg, rows of Dv
+          item->s_from = item->s_to = nullptr;
+          item->from_row = item->to_row = w.s_row;
+          item->from_col = item->to_col = w.s_col;
+          if (seg == 0) {
+            if (w.s_in) item->s_from = w.s_in + state + e0 * w.s_col;
+          } else if (FULL) {
+            item->s_from = args.seg[wi] + (seg - 1) * between + state + e0;
+            item->from_row = w.Dv;
+            item->from_col = 1;
+          }
+          if (!FULL) {
+            item->s_to = args.seg[wi] + seg * between + state + e0;
+            item->to_row = w.Dv;
+            item->to_col = 1;
+          } else if (seg == args.nseg - 1 && w.s_out) {
+            item->s_to = w.s_out + state + e0 * w.s_col;
+          }
+          item->nc = min(args.seg_chunks, (T + kL - 1) / kL - seg * args.seg_chunks);
+          item->t0 = seg * args.seg_chunks * kL;
+          item->head = (int)head;
+          item->e0 = e0;
+          item->ne = min(64, w.Dv - e0);
+          item->Dk = w.Dk;
+          item->wi = wi;
+          item->reverse = w.reverse;
+          item->after = w.after;
+          item->any_poison = 0;
+          mbar_arrive(full);
+        }
+        // r^n by squaring in 64 bits: r itself does not fit 32 (a slow head multiplies it a thousandfold)
+        const double r = 1.0 - (double)w.decay[w.n_decay > 1 ? head % w.n_decay : 0] / 4096.0;
+        double b = r, p = 1.0;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1, b *= b)
+          if (lane & m) p *= b;
+#pragma unroll
+        for (int i = 32; i <= 32 + kL; i += 32, p *= b)          // b: r^32
+          if (i + lane <= 32 + kL) item->pw[i + lane] = (float)p;
+        mbar_arrive(bar_powers + 8 * (n % kItems));
+      }
     }
     __syncwarp();
   }
@@ -928,9 +1062,12 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
 
 }  // namespace
 
-// Segments the axis is cut into: `ctas` CTAs per segment walk `chunks` chunks.  The fewest waves of
-// (segments x chunks) win; a cut axis is walked by the first launch too, at about half the cost of a
-// chunk, and every CTA pays about two chunks to fill and drain.
+// Segments the axis is cut into, each of them `ctas` items of one CTA.  In chunks: a CTA takes its share of
+// the items one after the other, each 0.8 longer than its chunks, and 1.6 to fill and drain; a cut axis is
+// walked by a first launch too, at half the cost of a chunk, and the join and the launches take 2, and a
+// twentieth for each segment.  Measured, us,
+// whole against cut in four: 16 heads of 128 channels and 8 chunks 69 and 53, 4 chunks 39 and 41; 35 heads of 64
+// and 8 chunks 47 and 41, 70 heads 47 and 63.
 int plan_segments(int64_t ctas, int64_t chunks) {
   const int64_t sms = sm_count();
   int best = 1;
@@ -938,8 +1075,8 @@ int plan_segments(int64_t ctas, int64_t chunks) {
   for (int64_t n = 1; n <= chunks && n <= 256; ++n) {
     const int64_t per = (chunks + n - 1) / n;
     if ((chunks + per - 1) / per != n) continue;       // the same cut as a smaller n
-    double cost = (double)((ctas * n + sms - 1) / sms) * (double)(per + 2);
-    if (n > 1) cost += (double)((ctas * (n - 1) + sms - 1) / sms) * (0.5 * (double)per + 2) + 4;
+    double cost = (double)((ctas * n + sms - 1) / sms) * ((double)per + 0.8) + 1.6;
+    if (n > 1) cost += (double)((ctas * (n - 1) + sms - 1) / sms) * (0.5 * (double)per + 0.8) + 3.6 + 0.05 * (double)n;
     if (n == 1 || cost < best_cost) { best = (int)n; best_cost = cost; }
     if (ctas * n > 16 * sms) break;
   }
@@ -963,7 +1100,9 @@ static int go(const TcArgs& a, cudaStream_t s) {
   SB_REQUIRE(ctas * a.nseg < (1LL << 31), "geometry too large");
   if (a.nseg > 1) {
     SB_CUDA(cudaFuncSetAttribute(attention_tc_kernel<KT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attention_tc_kernel<KT, false><<<(unsigned)(ctas * (a.nseg - 1)), kThreads, smem, s>>>(a);
+    TcArgs b = a;
+    b.items = ctas * (a.nseg - 1);
+    attention_tc_kernel<KT, false><<<(unsigned)(b.items < sm_count() ? b.items : sm_count()), kThreads, smem, s>>>(b);
     SB_CUDA(cudaGetLastError());
   }
   return SB_OK;
@@ -1022,7 +1161,8 @@ int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
     join_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(a, n);
     SB_CUDA(cudaGetLastError());
   }
-  const unsigned grid = (unsigned)(ctas * a.nseg);
+  a.items = ctas * a.nseg;
+  const unsigned grid = (unsigned)(a.items < sm_count() ? a.items : sm_count());
   if (wide) attention_tc_kernel<2, true><<<grid, kThreads, Shape<2>::smem, s>>>(a);
   else attention_tc_kernel<1, true><<<grid, kThreads, Shape<1>::smem, s>>>(a);
   SB_CUDA(cudaGetLastError());
