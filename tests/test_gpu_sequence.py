@@ -135,6 +135,53 @@ def test_attention_of_sizes_far_apart(cuda):
     check_walk(arrays, out, None, 300)
 
 
+MANY = [   # more heads than multiprocessors, several to each: n, h, dk, dv, T
+    (50, 16, 16, 20, 260), (41, 19, 24, 64, 131), (5, 80, 70, 128, 130), (31, 13, 64, 100, 129), (4, 13, 16, 12, 4224),
+    (90, 9, 8, 12, 128)]
+
+
+@pytest.mark.parametrize('shape', MANY)
+def test_attention_of_many_heads(cuda, shape):
+    """Heads that a multiprocessor takes one after the other: values, gradients, the same bits again."""
+    arrays, rng = make(17, *shape)
+    q, k, v, decay, s = arrays
+    leaves = [dev(a).requires_grad_() for a in (q, k, v, s)]
+    out, final = attention.dynamics(*leaves[:3], dev(decay), leaves[3], return_state=True)
+    check_walk(arrays, out.detach(), final.detach(), shape[-1])
+    go = rng.normal(size=v.shape).astype(np.float32)
+    gf = rng.normal(size=s.shape).astype(np.float32)
+    grads = torch.autograd.grad((out, final), leaves, (dev(go), dev(gf)), retain_graph=True)
+    want = O.attention_grads(q, k, v, decay, s, go, gf)
+    size = O.attention_grads(*(np.abs(a) for a in (q, k, v)), decay, np.abs(s), np.abs(go), np.abs(gf))
+    tol = O.attention_tol(max(shape[2:4]), shape[4], decay)
+    floor = O.attention_grads_floor(q, k, v, decay, s, go, gf)
+    for name, g, w, z, f in zip(('query', 'key', 'value', 'state'), grads, want, size, floor):
+        O.assert_sum_close(g, w, z, tol, name, f)
+    for a, b in zip(grads, torch.autograd.grad((out, final), leaves, (dev(go), dev(gf)))):
+        assert torch.equal(a, b)
+    assert _native.device_status() == 0
+
+
+@pytest.mark.parametrize('shape', [(50, 16, 16, 20, 260), (41, 19, 24, 64, 131), (5, 80, 70, 128, 130)])
+def test_attention_spoilt_heads_among_many(cuda, shape):
+    """What is not finite in some heads leaves every bit of the others as it was."""
+    arrays, rng = make(18, *shape)
+    with torch.no_grad():
+        want, ws = attention.dynamics(*(dev(a) for a in arrays), return_state=True)
+        heads = shape[0] * shape[1]
+        spoilt = np.zeros(heads, dtype=bool)
+        spoilt[rng.choice(heads, heads // 5, replace=False)] = True
+        spoilt = spoilt.reshape(shape[:2])
+        for i, a in enumerate(arrays[:3]):
+            at = np.argwhere(spoilt)[i::3]
+            a[at[:, 0], at[:, 1], 3, 100] = (np.nan, np.inf, -np.inf)[i]
+        got, gs = attention.dynamics(*(dev(a) for a in arrays), return_state=True)
+    keep = dev(~spoilt)
+    assert torch.equal(got[keep], want[keep]) and torch.equal(gs[keep], ws[keep])
+    assert torch.equal(got[..., :100], want[..., :100])
+    assert (~torch.isfinite(got[~keep][..., 100])).any(-1).all()
+
+
 @pytest.mark.parametrize('bad', [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize('which', [0, 1, 2])
 def test_attention_values_that_are_not_finite(cuda, which, bad):
