@@ -33,19 +33,22 @@
 // Roles of a CTA (one per SM, six warpgroups): k, v and q are each converted by a warpgroup (one step per
 // thread) out of raw tiles that TMA has landed, in place for k and v; one turns scores into P, one keeps the
 // state (32 elements per thread and 64 of Dk in registers, fp32) and writes the output; of the last, three
-// single threads issue the MMAs and the TMA loads.  Tensors that TMA cannot describe (T % 4 != 0, unaligned)
+// single threads issue the MMAs and the TMA loads and a warp works the items out.  Tensors that TMA cannot describe (T % 4 != 0, unaligned)
 // are loaded by the converting threads themselves.
 //
 // What bounds it is the instruction stream.  A chunk of 128 steps and 64 channels a side (131 KB, 3.0 us of
-// an SM's share of copy bandwidth; 0.65 us of MMA time at the bf16 rate) takes 6.5 us, 12,000 cycles, in which
-// a scheduler issues 4,500 instructions, mostly the splitting into fp16 pairs, at 0.38 per cycle with a
-// sixth of the fetches missing the instruction cache.  Steps on the way: one loading warpgroup with two
-// operands in registers 15.3 us, a warpgroup per operand 8.9, the same code for the three 7.7, TMA with
-// raw tiles 7.7, waits that hold the warp in hardware instead of polling 6.4.
+// an SM's share of copy bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 to 5.7 us on 148 SMs (18.2 for
+// 128 channels a side, both halves of v), in which a scheduler issues 4,250 instructions, mostly the splitting
+// into fp16 pairs, at 0.31 to 0.38 per cycle, its warps without a fetched instruction 3 cycles of 14.  Steps on
+// the way: one loading warpgroup with two operands in registers 15.3 us, a warpgroup per operand 8.9, the same
+// code for the three 7.7, TMA with raw tiles 7.7, waits that hold the warp in hardware instead of polling 6.4,
+// what describes a head in shared memory instead of registers 5.5.
 //
-// A head with T steps is one CTA, or several when there are fewer heads than SMs: the axis is then cut
-// into segments, a first launch takes each segment's growth from zero, a small one joins them, and the
-// walk starts every segment from its own state.
+// The grid is one CTA per SM, which takes its items (a head, one of the walks, 64 columns of v, a segment of the
+// axis) one after the other; the loaders are a chunk ahead across them, so short sequences do not fill and
+// drain for each head (1024 heads of 128 steps: 91 us with a CTA for each item, 67 so).  With fewer items than SMs
+// the axis is cut into segments: a first launch takes each segment's growth from zero, a small one joins them,
+// and the walk starts every segment from its own state.
 #include <string.h>
 
 #include "linear_attention.cuh"
@@ -1014,7 +1017,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           mbar_arrive(full);
         }
         // r^n by squaring in 64 bits: r itself does not fit 32 (a slow head multiplies it a thousandfold)
-        const double r = 1.0 - (double)w.decay[w.n_decay > 1 ? head % w.n_decay : 0] / 4096.0;
+        const double r = 1.0 - (double)w.decay[w.n_decay > 1 ? (w.head0 + head) % w.n_decay : 0] / 4096.0;
         double b = r, p = 1.0;
 #pragma unroll
         for (int m = 1; m < 32; m <<= 1, b *= b)
@@ -1043,7 +1046,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
     const int64_t per = (int64_t)w.Dk * w.Dv, total = per * args.heads;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
       const int64_t head = i / per;
-      double b = 1.0 - (double)w.decay[w.n_decay > 1 ? head % w.n_decay : 0] / 4096.0, p = 1.0;
+      double b = 1.0 - (double)w.decay[w.n_decay > 1 ? (w.head0 + head) % w.n_decay : 0] / 4096.0, p = 1.0;
       for (int64_t n = (int64_t)args.seg_chunks * kL; n; n >>= 1) {
         if (n & 1) p *= b;
         b *= b;
@@ -1068,27 +1071,43 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
 // twentieth for each segment.  Measured, us,
 // whole against cut in four: 16 heads of 128 channels and 8 chunks 69 and 53, 4 chunks 39 and 41; 35 heads of 64
 // and 8 chunks 47 and 41, 70 heads 47 and 63.
-int plan_segments(int64_t ctas, int64_t chunks) {
+struct Cut {
+  int nseg;
+  double cost;
+};
+static Cut plan_segments(int64_t ctas, int64_t chunks) {
   const int64_t sms = sm_count();
-  int best = 1;
-  double best_cost = 0;
+  Cut best{1, 0};
   for (int64_t n = 1; n <= chunks && n <= 256; ++n) {
     const int64_t per = (chunks + n - 1) / n;
     if ((chunks + per - 1) / per != n) continue;       // the same cut as a smaller n
     double cost = (double)((ctas * n + sms - 1) / sms) * ((double)per + 0.8) + 1.6;
     if (n > 1) cost += (double)((ctas * (n - 1) + sms - 1) / sms) * (0.5 * (double)per + 0.8) + 3.6 + 0.05 * (double)n;
-    if (n == 1 || cost < best_cost) { best = (int)n; best_cost = cost; }
+    if (n == 1 || cost < best.cost) best = Cut{(int)n, cost};
     if (ctas * n > 16 * sms) break;
   }
   return best;
 }
 
+// Heads that are walked whole by a launch of their own before the others, whose axis is cut, by the same costs:
+// as many as fill the SMs evenly.  Measured, us, together against apart (and the ratio of the costs): 180 heads of
+// 64 channels and 4096 steps 339 and 285 (0.79), 100 heads of 128 channels and 4096 steps 560 and 514 (0.97), the
+// training step of 32 heads of 128 channels and 4096 steps 808 and 733 (0.86), of 256 heads of 64 and 2000 steps
+// 716 and 716 (0.96).
+static int64_t whole_heads(int64_t heads, int64_t nsub, int64_t chunks) {
+  const int64_t rounds = heads * nsub / sm_count(), first = rounds * sm_count() / nsub;
+  if (rounds == 0 || first == heads) return 0;
+  const double apart = (double)rounds * ((double)chunks + 0.8) + 1.6 + plan_segments((heads - first) * nsub, chunks).cost;
+  return apart < 0.98 * plan_segments(heads * nsub, chunks).cost ? first : 0;
+}
+
 int64_t tc_scratch_floats(const Walk* walks, int n) {
-  int64_t ctas = 0, floats = 0;
-  for (int i = 0; i < n; ++i) ctas += walks[i].heads * ((walks[i].Dv + 63) / 64);
-  const int nseg = plan_segments(ctas, (walks[0].T + kL - 1) / kL);
+  int64_t nsub = 0, floats = 0;
+  for (int i = 0; i < n; ++i) nsub += (walks[i].Dv + 63) / 64;
+  const int64_t chunks = (walks[0].T + kL - 1) / kL, heads = walks[0].heads - whole_heads(walks[0].heads, nsub, chunks);
+  const int nseg = plan_segments(heads * nsub, chunks).nseg;
   if (nseg > 1)
-    for (int i = 0; i < n; ++i) floats += (int64_t)(nseg - 1) * walks[i].heads * walks[i].Dk * walks[i].Dv;
+    for (int i = 0; i < n; ++i) floats += (int64_t)(nseg - 1) * heads * walks[i].Dk * walks[i].Dv;
   return floats;
 }
 
@@ -1108,23 +1127,31 @@ static int go(const TcArgs& a, cudaStream_t s) {
   return SB_OK;
 }
 
-// Walks of one launch: the same heads and T, Dk on the same side of 64.
-int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
+// heads [from, from + heads) of the walks, their axis in nseg segments
+static int part(const Walk* walks, int n, int64_t from, int64_t heads, int nseg, float* scratch, cudaStream_t s) {
   TcArgs a;
   memset(&a, 0, sizeof(a));
-  int64_t ctas = 0;
   a.nsub = 0;
   for (int i = 0; i < n; ++i) {
-    a.w[i] = walks[i];
-    for (int e0 = 0; e0 < walks[i].Dv; e0 += 64) {
+    Walk& w = a.w[i];
+    w = walks[i];
+    const int64_t k = from * w.Dk * w.T, v = from * w.Dv * w.T, state = from * w.Dk * w.Dv;
+    w.heads = heads;
+    w.head0 += from;
+    w.q += k;
+    w.k += k;
+    w.v += v;
+    w.o += v;
+    if (w.s_in) w.s_in += state;
+    if (w.s_out) w.s_out += state;
+    for (int e0 = 0; e0 < w.Dv; e0 += 64) {
       a.sub_walk[a.nsub] = i;
       a.sub_e0[a.nsub++] = e0;
     }
   }
-  a.heads = walks[0].heads;
-  ctas = a.heads * a.nsub;
-  const int64_t chunks = (walks[0].T + kL - 1) / kL;
-  a.nseg = plan_segments(ctas, chunks);
+  a.heads = heads;
+  const int64_t ctas = a.heads * a.nsub, chunks = (walks[0].T + kL - 1) / kL;
+  a.nseg = nseg;
   a.seg_chunks = (int)((chunks + a.nseg - 1) / a.nseg);
   if (a.nseg > 1) {
     float* p = scratch;
@@ -1134,10 +1161,10 @@ int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
     }
   }
   uintptr_t bits = 0;
-  for (int i = 0; i < n; ++i) bits |= (uintptr_t)walks[i].q | (uintptr_t)walks[i].k | (uintptr_t)walks[i].v;
+  for (int i = 0; i < n; ++i) bits |= (uintptr_t)a.w[i].q | (uintptr_t)a.w[i].k | (uintptr_t)a.w[i].v;
   a.boxes = (bits & 15u) == 0 && walks[0].T % 4 == 0;
   for (int i = 0; i < n && a.boxes; ++i) {
-    const Walk& w = walks[i];
+    const Walk& w = a.w[i];
     const float* base[3] = {w.q, w.k, w.v};
     for (int x = 0; x < 3; ++x) {
       const uint64_t D = (uint64_t)(x == 2 ? w.Dv : w.Dk), row = (uint64_t)w.T * 4, all = row * D * (uint64_t)w.heads;
@@ -1167,6 +1194,15 @@ int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
   else attention_tc_kernel<1, true><<<grid, kThreads, Shape<1>::smem, s>>>(a);
   SB_CUDA(cudaGetLastError());
   return SB_OK;
+}
+
+// Walks of one launch: the same heads and T, Dk on the same side of 64.
+int tc_walks(const Walk* walks, int n, float* scratch, cudaStream_t s) {
+  int64_t nsub = 0;
+  for (int i = 0; i < n; ++i) nsub += (walks[i].Dv + 63) / 64;
+  const int64_t chunks = (walks[0].T + kL - 1) / kL, heads = walks[0].heads, first = whole_heads(heads, nsub, chunks);
+  if (first) SB_TRY(part(walks, n, 0, first, 1, nullptr, s));
+  return part(walks, n, first, heads - first, plan_segments((heads - first) * nsub, chunks).nseg, scratch, s);
 }
 
 }  // namespace la

@@ -25,6 +25,7 @@ struct Walk {
   int64_t s_row, s_col;
   int reverse;          // from the last step to the first
   int after;            // the state decays before a step is added (1) or after it has been read (0)
+  int64_t head0;        // the first head's place among all, for its decay
 };
 
 // Tensor-core walks (api_linear_attention_tc.cu): one launch for n <= 3 walks over the same heads and

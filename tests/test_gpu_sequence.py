@@ -137,7 +137,7 @@ def test_attention_of_sizes_far_apart(cuda):
 
 MANY = [   # more heads than multiprocessors, several to each: n, h, dk, dv, T
     (50, 16, 16, 20, 260), (41, 19, 24, 64, 131), (5, 80, 70, 128, 130), (31, 13, 64, 100, 129), (4, 13, 16, 12, 4224),
-    (90, 9, 8, 12, 128)]
+    (90, 9, 8, 12, 128), (15, 10, 8, 12, 2048), (5, 10, 16, 12, 2000)]
 
 
 @pytest.mark.parametrize('shape', MANY)
@@ -162,7 +162,8 @@ def test_attention_of_many_heads(cuda, shape):
     assert _native.device_status() == 0
 
 
-@pytest.mark.parametrize('shape', [(50, 16, 16, 20, 260), (41, 19, 24, 64, 131), (5, 80, 70, 128, 130)])
+@pytest.mark.parametrize('shape', [(50, 16, 16, 20, 260), (41, 19, 24, 64, 131), (5, 80, 70, 128, 130),
+                                   (15, 10, 8, 12, 2048)])
 def test_attention_spoilt_heads_among_many(cuda, shape):
     """What is not finite in some heads leaves every bit of the others as it was."""
     arrays, rng = make(18, *shape)
