@@ -33,8 +33,8 @@
 // Roles of a CTA (one per SM, six warpgroups): k, v and q are each converted by a warpgroup (one step per
 // thread) out of raw tiles that TMA has landed, in place for k and v; one turns scores into P, one keeps the
 // state (32 elements per thread and 64 of Dk in registers, fp32) and writes the output; of the last, three
-// single threads issue the MMAs and the TMA loads and a warp works the items out.  Tensors that TMA cannot describe (T % 4 != 0, unaligned)
-// are loaded by the converting threads themselves.
+// single threads issue the MMAs and the TMA loads and a warp works the items out.  Tensors that TMA cannot
+// describe (T % 4 != 0, unaligned) are loaded by the converting threads themselves.
 //
 // What bounds it is the instruction stream.  A chunk of 128 steps and 64 channels a side (131 KB, 3.0 us of
 // an SM's share of copy bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 to 5.7 us on 148 SMs (18.2 for
