@@ -66,10 +66,10 @@ constexpr int kL = 128;                      // steps per chunk
 constexpr int kTileB = kL * 128;             // bytes of a [128 steps][64 channels] fp16 tile
 constexpr int kThreads = 768;
 // Registers per thread of the six warpgroups: 80 at launch (65536 / 768, in steps of 8), moved to where
-// the vectors live.  Each row adds up to 6 * 80.
-template <int KT>
+// the vectors live.  The sum may not pass 6 * 80.  148 heads of 2048 steps, us: 99 (64 channels) and 270 (128);
+// with 88 for a loader, 104 for the state and 40 for the MMAs 108; with 88, 112 and 40 293 to 299.
 struct Regs {
-  static constexpr int load = KT == 1 ? 96 : 88, p = KT == 1 ? 72 : 64, s = KT == 1 ? 80 : 112, mma = 40;
+  static constexpr int load = 96, p = 64, s = 96, mma = 32;
   static_assert(3 * load + p + s + mma <= 480, "more registers than the block was launched with");
 };
 constexpr int kMaxSub = 6;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 
   if (role < 3) {
     // ---------------- k, v, q: load, convert, hand on ----------------
-    regs_inc<Regs<KT>::load>();
+    regs_inc<Regs::load>();
     const int j = th;
     const bool is_k = role == 0, is_v = role == 1, is_q = role == 2;
     // Passes over an operand.  Dk > 64 needs the largest magnitude of both halves before either is converted:
@@ -535,9 +535,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             for (int d = 0; d < 32; ++d) x[d] = 0;
           }
         }
-        // the weighted rows first where the growth waits for them (Dk > 64: 18.2 against 20.2 us per chunk of both
-        // halves of v; Dk <= 64: 6.9 against 6.5)
-        const bool weighted = is_v && (!FULL || pass == (KT == 2 ? 0 : 1));
+        // the weighted rows first, the growth waits for them (148 heads of 2048 steps: 99 against 101 us, with
+        // 128 channels 298 against 318)
+        const bool weighted = is_v && pass == 0;
         const float by = weighted ? scale_w : scale;
         const uint64_t sc = pair(by, by);
         if (is_q) {
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     }
   } else if (role == 3) {
     // ---------------- scores -> P: thread = row i ----------------
-    if constexpr (Regs<KT>::p < 80) regs_dec<Regs<KT>::p>();
+    regs_dec<Regs::p>();
     if constexpr (FULL) {
       const int l = th;
       int g = 0;
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     }
   } else if (role == 4) {
     // ---------------- state (thread = column e, half of Dk) and output (thread = step i) ----------------
-    if constexpr (Regs<KT>::s > 80) regs_inc<Regs<KT>::s>();
+    regs_inc<Regs::s>();
     const int l = th, e = l & 63, half = l >> 6;
     constexpr int NSt = 32 * KT;                 // state elements per thread: d = half * NSt ...
     float St[NSt];
@@ -813,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     }
     if (FULL && out_g >= 0) write_output(false);
   } else {
-    regs_dec<Regs<KT>::mma>();
+    regs_dec<Regs::mma>();
     if (th == 0) {
       // ---------------- MMAs ----------------
       constexpr uint32_t id_scores = idesc_f16(kL), id_inter = idesc_f16(64), id_intra = idesc_f16(64) | kBMajorMN,
