@@ -37,12 +37,13 @@
 // describe (T % 4 != 0, unaligned) are loaded by the converting threads themselves.
 //
 // What bounds it is the instruction stream.  A chunk of 128 steps and 64 channels a side (131 KB, 3.0 us of
-// an SM's share of copy bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 to 5.7 us on 148 SMs (18.2 for
+// an SM's share of copy bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 to 5.7 us on 148 SMs (15.7 for
 // 128 channels a side, both halves of v), in which a scheduler issues 4,250 instructions, mostly the splitting
 // into fp16 pairs, at 0.31 to 0.38 per cycle, its warps without a fetched instruction 3 cycles of 14.  Steps on
 // the way: one loading warpgroup with two operands in registers 15.3 us, a warpgroup per operand 8.9, the same
 // code for the three 7.7, TMA with raw tiles 7.7, waits that hold the warp in hardware instead of polling 6.4,
-// what describes a head in shared memory instead of registers 5.5.
+// what describes a head in shared memory instead of registers 5.5,
+// a register split with 96 for the state's warps too 5.3 (128 channels 18.2 before, 15.7 so).
 //
 // The grid is one CTA per SM, which takes its items (a head, one of the walks, 64 columns of v, a segment of the
 // axis) one after the other; the loaders are a chunk ahead across them, so short sequences do not fill and
@@ -1092,8 +1093,8 @@ static Cut plan_segments(int64_t ctas, int64_t chunks) {
 // Heads that are walked whole by a launch of their own before the others, whose axis is cut, by the same costs:
 // as many as fill the SMs evenly.  Measured, us, together against apart (and the ratio of the costs): 180 heads of
 // 64 channels and 4096 steps 339 and 285 (0.79), 100 heads of 128 channels and 4096 steps 560 and 514 (0.97), the
-// training step of 32 heads of 128 channels and 4096 steps 808 and 733 (0.86), of 256 heads of 64 and 2000 steps
-// 716 and 716 (0.96).
+// training step of 32 heads of 128 channels and 4096 steps 808 and 733 (0.86; 687 with today's registers), of 256
+// heads of 64 channels and 2000 steps 716 and 716 (0.96).
 static int64_t whole_heads(int64_t heads, int64_t nsub, int64_t chunks) {
   const int64_t rounds = heads * nsub / sm_count(), first = rounds * sm_count() / nsub;
   if (rounds == 0 || first == heads) return 0;
