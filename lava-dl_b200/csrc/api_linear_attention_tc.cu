@@ -332,11 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   // What travels beside the mantissas.  A slot of two is rewritten for chunk c + 2 once the read-out of
   // chunk c has ended, a slot of four once the output of chunk c + 1 has been written.
   __shared__ int f_s[2][kL];                                        // k's exponent
-  __shared__ int fg_s[2][kL];                                       // k's and v's exponents together
-  __shared__ __align__(16) float col_s[kL];                         // of a column of P: 2^(fg - largest fg)
+  __shared__ __align__(16) int fg_s[2][kL];                         // k's and v's exponents together
   __shared__ int m_s[4][kL], qe_s[4][kL], mw_s[4];
   __shared__ float scan_s[4];
-  __shared__ int fmax_s[4], kmax_s[2][4];
+  __shared__ int kmax_s[2][4];
   __shared__ Item items_s[kItems];
   __shared__ __align__(16) float scale_s[2][64];
   __shared__ float top_s[kL];
@@ -603,27 +602,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           const float up = __shfl_up_sync(0xffffffffu, mk, o);
           if (lane >= o) mk = fmaxf(mk, up);
         }
-        const int fmax = __reduce_max_sync(0xffffffffu, fg);
-        if (lane == 31) {
-          scan_s[tw] = mk;
-          fmax_s[tw] = fmax;
-        }
+        if (lane == 31) scan_s[tw] = mk;
         bar_sync(6, 128);
-        const int mc = max(max(fmax_s[0], fmax_s[1]), max(fmax_s[2], fmax_s[3]));
 #pragma unroll
         for (int i = 0; i < 3; ++i)
           if (i < tw) mk = fmaxf(mk, scan_s[i]);
         const int m = max(kNoTerm, (int)floorf(fmaxf(mk + (float)l * slope, (float)kNoTerm)) + 1);
         m_s[g & 3][l] = m;
-        col_s[l] = fg == kNoTerm ? 0.f : p2(max(fg - mc, -126));
-        bar_sync(6, 128);
+        bar_sync(6, 128);                        // (scan_s has been read)
         wait_phase(bar_sp, (uint32_t)g & 1u, dead);
         tc_fence_after();
-        // |q_i . k_j| <= 2^score of the scaled vectors: P is held as its multiple of 2^(m + score - 15)
-        const float rowf = p2(max(-126, min(mc - m - (S_::score - 15), 127)));
-        const uint64_t rf = pair(rowf, rowf);
+        // |q_i . k_j| <= 2^score of the scaled vectors: P is held as its multiple of 2^(m + score - 15).  The
+        // exponents of a column and a row meet as whole numbers: as two factors, each relative to a third number,
+        // both would have to be floats, and steps of a chunk lie further apart than a float's range.
+        const int row = m + (S_::score - 15);
         const float* pw = &item->pw[32 + l];      // r^(i - j), zero for j > i: the mask
-        const float* col = col_s;
+        const int* col = fg_s[g & 1];
+        auto scaled = [row](uint64_t x, int f0, int f1) {
+          return mul2(x, pair(p2(max(-126, min(f0 - row, 127))), p2(max(-126, min(f1 - row, 127)))));
+        };
 #pragma unroll 1
         for (int b = 0; b < 128; b += 32, pw -= 32, col += 32) {
           uint32_t s[32];                        // 16 columns of hi and 16 of lo, in the place of 32 scores
@@ -633,12 +630,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             tmem_ld_wait();
 #pragma unroll
             for (int jj = 0; jj < 32; jj += 4) {
-              const float4 cf = *reinterpret_cast<const float4*>(col + jj);
+              const int4 cf = *reinterpret_cast<const int4*>(col + jj);
               // the power first: its zeros take whatever the steps after i hold
               const uint64_t x = mul2(pair(__uint_as_float(r[jj]), __uint_as_float(r[jj + 1])), pair(pw[-jj], pw[-jj - 1]));
               const uint64_t y = mul2(pair(__uint_as_float(r[jj + 2]), __uint_as_float(r[jj + 3])), pair(pw[-jj - 2], pw[-jj - 3]));
-              split2(mul2(mul2(x, pair(cf.x, cf.y)), rf), &s[jj / 2], &s[16 + jj / 2]);
-              split2(mul2(mul2(y, pair(cf.z, cf.w)), rf), &s[jj / 2 + 1], &s[17 + jj / 2]);
+              split2(scaled(x, cf.x, cf.y), &s[jj / 2], &s[16 + jj / 2]);
+              split2(scaled(y, cf.z, cf.w), &s[jj / 2 + 1], &s[17 + jj / 2]);
             }
           } else {
 #pragma unroll

@@ -1,0 +1,145 @@
+"""Linear attention where the sizes of a sequence's steps lie far apart: every finite input whose states
+fit fp32 has to come out right, at the steps before a large one as well as at those behind it.
+
+Tolerance, per head, for an element against the sum of its own terms' magnitudes.  fp16 pairs keep an
+element to 2^-22, and what a product leaves out is 2^-22: a term passes two such products (scores and
+read-out, or growth and read-out), 6 * 2^-22 = 12 * 2^-23.  Additions of the tensor cores lose at most
+2^-23 each: width for a score or the state's read-out, 128 for the read-out of a chunk or the state's
+growth.  Powers of r and weights: eight roundings of 2^-24.  The state takes two roundings of 2^-24 a
+chunk, or a step where the walk goes step by step (fewer than 128 steps), and as many where segments are
+joined.  Together, with n = T / 128 chunks (steps below 128):  2^-23 (width + 128 + 16 + 2 n + 8).
+Unlike a bound for the slowest head this charges a head's memory once a chunk, and no sequence of less than
+2^12 steps gets more than 2^-15 of it, so an operand held in one fp16 (2^-12) does not pass.
+
+Floors: 2^-28 of the sums over the largest magnitudes of each step's vectors (``_sequence.py`` has the
+derivation), and what an fp32 state below the normal numbers loses, 2^-150 for each of its updates times
+the query's magnitudes.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import _sequence as O
+import lava_dl_b200.slayer as slayer
+from lava_dl_b200 import _native
+
+pytestmark = pytest.mark.gpu
+attention = slayer.neuron.dynamics.linear_attention
+
+
+def dev(a):
+    return None if a is None else torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def head_tol(width, T):
+    updates = 2 * (T // 128 + 1) if T >= 128 else T
+    return 2.0 ** -23 * (width + 128 + 16 + updates + 8)
+
+
+def state_floor(reader, T):
+    """What the states' subnormal roundings can add to an output read by `reader` [n, h, d, T]."""
+    return 2.0 ** -150 * (T + 1) * np.abs(reader.astype(np.float64)).sum(axis=2, keepdims=True)
+
+
+def exponents(kind, rng, shape, span):
+    """One exponent for every step, -span .. span (the step's key times value: twice that)."""
+    T = shape[-1]
+    if kind == 'rising':          # tiny steps, then large ones from the middle of a chunk on
+        e = np.where(np.arange(T) % 128 < 64, -span, span) + np.zeros(shape)
+    elif kind == 'falling':
+        e = np.where(np.arange(T) % 128 < 64, span, -span) + np.zeros(shape)
+    elif kind == 'fading':        # a signal that vanishes over the whole axis
+        e = np.linspace(span, -span, T) + np.zeros(shape)
+    elif kind == 'growing':
+        e = np.linspace(-span, span, T) + np.zeros(shape)
+    elif kind == 'last':          # one large step at the end of a chunk
+        e = np.where(np.arange(T) % 128 == 127, span, -span) + np.zeros(shape)
+    else:
+        e = rng.integers(-span, span + 1, size=shape).astype(float)
+    return np.rint(e)
+
+
+def far_apart(seed, n, h, dk, dv, T, kind, span, decay, back=False):
+    """Key and value (or, for the walks back in time, query and output gradient) spread by 2^span each way; the
+    readers' exponents bring the outputs (or gradients of key and value) back to where fp32 holds them."""
+    rng = np.random.default_rng(seed)
+    q, k, v, go = (rng.normal(size=(n, h, d, T)) for d in (dk, dk, dv, dv))
+    e = exponents(kind, rng, (n, h, 1, T), span)
+    r = 1.0 - np.asarray(decay, dtype=np.float64).reshape(1, -1, 1) / 4096.0
+    with np.errstate(divide='ignore'):
+        log_r = np.maximum(np.log2(r), -1e4)
+    size = np.full((n, h, 1), -1e9)
+    reach = np.empty((n, h, 1, T))
+    for t in (reversed(range(T)) if back else range(T)):      # the exponent of the state's largest part
+        size = np.maximum(size + log_r, 2 * e[..., t])
+        reach[..., t] = size
+    reach = np.clip(np.rint(reach), -110, 110)
+    read = np.exp2(-reach)
+    part = np.exp2(e)
+    if back:
+        q, go, k, v = q * part, go * part, k * read, v * read
+    else:
+        k, v, q, go = k * part, v * part, q * read, go * read
+    return [a.astype(np.float32) for a in (q, k, v, go)], np.asarray(decay, dtype=np.float32)
+
+
+def check_forward(q, k, v, decay):
+    T = q.shape[-1]
+    with torch.no_grad():
+        out, final = attention.dynamics(dev(q), dev(k), dev(v), dev(decay), return_state=True)
+    want, ws = O.attention(q, k, v, decay)
+    size, ss = O.attention(np.abs(q), np.abs(k), np.abs(v), decay)
+    floor, fs = O.attention_floor(q, k, v, decay)
+    tol = head_tol(q.shape[2], T)
+    O.assert_sum_close(out, want, size, tol, 'output', floor + state_floor(q, T))
+    O.assert_sum_close(final, ws, ss, tol, 'state', fs)
+    assert _native.device_status() == 0
+
+
+def check_backward(q, k, v, go, decay, which):
+    """`which`: the gradients whose states fit fp32."""
+    T = q.shape[-1]
+    leaves = [dev(a).requires_grad_() for a in (q, k, v)]
+    grads = torch.autograd.grad(attention.dynamics(*leaves, dev(decay)), leaves, dev(go))
+    want = O.attention_grads(q, k, v, decay, None, go, None)
+    size = O.attention_grads(np.abs(q), np.abs(k), np.abs(v), decay, None, np.abs(go), None)
+    floor = O.attention_grads_floor(q, k, v, decay, None, go, None)
+    tol = head_tol(max(q.shape[2], v.shape[2]), T)
+    for i in which:
+        name, reader = (('query', go), ('key', v), ('value', k))[i]
+        O.assert_sum_close(grads[i], want[i], size[i], tol, name, floor[i] + state_floor(reader, T))
+    assert _native.device_status() == 0
+
+
+SLOW = [2.048, 40.96, 409.6]             # memories of 2000, 100 and 10 steps
+KINDS = ['rising', 'falling', 'fading', 'growing', 'last', 'random']
+WIDTHS = [(64, 64, 300), (40, 72, 277), (128, 96, 260), (16, 16, 128), (64, 64, 1284)]
+
+
+@pytest.mark.parametrize('span', [20, 33, 56])
+@pytest.mark.parametrize('kind', KINDS)
+@pytest.mark.parametrize('dk, dv, T', WIDTHS)
+def test_forward_of_steps_far_apart(cuda, dk, dv, T, kind, span):
+    (q, k, v, _), decay = far_apart(21, 2, 3, dk, dv, T, kind, span, SLOW)
+    check_forward(q, k, v, decay)
+
+
+@pytest.mark.parametrize('span', [33, 56])
+@pytest.mark.parametrize('kind', KINDS)
+@pytest.mark.parametrize('dk, dv, T', WIDTHS)
+def test_backward_of_steps_far_apart(cuda, dk, dv, T, kind, span):
+    for back in (False, True):
+        (q, k, v, go), decay = far_apart(22, 2, 3, dk, dv, T, kind, span, SLOW, back)
+        check_backward(q, k, v, go, decay, (1, 2) if back else (0,))
+
+
+@pytest.mark.parametrize('tiny', [1e-18, 2.0 ** -64, 2.0 ** -65, 1e-20, 1e-22])
+@pytest.mark.parametrize('query', [1.0, 1e10])
+@pytest.mark.parametrize('dk, dv', [(64, 64), (128, 64)])
+def test_tiny_steps_before_a_large_one(cuda, dk, dv, query, tiny):
+    """A later step of ordinary size leaves the outputs before it as they are."""
+    shape = (1, 1, dk, 256)
+    q, k, v = np.full(shape, query, np.float32), np.full(shape, tiny, np.float32), np.full((1, 1, dv, 256), tiny, np.float32)
+    k[..., 64:128] = v[..., 64:128] = 1.0
+    check_forward(q, k, v, np.array([2.048], np.float32))
