@@ -688,10 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         tc_fence_after();
         const int qe = qe_s[out_g & 3][l], m = m_s[out_g & 3][l] + S_::score - 15;
         const bool bad = qe == 0x7fffffff;
-        const Factors fi = p2_wide((bad ? 0 : qe) + m), fx = p2_wide(bad ? 0 : qe);
-        const float nan = __int_as_float(0x7fffffff), rowx = fx.b * item.pw[32 + l + item.after];
-        const uint64_t ia = pair(bad ? nan : fi.a, bad ? nan : fi.a), ib = pair(fi.b, fi.b), xa = pair(fx.a, fx.a),
-                       xb = pair(rowx, rowx);
+        const Factors fi = p2_wide((bad ? 0 : qe) + m);
+        // the state's part: times the row's exponent before the column's where that takes it down and after it
+        // where that takes it up, so that nothing leaves a float's range that comes back into it
+        const int rx_e = bad ? 0 : qe, first = min(rx_e, 0);
+        const float nan = __int_as_float(0x7fffffff), rowa = p2(first) * item.pw[32 + l + item.after], rowb = p2(rx_e - first);
+        const uint64_t ia = pair(bad ? nan : fi.a, bad ? nan : fi.a), ib = pair(fi.b, fi.b), xa = pair(rowa, rowa),
+                       xb = pair(rowb, rowb);
         const int ne = item.ne;
         const bool plain = out_t0 + kL <= T && ne == 64;
         const int live = out_t < T ? ne : 0;
@@ -710,8 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           float y[16];
 #pragma unroll
           for (int x = 0; x < 16; x += 2) {
-            const uint64_t inter = mul2(mul2(pair(__uint_as_float(rx[x]), __uint_as_float(rx[x + 1])), xa),
-                                        mul2(pair(sc[x], sc[x + 1]), xb));
+            const uint64_t inter = mul2(mul2(mul2(pair(__uint_as_float(rx[x]), __uint_as_float(rx[x + 1])), xa),
+                                             pair(sc[x], sc[x + 1])), xb);
             const float2 v = unpair(fma2(mul2(pair(__uint_as_float(ri[x]), __uint_as_float(ri[x + 1])), ia), ib, inter));
             y[x] = v.x;
             y[x + 1] = v.y;

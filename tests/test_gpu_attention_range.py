@@ -134,6 +134,17 @@ def test_backward_of_steps_far_apart(cuda, dk, dv, T, kind, span):
         check_backward(q, k, v, go, decay, (1, 2) if back else (0,))
 
 
+@pytest.mark.parametrize('dk', [64, 128])
+def test_zero_read_out_of_a_large_state(cuda, dk):
+    """A query that meets nothing of a state of the largest numbers reads zero, at any size of its own."""
+    q, s = np.zeros((1, 1, dk, 256), np.float32), np.zeros((1, 1, dk, 64), np.float32)
+    q[:, :, 0], s[:, :, 1] = 3e38, 3e38
+    zero = np.zeros_like(q)
+    with torch.no_grad():
+        out = attention.dynamics(dev(q), dev(zero), dev(zero[:, :, :64]), dev(np.array([2.048], np.float32)), dev(s))
+    assert torch.equal(out, torch.zeros_like(out))
+
+
 @pytest.mark.parametrize('tiny', [1e-18, 2.0 ** -64, 2.0 ** -65, 1e-20, 1e-22])
 @pytest.mark.parametrize('query', [1.0, 1e10])
 @pytest.mark.parametrize('dk, dv', [(64, 64), (128, 64)])
