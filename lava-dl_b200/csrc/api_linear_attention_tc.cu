@@ -138,6 +138,7 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool x) {
   return any != 0;
 }
 
+__device__ __forceinline__ bool not_finite(float top) { return __float_as_uint(top) >= 0x7f800000u; }
 __device__ __forceinline__ float p2(int n) { return __int_as_float((n + 127) << 23); }   // -126 <= n <= 127
 struct Factors {
   float a, b;
@@ -146,6 +147,24 @@ struct Factors {
 __device__ __forceinline__ Factors p2_wide(int n) {
   n = max(-252, min(n, 254));
   return Factors{p2(n >> 1), p2(n - (n >> 1))};
+}
+// the same for n from -149 on, and zero below
+__device__ __forceinline__ float p2_low(int n) {
+  return n >= -126 ? p2(n) : __int_as_float(n >= -149 ? 1 << (n + 149) : 0);
+}
+// Powers of r leave a float's range within a chunk (r = 0.1 after 38 steps), while the states they apply to have
+// 2^254 to lose.  So r = c 2^-kappa with c next to 1, and r^n = c^n 2^(-kappa n): c^n stays within 2^-64 .. 2^64
+// and kappa n joins the other exponents.  A power as mantissa and exponent:
+struct Power {
+  float m;      // 1 to 2, signed
+  int e;
+};
+constexpr int kNoPower = -100000;   // exponent of zero
+__device__ __forceinline__ Power power(float c, int down) {
+  const uint32_t b = __float_as_uint(c);
+  if ((b & 0x7fffffffu) == 0) return Power{0.f, kNoPower};
+  if (not_finite(fabsf(c))) return Power{c, -down};
+  return Power{__uint_as_float((b & 0x807fffffu) | 0x3f800000u), (int)((b >> 23) & 0xff) - 127 - down};
 }
 // largest magnitude of three, NaN if one is NaN
 __device__ __forceinline__ float max_abs3(float a, float b, float c) {
@@ -296,7 +315,6 @@ __device__ __forceinline__ int fit_exponent(float top) {
   const int e = (int)(__float_as_uint(top) >> 23) - 127;
   return max(e, -113) - 13;
 }
-__device__ __forceinline__ bool not_finite(float top) { return __float_as_uint(top) >= 0x7f800000u; }
 template <int R>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
@@ -319,7 +337,8 @@ struct Item {
   int wi, reverse, after;
   int any_poison;
   int poison[64];            // first spoilt step of each column
-  float pw[32 + kL + 1];     // r^n at 32 + n; zeros before it are the causal mask
+  int kappa;
+  float pw[32 + kL + 1];     // c^n = r^n 2^(kappa n) at 32 + n; zeros before it are the causal mask
 };
 constexpr int kItems = 4;    // in the works
 
@@ -332,7 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   // What travels beside the mantissas.  A slot of two is rewritten for chunk c + 2 once the read-out of
   // chunk c has ended, a slot of four once the output of chunk c + 1 has been written.
   __shared__ int f_s[2][kL];                                        // k's exponent
-  __shared__ __align__(16) int fg_s[2][kL];                         // k's and v's exponents together
+  __shared__ int fg_s[2][kL];                                       // k's and v's exponents together
+  __shared__ __align__(16) int col_s[kL];                           // of a column of P
   __shared__ int m_s[4][kL], qe_s[4][kL], mw_s[4];
   __shared__ float scan_s[4];
   __shared__ int kmax_s[2][4];
@@ -512,9 +532,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             const int vg = fit_exponent(top);
             const int fg = (top > 0.f && f > kNoTerm) ? f + vg : kNoTerm;
             // weight of the step in the state, and the largest exponent of the weighted steps
-            const float wt = t < T ? item->pw[32 + min(kL, T - t0) - item->after - j] : 0.f;
-            const int we = (int)((__float_as_uint(wt) >> 23) & 0xff) - 127;
-            const int key = wt != 0.f && fg != kNoTerm ? fg + we : kNoTerm;
+            const int lag = min(kL, T - t0) - item->after - j;
+            const Power wt = power(t < T ? item->pw[32 + lag] : 0.f, item->kappa * lag);
+            const int key = wt.e != kNoPower && fg != kNoTerm ? fg + wt.e : kNoTerm;
             const int kmax = __reduce_max_sync(0xffffffffu, key);
             if (lane == 0) kmax_s[g & 1][tw] = kmax;
             bar_sync(1, 128);
@@ -523,9 +543,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             if (FULL) fg_s[g & 1][j] = fg;
             if (j == 0) mw_s[g & 3] = mw;
             scale = p2(-vg);
-            // 2^-g r^(..) 2^(fg - mw): the two powers of two together, the weight's mantissa first.  What this
-            // takes below a float's range is nothing in fp16 either.
-            scale_w = key != kNoTerm ? (wt * p2(max(-we, -126))) * p2(max(fg + we - mw, -100)) * scale : 0.f;
+            // 2^-g r^(..) 2^(fg - mw): the powers of two together.  What this takes below a float's range is
+            // nothing in fp16 either.
+            scale_w = key != kNoTerm ? wt.m * p2(max(key - mw, -100)) * scale : 0.f;
           }
         }
         if (pass < mid) continue;
@@ -588,8 +608,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       for (int n = 0;; ++n) {
       const Item* const item = group_item(n, true);
       if (!item) break;
-      // log2 r, for exponents only; a head that forgets everything at once gets a steep slope
-      const float slope = fminf(fmaxf(log2f(fabsf(item->pw[33])), -250.f), 250.f);
+      const int kappa = item->kappa;
+      // log2 r, for exponents only; a head that forgets everything at once gets a slope that is steeper than any
+      // two steps lie apart
+      const float slope = fminf(fmaxf(log2f(fabsf(item->pw[33])) - (float)kappa, -1000.f), 250.f);
 #pragma unroll 1
       for (int left = item->nc; left > 0; --left, ++g) {
         const uint32_t sp = trow + S_::sp;
@@ -609,17 +631,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           if (i < tw) mk = fmaxf(mk, scan_s[i]);
         const int m = max(kNoTerm, (int)floorf(fmaxf(mk + (float)l * slope, (float)kNoTerm)) + 1);
         m_s[g & 3][l] = m;
-        bar_sync(6, 128);                        // (scan_s has been read)
+        col_s[l] = fg + kappa * l;
+        bar_sync(6, 128);
         wait_phase(bar_sp, (uint32_t)g & 1u, dead);
         tc_fence_after();
         // |q_i . k_j| <= 2^score of the scaled vectors: P is held as its multiple of 2^(m + score - 15).  The
         // exponents of a column and a row meet as whole numbers: as two factors, each relative to a third number,
-        // both would have to be floats, and steps of a chunk lie further apart than a float's range.
-        const int row = m + (S_::score - 15);
-        const float* pw = &item->pw[32 + l];      // r^(i - j), zero for j > i: the mask
-        const int* col = fg_s[g & 1];
-        auto scaled = [row](uint64_t x, int f0, int f1) {
-          return mul2(x, pair(p2(max(-126, min(f0 - row, 127))), p2(max(-126, min(f1 - row, 127)))));
+        // both would have to be floats, and steps of a chunk lie further apart than a float's range.  By the choice
+        // of m and with c^n above 2^-64 their difference is below 64; what lies 127 below one is nothing in fp16.
+        const int above = 127 - (m + (S_::score - 15) + kappa * l);
+        const float* pw = &item->pw[32 + l];      // c^(i - j), zero for j > i: the mask
+        const int* col = col_s;
+        auto scaled = [above](uint64_t x, int f0, int f1) {
+          return mul2(x, pair(__int_as_float(__viaddmin_s32_relu(f0, above, 254) << 23),
+                              __int_as_float(__viaddmin_s32_relu(f1, above, 254) << 23)));
         };
 #pragma unroll 1
         for (int b = 0; b < 128; b += 32, pw -= 32, col += 32) {
@@ -689,10 +714,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const int qe = qe_s[out_g & 3][l], m = m_s[out_g & 3][l] + S_::score - 15;
         const bool bad = qe == 0x7fffffff;
         const Factors fi = p2_wide((bad ? 0 : qe) + m);
-        // the state's part: times the row's exponent before the column's where that takes it down and after it
-        // where that takes it up, so that nothing leaves a float's range that comes back into it
-        const int rx_e = bad ? 0 : qe, first = min(rx_e, 0);
-        const float nan = __int_as_float(0x7fffffff), rowa = p2(first) * item.pw[32 + l + item.after], rowb = p2(rx_e - first);
+        // the state's part: times the row's exponent and power before the column's exponent where that takes it
+        // down and after it where that takes it up, so that nothing leaves a float's range that comes back into it
+        const int lag = l + item.after;
+        const Power rp = power(item.pw[32 + lag], item.kappa * lag);
+        const int rx_e = (bad ? 0 : qe) + rp.e, first = max(min(rx_e, 0), -126);
+        const float nan = __int_as_float(0x7fffffff), rowa = rp.m * p2(first), rowb = p2_low(min(rx_e - first, 127));
         const uint64_t ia = pair(bad ? nan : fi.a, bad ? nan : fi.a), ib = pair(fi.b, fi.b), xa = pair(rowa, rowa),
                        xb = pair(rowb, rowb);
         const int ne = item.ne;
@@ -768,8 +795,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         wait_phase(bar_ds, (uint32_t)g & 1u, dead);
         tc_fence_after();
         const Factors mw = p2_wide(mw_s[g & 3]);
-        const float carry = item->pw[32 + min(kL, T - t0)];
-        const uint64_t ma = pair(mw.a, mw.a), mb = pair(mw.b, mw.b), cy = pair(carry, carry);
+        const int steps = min(kL, T - t0);
+        const Power carry = power(item->pw[32 + steps], item->kappa * steps);
+        const float carried = carry.m * p2(max(-126, min(carry.e, 126)));
+        const uint64_t ma = pair(mw.a, mw.a), mb = pair(mw.b, mw.b), cy = pair(carried, carried);
+        if (carry.e < -126) {                    // what of the power is below a float
+          const float rest = p2_low(carry.e + 126);
+#pragma unroll
+          for (int i = 0; i < NSt; ++i) St[i] *= rest;
+        }
         // (rows 64-127 of the accumulator repeat rows 0-63)
 #pragma unroll
         for (int b = 0; b < NSt; b += 32) {
@@ -1017,14 +1051,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           item->any_poison = 0;
           mbar_arrive(full);
         }
-        // r^n by squaring in 64 bits: r itself does not fit 32 (a slow head multiplies it a thousandfold)
+        // c^n by squaring in 64 bits: r itself does not fit 32 (a slow head multiplies it a thousandfold)
         const double r = 1.0 - (double)w.decay[w.n_decay > 1 ? (w.head0 + head) % w.n_decay : 0] / 4096.0;
-        double b = r, p = 1.0;
+        const int kappa = r != 0.0 ? max(-128, min(__float2int_rn(-log2f(fabsf((float)r))), 128)) : 0;
+        double b = r * __hiloint2double((1023 + kappa) << 20, 0), p = 1.0;
 #pragma unroll
         for (int m = 1; m < 32; m <<= 1, b *= b)
           if (lane & m) p *= b;
+        if (lane == 0) item->kappa = kappa;
 #pragma unroll
-        for (int i = 32; i <= 32 + kL; i += 32, p *= b)          // b: r^32
+        for (int i = 32; i <= 32 + kL; i += 32, p *= b)          // b: c^32
           if (i + lane <= 32 + kL) item->pw[i + lane] = (float)p;
         mbar_arrive(bar_powers + 8 * (n % kItems));
       }
@@ -1052,12 +1088,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
         if (n & 1) p *= b;
         b *= b;
       }
-      const float r = (float)p;
       float* s = args.seg[wi] + i;
       float x = *s;
       for (int g = 1; g < args.nseg - 1; ++g) {
         s += total;
-        x = fmaf(r, x, *s);
+        x = (float)fma(p, (double)x, (double)*s);     // the power may be less than any float
         *s = x;
       }
     }

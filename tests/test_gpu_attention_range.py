@@ -134,6 +134,53 @@ def test_backward_of_steps_far_apart(cuda, dk, dv, T, kind, span):
         check_backward(q, k, v, go, decay, (1, 2) if back else (0,))
 
 
+FAST = [2048.0, 3300.0, 4055.0, 4095.9, 4096.0]      # r of 0.5, 0.19, 0.01, 2^-15.3 and 0
+
+
+@pytest.mark.parametrize('span', [33, 56])
+@pytest.mark.parametrize('kind', KINDS)
+@pytest.mark.parametrize('dk, dv, T', [(64, 64, 300), (40, 72, 277), (128, 96, 260)])
+def test_heads_of_short_memory(cuda, dk, dv, T, kind, span):
+    """Powers of r below any float: what decays by them was large enough to be seen all the same."""
+    (q, k, v, _), decay = far_apart(23, 1, 5, dk, dv, T, kind, span, FAST)
+    check_forward(q, k, v, decay)
+    for back in (False, True):
+        (q, k, v, go), decay = far_apart(24, 1, 5, dk, dv, T, kind, span, FAST, back)
+        check_backward(q, k, v, go, decay, (1, 2) if back else (0,))
+
+
+@pytest.mark.parametrize('dk, dv, T', [(64, 64, 300), (64, 40, 301), (128, 128, 260), (8, 8, 4096)])
+def test_large_states_that_fade(cuda, dk, dv, T):
+    """Nothing but a state from before, down to where fp32 ends; in the longest, cut into segments."""
+    rng = np.random.default_rng(25)
+    decay = np.array([2048.0, 1500.0, 3300.0, 300.0], np.float32)
+    r = 1.0 - decay.astype(np.float64).reshape(1, 4, 1, 1) / 4096.0
+    s = (rng.normal(size=(1, 4, dk, dv)) * 2.0 ** 120).astype(np.float32)
+    gone = 120 + np.log2(r) * np.arange(1, T + 1)                   # exponent of the state
+    q = (rng.normal(size=(1, 4, dk, T)) * np.exp2(-np.clip(gone, -110, 120))).astype(np.float32)
+    zero_k, zero_v = np.zeros((1, 4, dk, T), np.float32), np.zeros((1, 4, dv, T), np.float32)
+    with torch.no_grad():
+        out, final = attention.dynamics(*(dev(a) for a in (q, zero_k, zero_v, decay, s)), return_state=True)
+    want, ws = O.attention(q, zero_k, zero_v, decay, s)
+    size, ss = O.attention(np.abs(q), zero_k, zero_v, decay, np.abs(s))
+    floor, _ = O.attention_floor(q, zero_k, zero_v, decay, s)
+    assert (np.abs(want[:, :, :, 100]) > 1e-3).any()                # well inside fp32
+    O.assert_sum_close(out, want, size, head_tol(dk, T), 'output', floor + state_floor(q, T))
+    O.assert_sum_close(final, ws, ss, head_tol(dk, T), 'state')
+
+
+def test_decay_that_is_not_a_number(cuda):
+    """Nothing finite comes out of it, whichever kernel takes the length; other heads do not notice."""
+    for T in (20, 300):
+        (q, k, v, _), decay = far_apart(26, 2, 3, 16, 24, T, 'random', 3, SLOW)
+        with torch.no_grad():
+            want = attention.dynamics(dev(q), dev(k), dev(v), dev(decay))
+            decay[1] = np.nan
+            got = attention.dynamics(dev(q), dev(k), dev(v), dev(decay))
+        assert torch.isnan(got[:, 1]).all()
+        assert torch.equal(got[:, ::2], want[:, ::2])
+
+
 @pytest.mark.parametrize('dk', [64, 128])
 def test_zero_read_out_of_a_large_state(cuda, dk):
     """A query that meets nothing of a state of the largest numbers reads zero, at any size of its own."""
