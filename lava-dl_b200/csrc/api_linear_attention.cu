@@ -19,13 +19,21 @@ using namespace sb::la;
 
 namespace {
 
+// r is applied as the sum of two floats: over the thousand steps a slow head remembers, half an ulp of
+// r would grow a thousandfold.  decay / 4096 is exact, and so is what 1 - decay / 4096 loses to rounding.
+struct Keep {
+  float r, lo;
+};
+__device__ __forceinline__ Keep keep_of(float decay) {
+  const float delta = decay * (1.0f / 4096.0f), r = __fsub_rn(1.0f, delta);
+  return Keep{r, __fsub_rn(__fsub_rn(1.0f, r), delta)};
+}
+
 // ---------------------------------------------------------------------------
 // Walk step by step: any size, any length.
 // A block of 128 threads owns one head and 64 columns of its state; a thread holds NI x 4 elements of
 // it (rows dg + 8 i, four neighbouring columns).  The row sums of a tile of steps are joined through
 // shared memory at the end of the tile.
-// r is applied as the sum of two floats: over the thousand steps a slow head remembers, half an ulp of
-// r would grow a thousandfold.  decay / 4096 is exact, and so is what 1 - decay / 4096 loses to rounding.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 8;
 
@@ -47,8 +55,8 @@ __global__ void __launch_bounds__(128) walk_kernel(const __grid_constant__ Walks
   const int e0 = blockIdx.y * 64;
   if (e0 >= w.Dv) return;
   const int ne = min(64, w.Dv - e0);
-  const float delta = w.decay[w.n_decay > 1 ? head % w.n_decay : 0] * (1.0f / 4096.0f);
-  const float r = __fsub_rn(1.0f, delta), r_lo = __fsub_rn(__fsub_rn(1.0f, r), delta);
+  const Keep keep = keep_of(w.decay[w.n_decay > 1 ? head % w.n_decay : 0]);
+  const float r = keep.r, r_lo = keep.lo;
   const float* q = w.q + head * w.Dk * w.T;
   const float* k = w.k + head * w.Dk * w.T;
   const float* v = w.v + (head * w.Dv + e0) * w.T;
@@ -254,7 +262,7 @@ step_kernel(const float* __restrict__ q, const float* __restrict__ k, const floa
       qd[i] = __ldg(q + head * Dk + d);
     }
   }
-  const float r = 1.0f - decay[n_decay > 1 ? head % n_decay : 0] * (1.0f / 4096.0f);
+  const Keep keep = keep_of(decay[n_decay > 1 ? head % n_decay : 0]);
   float ve[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < 4; ++e) ve[e] = col + e < Dv ? __ldg(v + head * Dv + col + e) : 0.f;
@@ -264,7 +272,7 @@ step_kernel(const float* __restrict__ q, const float* __restrict__ k, const floa
     if (d < Dk && col < Dv) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[i][e] = fmaf(r, x[i][e], kd[i] * ve[e]);
+        x[i][e] = fmaf(keep.r, x[i][e], fmaf(keep.lo, x[i][e], kd[i] * ve[e]));
         acc[e] = fmaf(qd[i], x[i][e], acc[e]);
       }
       if (VEC) {

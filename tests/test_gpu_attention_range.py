@@ -201,3 +201,29 @@ def test_tiny_steps_before_a_large_one(cuda, dk, dv, query, tiny):
     q, k, v = np.full(shape, query, np.float32), np.full(shape, tiny, np.float32), np.full((1, 1, dv, 256), tiny, np.float32)
     k[..., 64:128] = v[..., 64:128] = 1.0
     check_forward(q, k, v, np.array([2.048], np.float32))
+
+
+def test_single_steps_of_a_slow_head(cuda):
+    """Thousands of steps on a kept state decay by r itself, not by r rounded to a float.
+
+    A step rounds an element once, by a relative error of -2^-24 .. 2^-24 (its deviation at most 2^-24 / sqrt 3),
+    one step's independent of the next one's as the mantissas are.  Elements are not independent: a step takes a
+    mantissa of 2^23 .. 2^24 units down by 2^23 (1 - r) units or more, so that is the least number of different
+    courses that mantissas can take (204 for a decay of 0.1), and elements on one course go on alike.  The mean over
+    C = 2^23 (1 - r) courses after N steps deviates by 2^-24 sqrt(N / 3 C); six of those are allowed.  r rounded to
+    a float moves every element by N times what the rounding loses, the same way."""
+    steps, width = 4000, 64
+    decay = np.array([0.05, 0.1, 0.3], np.float32)
+    r = 1.0 - decay.astype(np.float64) / 4096.0
+    lost = np.abs(r - r.astype(np.float32))
+    courses = 2.0 ** 23 * (1.0 - r)
+    assert (courses < width ** 2).all()
+    tol = 6 * 2.0 ** -24 * np.sqrt(steps / 3 / courses)
+    assert (steps * lost > 30 * tol).all()
+    rng = np.random.default_rng(27)
+    start = rng.normal(size=(1, 3, width, width)).astype(np.float32)
+    state, zero, d = dev(start), torch.zeros(1, 3, width, device='cuda'), dev(decay)
+    for _ in range(steps):
+        attention.step(zero, zero, zero, d, state)
+    error = (state.cpu().numpy() / (start.astype(np.float64) * (r ** steps).reshape(1, 3, 1, 1)) - 1.0).mean(axis=(0, 2, 3))
+    assert (np.abs(error) <= tol).all(), error / tol
