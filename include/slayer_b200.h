@@ -409,7 +409,8 @@ int sb_cuba_recurrent_bwd(const float* grad_spike, const float* voltage, const f
  * q, k: [heads, Dk, T]; v, out: [heads, Dv, T]; states: [heads, Dk, Dv]; heads = samples * H, decay
  * float[n_decay] with n_decay 1 or H (head i uses decay[i % H]); 1 <= Dk, Dv <= 128.
  * state (nullable: zero) is S before the first step, final_state (nullable) receives S after the last.
- * `scratch` has sb_linear_attention_scratch_bytes(..., backward) bytes (0: may be null). */
+ * `scratch` has sb_linear_attention_scratch_bytes(..., backward) bytes (0: may be null), asked for with the
+ * device of the launch current: the number goes by its multiprocessors. */
 int64_t sb_linear_attention_scratch_bytes(int64_t heads, int64_t Dk, int64_t Dv, int64_t T, int backward);
 int sb_linear_attention_fwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
                             const float* state, float* out, float* final_state, int64_t heads, int64_t H,

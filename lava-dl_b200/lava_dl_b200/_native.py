@@ -178,6 +178,16 @@ def call(name, device_tensor, *args):
         check(rc, name)
 
 
+def ask(name, device, *args):
+    """Value of an entry point that depends on the device, asked for with ``device`` current (as :func:`call` runs
+    what the value is for)."""
+    fn = getattr(_lib or load(), name)
+    if device.index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(device.index):
+        return fn(*args)
+
+
 def device_status():
     bits = c_uint(0)
     check(load().sb_device_status(ctypes.byref(bits)), 'sb_device_status')

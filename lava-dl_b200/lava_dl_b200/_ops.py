@@ -815,7 +815,8 @@ def _attention_check(q, k, v, decay, state, time):
 
 
 def _attention_scratch(heads, dk, dv, T, backward, device):
-    nbytes = N.load().sb_linear_attention_scratch_bytes(heads, dk, dv, T, int(backward))
+    # (the cut into segments goes by the device's multiprocessors)
+    nbytes = N.ask('sb_linear_attention_scratch_bytes', device, heads, dk, dv, T, int(backward))
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
