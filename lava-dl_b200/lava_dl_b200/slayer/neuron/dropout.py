@@ -35,9 +35,12 @@ def dropout(input, p, key, per_step=False):
 class Dropout(torch.nn.Module):
     """Dropout module for the ``dropout`` argument of the neurons.
 
-    Every call in training mode uses a new mask; outside of it the input passes.  The generator's
-    state ``(seed, offset)`` lives on the device and is moved on there, so replays of a captured
-    training step use new masks as well.
+    Every call in training mode uses a new mask; outside of it the input passes.  Without a ``seed`` the
+    key of a call comes from torch's generator of the input's device: the masks follow
+    ``torch.manual_seed`` and the generator's state (a checkpointed segment that is recomputed repeats
+    its masks, a resumed run goes on with them), and replays of a captured training step use new ones.
+    With a ``seed`` the n-th call takes the key ``(seed, n)``, counted on the device, whatever else draws
+    numbers; a forward that a backward pass recomputes cannot tell which call it repeats, and is refused.
 
     Parameters
     ----------
@@ -46,7 +49,7 @@ class Dropout(torch.nn.Module):
     per_step : bool
         drop single values instead of whole neurons.
     seed : int or None
-        seed of the generator; drawn from torch's default generator when ``None``.
+        seed of a generator of the module's own, whose state is ``generator``, int64 ``(seed, offset)``.
     """
 
     def __init__(self, p=0.5, per_step=False, seed=None):
@@ -55,16 +58,23 @@ class Dropout(torch.nn.Module):
             raise ValueError(f'dropout probability has to be between 0 and 1, but got {p}')
         self.p = float(p)
         self.per_step = per_step
-        if seed is None:
-            seed = int(torch.randint(0, 2 ** 62, (1,)))
-        self.register_buffer('generator', torch.tensor([seed, 0], dtype=torch.int64), persistent=False)
+        self.register_buffer('generator', None if seed is None else torch.tensor([seed, 0], dtype=torch.int64),
+                             persistent=False)
 
     def forward(self, input):
         if not self.training or self.p == 0.0:
             return input
-        if self.generator.device != input.device:
-            self.generator = self.generator.to(input.device)
-        return dropout(input, self.p, _ops.dropout_next(self.generator), self.per_step)
+        return dropout(input, self.p, self._key(input.device), self.per_step)
+
+    def _key(self, device):
+        if self.generator is None:
+            return torch.empty(2, dtype=torch.int64, device=device).random_()
+        if torch._C._current_graph_task_id() != -1:     # inside a backward pass
+            raise RuntimeError('this forward is recomputed by a backward pass, and Dropout with a seed of its own '
+                               'cannot repeat its mask; leave seed=None under activation checkpointing')
+        if self.generator.device != device:
+            self.generator = self.generator.to(device)
+        return _ops.dropout_next(self.generator)
 
     def extra_repr(self):
         return f'p={self.p}, per_step={self.per_step}'
