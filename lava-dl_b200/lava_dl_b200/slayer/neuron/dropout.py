@@ -49,7 +49,8 @@ class Dropout(torch.nn.Module):
     per_step : bool
         drop single values instead of whole neurons.
     seed : int or None
-        seed of a generator of the module's own, whose state is ``generator``, int64 ``(seed, offset)``.
+        seed of a generator of the module's own, whose state is ``generator``, int64 ``(seed, offset)``; no
+        part of ``state_dict()`` and no buffer: ranks that are to drop different neurons take different seeds.
     """
 
     def __init__(self, p=0.5, per_step=False, seed=None):
@@ -58,8 +59,16 @@ class Dropout(torch.nn.Module):
             raise ValueError(f'dropout probability has to be between 0 and 1, but got {p}')
         self.p = float(p)
         self.per_step = per_step
-        self.register_buffer('generator', None if seed is None else torch.tensor([seed, 0], dtype=torch.int64),
-                             persistent=False)
+        # no buffer: DistributedDataParallel would give every rank the first one's at each forward
+        self.generator = None if seed is None else torch.tensor([seed, 0], dtype=torch.int64)
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        if self.generator is not None:
+            device = fn(torch.empty(0, device=self.generator.device)).device
+            if device.type != 'meta':
+                self.generator = self.generator.to(device)
+        return self
 
     def forward(self, input):
         if not self.training or self.p == 0.0:

@@ -1,5 +1,7 @@
 """neuron.Dropout without a GPU: the two device calls are stand-ins that work on CPU tensors."""
 
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -68,3 +70,18 @@ def test_seeded_module_refuses_to_be_recomputed(on_cpu, reentrant):
         y.sum().backward()
     y = checkpoint(drop.eval(), x, use_reentrant=reentrant)     # nothing to repeat
     y.sum().backward()
+
+
+def test_generator_is_no_buffer(on_cpu):
+    """DistributedDataParallel broadcasts buffers from rank 0 before each forward."""
+    for drop in (slayer.neuron.Dropout(0.5), slayer.neuron.Dropout(0.5, seed=3)):
+        assert not list(drop.buffers()) and not drop.state_dict()
+    assert slayer.neuron.Dropout(0.5).generator is None
+    a, b = masks(drop, 2)
+    assert drop.generator.tolist() == [3, 2]
+    drop.half()                                     # moves to a device, never to a type
+    assert drop.generator.dtype == torch.int64 and drop.generator.tolist() == [3, 2]
+    twin = copy.deepcopy(drop)
+    assert torch.equal(masks(drop)[0], masks(twin)[0]) and drop.generator is not twin.generator
+    drop.generator.copy_(torch.tensor([3, 0]))      # a resumed run sets it back
+    assert torch.equal(masks(drop)[0], a) and torch.equal(masks(drop)[0], b)
