@@ -46,6 +46,8 @@ class Dropout(torch.nn.Module):
     ----------
     p : float
         probability of a drop, 0..1.
+    inplace : bool
+        the reference's second argument; ``False`` only.
     per_step : bool
         drop single values instead of whole neurons.
     seed : int or None
@@ -53,8 +55,10 @@ class Dropout(torch.nn.Module):
         part of ``state_dict()`` and no buffer: ranks that are to drop different neurons take different seeds.
     """
 
-    def __init__(self, p=0.5, per_step=False, seed=None):
+    def __init__(self, p=0.5, inplace=False, *, per_step=False, seed=None):
         super().__init__()
+        if inplace:
+            raise ValueError('dropout in place is not supported; the mask is never stored, so nothing is saved by it')
         if not 0.0 <= p <= 1.0:
             raise ValueError(f'dropout probability has to be between 0 and 1, but got {p}')
         self.p = float(p)

@@ -85,3 +85,11 @@ def test_generator_is_no_buffer(on_cpu):
     assert torch.equal(masks(drop)[0], masks(twin)[0]) and drop.generator is not twin.generator
     drop.generator.copy_(torch.tensor([3, 0]))      # a resumed run sets it back
     assert torch.equal(masks(drop)[0], a) and torch.equal(masks(drop)[0], b)
+
+
+def test_arguments():
+    """The reference's second argument is `inplace`."""
+    assert not slayer.neuron.Dropout(0.1, False).per_step
+    with pytest.raises(ValueError, match='in place'):
+        slayer.neuron.Dropout(0.1, True)
+    assert slayer.neuron.Dropout(0.1, per_step=True).per_step
