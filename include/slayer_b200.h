@@ -441,7 +441,8 @@ int sb_qdense_fwd(const float* x, const signed char* w, const float* w_scale, fl
  * int64[2] = {seed, offset}.  The same call on the output gradient is the backward pass. */
 int sb_dropout(const float* x, float* y, const int64_t* key, int64_t rows, int64_t T, double p, int per_step,
                void* stream);
-/* key = state; state[1] += 1 (both device int64[2]): the next call's key, also when replayed in a graph. */
+/* key = state; state[1] += 1 (both device int64[2]): the next call's key, also when replayed in a graph.  Calls on
+ * several streams at once get different keys. */
 int sb_dropout_next(int64_t* state, int64_t* key, void* stream);
 
 #ifdef __cplusplus

@@ -154,11 +154,11 @@ dropout_rows_kernel(const float* __restrict__ x, float* __restrict__ y, const in
   }
 }
 
-// One step of the generator's state: the key of this call is handed out, the offset moves on.
+// One step of the generator's state: the key of this call is handed out, the offset moves on.  Atomic, so that
+// calls on several streams get keys of their own (which gets which is open).
 __global__ void dropout_next_kernel(int64_t* state, int64_t* key) {
   key[0] = state[0];
-  key[1] = state[1];
-  state[1] = (int64_t)((uint64_t)state[1] + 1u);
+  key[1] = (int64_t)atomicAdd(reinterpret_cast<unsigned long long*>(state + 1), 1ull);
 }
 
 }  // namespace

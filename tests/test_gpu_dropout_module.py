@@ -5,6 +5,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import lava_dl_b200.slayer as slayer
+from lava_dl_b200 import _ops
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +72,23 @@ def test_seeded_module_refuses_to_be_recomputed(cuda):
     y = checkpoint(drop, x, use_reentrant=False)
     with pytest.raises(RuntimeError, match='recomputed'):
         y.sum().backward()
+
+
+def test_streams_get_keys_of_their_own(cuda):
+    """Branches of a graph run side by side, whatever time the host takes between launches."""
+    state, streams, keys = torch.tensor([9, 100], device='cuda'), [torch.cuda.Stream() for _ in range(8)], []
+    _ops.dropout_next(state.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for stream in streams:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                keys += [_ops.dropout_next(state) for _ in range(50)]
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        keys = torch.stack(keys)
+    for i in range(5):
+        graph.replay()
+        assert state.tolist() == [9, 100 + 400 * (i + 1)] and bool((keys[:, 0] == 9).all())
+        assert sorted(keys[:, 1].tolist()) == list(range(100 + 400 * i, 500 + 400 * i))
