@@ -11,6 +11,7 @@ from ctypes import c_void_p
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -787,6 +788,19 @@ def _same_device(first, **others):
 def _written(t):
     """Tell autograd that a kernel wrote to ``t``: a graph that saved it must not use the new values."""
     torch.autograd.graph.increment_version(t)
+
+
+def plain_call():
+    """Whether a call that needs no gradient may pass ``autograd.Function`` by, whose host time is that of a launch:
+    not while forward-mode levels are open (it is what refuses a tangent) or a trace records."""
+    return forward_ad._current_level < 0 and torch._C._get_tracing_state() is None
+
+
+def refuse_tangents(what, *tensors):
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f'{what} has no forward-mode derivative')
 
 
 def _attention_check(q, k, v, decay, state, time):

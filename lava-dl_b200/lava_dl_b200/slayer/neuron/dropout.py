@@ -27,7 +27,7 @@ def dropout(input, p, key, per_step=False):
     torch tensor
         shaped like ``input``.
     """
-    if not torch.is_grad_enabled():
+    if not torch.is_grad_enabled() and _ops.plain_call():
         return _ops.dropout(input, p, key, per_step)
     return _Dropout.apply(input, key, p, per_step)
 

@@ -39,9 +39,9 @@ def dynamics(query, key, value, decay, state=None, return_state=False):
     torch tensor or pair of torch tensors
         output, shaped like ``value`` (and the state).
     """
-    if not torch.is_grad_enabled():
+    if not torch.is_grad_enabled() and _ops.plain_call():
         output, final = _ops.linear_attention_fwd(query, key, value, decay, state, return_state)
-    elif decay.requires_grad:
+    elif torch.is_grad_enabled() and decay.requires_grad:
         raise RuntimeError('linear attention has no gradient for its decay; pass decay.detach()')
     else:
         output, final = _LinearAttention.apply(query, key, value, decay, state, return_state)
@@ -74,6 +74,11 @@ def step(query, key, value, decay, state):
                                     or decay.requires_grad or (state is not None and state.requires_grad)):
         raise RuntimeError('linear attention steps update their state in place and have no gradient; use dynamics(), '
                            'or call step() under torch.no_grad()')
+    if not _ops.plain_call():
+        _ops.refuse_tangents('a linear attention step', query, key, value, decay, state)
+        if torch._C._get_tracing_state() is not None:
+            raise RuntimeError('a linear attention step cannot be traced: traces do not see that its state changes; '
+                               'capture it in a CUDA graph')
     return _ops.linear_attention_step(query, key, value, decay, state)
 
 

@@ -79,14 +79,26 @@ class QuantDense(torch.nn.Module):
         if torch.is_grad_enabled() and input.requires_grad:
             raise RuntimeError('QuantDense is an inference synapse: its rounding has no gradient')
         if input.dim() == 3:
-            return _ops.qdense_fwd(input, self.weight_q, self.weight_scale, self.in_neurons)
+            return self._product(input)
         if input.dim() != 5 or tuple(input.shape[1:4]) != self.in_shape:
             raise ValueError(f'expected input of shape [batch, {self.in_neurons}, time] or '
                              f'[batch, {", ".join(map(str, self.in_shape))}, time], found {tuple(input.shape)}')
         n, t = input.shape[0], input.shape[-1]
-        flat = _ops.qdense_fwd(input.reshape(n, self.in_neurons, t), self.weight_q, self.weight_scale,
-                               self.in_neurons)
-        return flat.reshape(n, self.out_neurons, 1, 1, t)
+        return self._product(input.reshape(n, self.in_neurons, t)).reshape(n, self.out_neurons, 1, 1, t)
+
+    def _product(self, input):
+        if _ops.plain_call():
+            return _ops.qdense_fwd(input, self.weight_q, self.weight_scale, self.in_neurons)
+        _ops.refuse_tangents('QuantDense', input)
+        return _Product.apply(input, self.weight_q, self.weight_scale, self.in_neurons)
 
     def extra_repr(self):
         return f'{self.in_neurons}, {self.out_neurons}'
+
+
+class _Product(torch.autograd.Function):
+    """For traces, which record a Function as a call."""
+
+    @staticmethod
+    def forward(ctx, input, weight, weight_scale, in_neurons):
+        return _ops.qdense_fwd(input, weight, weight_scale, in_neurons)
