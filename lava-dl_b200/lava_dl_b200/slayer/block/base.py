@@ -190,23 +190,22 @@ class AbstractDense(_Block):
 
 
     def quantize(self):
-        """Replace the synapse by its 8-bit inference form (``synapse.QuantDense``), mask included;
-        weights on the neuron's grid are kept exactly.  Returns the block."""
-        if self.mask is not None:
-            self.synapse.weight.data *= self.mask
-            self.mask = None
-        self.synapse = _quantized(self.synapse, self.neuron)
+        """Replace the synapse by its 8-bit inference form (``synapse.QuantDense``), mask included (also
+        under weight normalisation, where the float block's own mask has no effect: its forward computes the
+        weight anew); weights on the neuron's grid are kept exactly.  Returns the block."""
+        self.synapse = _quantized(self.synapse, self.neuron, self.mask)
+        self.mask = None
         return self
 
 
-def _quantized(dense, neuron):
+def _quantized(dense, neuron, mask=None):
     """The 8-bit form of a dense synapse, on the neuron's weight grid when that is its pre-hook."""
     if isinstance(dense, QuantDense):
         return dense
     if dense.complex:
         raise NotImplementedError('complex synapses have no 8-bit form')
     on_grid = dense.pre_hook_fx == neuron.quantize_8bit
-    return QuantDense.from_dense(dense, 2 / neuron.w_scale if on_grid else None)
+    return QuantDense.from_dense(dense, 2 / neuron.w_scale if on_grid else None, mask)
 
 
 class AbstractAttention(_Block):

@@ -44,7 +44,7 @@ class QuantDense(torch.nn.Module):
         self.register_buffer('weight_scale', scale.expand(out_neurons).contiguous())
 
     @classmethod
-    def from_dense(cls, dense, step=None):
+    def from_dense(cls, dense, step=None, mask=None):
         """From a ``synapse.Dense``, its pre-hook applied.
 
         Parameters
@@ -53,11 +53,18 @@ class QuantDense(torch.nn.Module):
         step : float or None
             grid of the weights (``2 / w_scale`` of the neuron whose ``quantize_8bit`` is the pre-hook):
             kept exactly.  ``None`` rounds every output neuron's weights to 1/127 of their largest.
+        mask : tensor or None
+            multiplied onto the weights before the pre-hook.
         """
         with torch.no_grad():
             if dense.weight_norm_enabled:
-                dense.weight = torch._weight_norm(dense.weight_v, dense.weight_g, 0)
-            weight = dense._hooked_weight().detach()
+                weight = torch._weight_norm(dense.weight_v, dense.weight_g, 0)
+            else:
+                weight = dense.weight.detach()
+            if mask is not None:
+                weight = weight * mask
+            if dense.pre_hook_fx is not None:
+                weight = dense.pre_hook_fx(weight)
             in_shape = tuple(weight.shape[1:4])
             weight = weight.reshape(weight.shape[0], -1).float()
             if step is None:
