@@ -420,6 +420,15 @@ int sb_linear_attention_bwd(const float* q, const float* k, const float* v, cons
                             const float* state, const float* grad_out, const float* grad_final, float* grad_q,
                             float* grad_k, float* grad_v, float* grad_state, int64_t heads, int64_t H, int64_t Dk,
                             int64_t Dv, int64_t T, void* scratch, void* stream);
+/* The same step by step in fp32 throughout, at any length: no pairs of 16-bit numbers, no scratch, several times
+ * the time of a long sequence. */
+int sb_linear_attention_fwd_fp32(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                                 const float* state, float* out, float* final_state, int64_t heads, int64_t H,
+                                 int64_t Dk, int64_t Dv, int64_t T, void* stream);
+int sb_linear_attention_bwd_fp32(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                                 const float* state, const float* grad_out, const float* grad_final, float* grad_q,
+                                 float* grad_k, float* grad_v, float* grad_state, int64_t heads, int64_t H, int64_t Dk,
+                                 int64_t Dv, int64_t T, void* stream);
 /* One step: q, k [heads, Dk], v, out [heads, Dv]; state [heads, Dk, Dv] is updated in place. */
 int sb_linear_attention_step(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
                              float* state, float* out, int64_t heads, int64_t H, int64_t Dk, int64_t Dv,

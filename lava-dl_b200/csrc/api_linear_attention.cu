@@ -197,8 +197,8 @@ int by_width(const Walk* in, int n, Walk* out) {
   return narrow;
 }
 
-int run_walks(const Walk* walks, int n, void* scratch, cudaStream_t s) {
-  if (walks_by_steps(walks, n)) return launch_walks(walks, n, s);
+int run_walks(const Walk* walks, int n, bool fp32, void* scratch, cudaStream_t s) {
+  if (fp32 || walks_by_steps(walks, n)) return launch_walks(walks, n, s);
   Walk w[3];
   const int narrow = by_width(walks, n, w);
   float* f = static_cast<float*>(scratch);
@@ -318,6 +318,30 @@ int check_shape(int64_t heads, int64_t H, int64_t n_decay, int64_t Dk, int64_t D
   return SB_OK;
 }
 
+int forward(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay, const float* state,
+            float* out, float* final_state, int64_t heads, int64_t H, int64_t Dk, int64_t Dv, int64_t T, bool fp32,
+            void* scratch, void* stream) {
+  SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
+  if (heads == 0) return SB_OK;
+  SB_REQUIRE(decay && (T == 0 || (q && k && v && out)), "null tensor pointer");
+  const Walk w{q, k, v, out, decay, state, final_state, (int)n_decay, heads, (int)Dk, (int)Dv, T, Dv, 1, 0, 1};
+  return run_walks(&w, 1, fp32, scratch, (cudaStream_t)stream);
+}
+
+int backward(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay, const float* state,
+             const float* grad_out, const float* grad_final, float* grad_q, float* grad_k, float* grad_v,
+             float* grad_state, int64_t heads, int64_t H, int64_t Dk, int64_t Dv, int64_t T, bool fp32, void* scratch,
+             void* stream) {
+  SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
+  if (heads == 0) return SB_OK;
+  SB_REQUIRE(decay && (T == 0 || (q && k && v && grad_out && grad_q && grad_k && grad_v)), "null tensor pointer");
+  const int nd = (int)n_decay, dk = (int)Dk, dv = (int)Dv;
+  const Walk w[3] = {{grad_out, v, k, grad_q, decay, state, nullptr, nd, heads, dv, dk, T, 1, Dv, 0, 1},
+                     {v, grad_out, q, grad_k, decay, grad_final, nullptr, nd, heads, dv, dk, T, 1, Dv, 1, 0},
+                     {k, q, grad_out, grad_v, decay, grad_final, grad_state, nd, heads, dk, dv, T, Dv, 1, 1, 0}};
+  return run_walks(w, 3, fp32, scratch, (cudaStream_t)stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -336,25 +360,29 @@ int64_t sb_linear_attention_scratch_bytes(int64_t heads, int64_t Dk, int64_t Dv,
 int sb_linear_attention_fwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
                             const float* state, float* out, float* final_state, int64_t heads, int64_t H, int64_t Dk,
                             int64_t Dv, int64_t T, void* scratch, void* stream) {
-  SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
-  if (heads == 0) return SB_OK;
-  SB_REQUIRE(decay && (T == 0 || (q && k && v && out)), "null tensor pointer");
-  const Walk w{q, k, v, out, decay, state, final_state, (int)n_decay, heads, (int)Dk, (int)Dv, T, Dv, 1, 0, 1};
-  return run_walks(&w, 1, scratch, (cudaStream_t)stream);
+  return forward(q, k, v, decay, n_decay, state, out, final_state, heads, H, Dk, Dv, T, false, scratch, stream);
+}
+
+int sb_linear_attention_fwd_fp32(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                                 const float* state, float* out, float* final_state, int64_t heads, int64_t H,
+                                 int64_t Dk, int64_t Dv, int64_t T, void* stream) {
+  return forward(q, k, v, decay, n_decay, state, out, final_state, heads, H, Dk, Dv, T, true, nullptr, stream);
 }
 
 int sb_linear_attention_bwd(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
                             const float* state, const float* grad_out, const float* grad_final, float* grad_q,
                             float* grad_k, float* grad_v, float* grad_state, int64_t heads, int64_t H, int64_t Dk,
                             int64_t Dv, int64_t T, void* scratch, void* stream) {
-  SB_TRY(check_shape(heads, H, n_decay, Dk, Dv, T));
-  if (heads == 0) return SB_OK;
-  SB_REQUIRE(decay && (T == 0 || (q && k && v && grad_out && grad_q && grad_k && grad_v)), "null tensor pointer");
-  const int nd = (int)n_decay, dk = (int)Dk, dv = (int)Dv;
-  const Walk w[3] = {{grad_out, v, k, grad_q, decay, state, nullptr, nd, heads, dv, dk, T, 1, Dv, 0, 1},
-                     {v, grad_out, q, grad_k, decay, grad_final, nullptr, nd, heads, dv, dk, T, 1, Dv, 1, 0},
-                     {k, q, grad_out, grad_v, decay, grad_final, grad_state, nd, heads, dk, dv, T, Dv, 1, 1, 0}};
-  return run_walks(w, 3, scratch, (cudaStream_t)stream);
+  return backward(q, k, v, decay, n_decay, state, grad_out, grad_final, grad_q, grad_k, grad_v, grad_state, heads, H, Dk,
+                  Dv, T, false, scratch, stream);
+}
+
+int sb_linear_attention_bwd_fp32(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,
+                                 const float* state, const float* grad_out, const float* grad_final, float* grad_q,
+                                 float* grad_k, float* grad_v, float* grad_state, int64_t heads, int64_t H, int64_t Dk,
+                                 int64_t Dv, int64_t T, void* stream) {
+  return backward(q, k, v, decay, n_decay, state, grad_out, grad_final, grad_q, grad_k, grad_v, grad_state, heads, H, Dk,
+                  Dv, T, true, nullptr, stream);
 }
 
 int sb_linear_attention_step(const float* q, const float* k, const float* v, const float* decay, int64_t n_decay,

@@ -88,6 +88,8 @@ SIGNATURES = {
     'sb_linear_attention_scratch_bytes': (_I64, [_I64, _I64, _I64, _I64, c_int]),
     'sb_linear_attention_fwd': (c_int, [_P, _P, _P, _P, _I64, _P, _P, _P] + [_I64] * 5 + [_P, _P]),
     'sb_linear_attention_bwd': (c_int, [_P, _P, _P, _P, _I64] + [_P] * 7 + [_I64] * 5 + [_P, _P]),
+    'sb_linear_attention_fwd_fp32': (c_int, [_P, _P, _P, _P, _I64, _P, _P, _P] + [_I64] * 5 + [_P]),
+    'sb_linear_attention_bwd_fp32': (c_int, [_P, _P, _P, _P, _I64] + [_P] * 7 + [_I64] * 5 + [_P]),
     'sb_linear_attention_step': (c_int, [_P, _P, _P, _P, _I64, _P, _P] + [_I64] * 4 + [_P]),
     'sb_qdense_scratch_bytes': (_I64, [_I64, _I64]),
     'sb_qdense_fwd': (c_int, [_P, _P, _P, _P] + [_I64] * 5 + [_P, _P]),

@@ -834,20 +834,28 @@ def _attention_scratch(heads, dk, dv, T, backward, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
-def linear_attention_fwd(q, k, v, decay, state=None, want_final=False):
+def _attention_call(direction, precise, q, heads, h, dk, dv, T, *args):
+    args += (heads, max(h, 1), dk, dv, T)
+    if precise:
+        N.call(f'sb_linear_attention_{direction}_fp32', q, *args, N.stream_of(q))
+    else:
+        scratch = _attention_scratch(heads, dk, dv, T, direction == 'bwd', q.device)
+        N.call(f'sb_linear_attention_{direction}', q, *args, N.ptr(scratch), N.stream_of(q))
+
+
+def linear_attention_fwd(q, k, v, decay, state=None, want_final=False, precise=False):
     n, h, dk, dv = _attention_check(q, k, v, decay, state, True)
     q, k, v, decay = _c(q), _c(k), _c(v), _param(decay, q)
     state = None if state is None else _c(state)
     T = q.shape[-1]
     out = torch.empty_like(v)
     final = torch.empty(n, h, dk, dv, device=q.device, dtype=torch.float32) if want_final else None
-    scratch = _attention_scratch(n * h, dk, dv, T, False, q.device)
-    N.call('sb_linear_attention_fwd', q, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(), N.ptr(state),
-           N.ptr(out), N.ptr(final), n * h, max(h, 1), dk, dv, T, N.ptr(scratch), N.stream_of(q))
+    _attention_call('fwd', precise, q, n * h, h, dk, dv, T, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(),
+                    N.ptr(state), N.ptr(out), N.ptr(final))
     return out, final
 
 
-def linear_attention_bwd(q, k, v, decay, state, grad_out, grad_final, want_grad_state):
+def linear_attention_bwd(q, k, v, decay, state, grad_out, grad_final, want_grad_state, precise=False):
     n, h, dk, dv = _attention_check(q, k, v, decay, state, True)
     q, k, v, decay, grad_out = _c(q), _c(k), _c(v), _param(decay, q), _c(grad_out)
     state = None if state is None else _c(state)
@@ -855,10 +863,8 @@ def linear_attention_bwd(q, k, v, decay, state, grad_out, grad_final, want_grad_
     T = q.shape[-1]
     gq, gk, gv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     gs = torch.empty(n, h, dk, dv, device=q.device, dtype=torch.float32) if want_grad_state else None
-    scratch = _attention_scratch(n * h, dk, dv, T, True, q.device)
-    N.call('sb_linear_attention_bwd', q, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(), N.ptr(state),
-           N.ptr(grad_out), N.ptr(grad_final), N.ptr(gq), N.ptr(gk), N.ptr(gv), N.ptr(gs), n * h, max(h, 1), dk, dv,
-           T, N.ptr(scratch), N.stream_of(q))
+    _attention_call('bwd', precise, q, n * h, h, dk, dv, T, N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(decay), decay.numel(),
+                    N.ptr(state), N.ptr(grad_out), N.ptr(grad_final), N.ptr(gq), N.ptr(gk), N.ptr(gv), N.ptr(gs))
     return gq, gk, gv, gs
 
 

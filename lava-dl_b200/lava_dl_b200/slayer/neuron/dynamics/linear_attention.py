@@ -7,7 +7,7 @@ from torch.autograd.function import once_differentiable
 from .... import _ops
 
 
-def dynamics(query, key, value, decay, state=None, return_state=False):
+def dynamics(query, key, value, decay, state=None, return_state=False, precise=False):
     """Linear attention over whole sequences.
 
     .. math::
@@ -16,8 +16,16 @@ def dynamics(query, key, value, decay, state=None, return_state=False):
         o[t] &= S[t]^\\top q[t]
 
     Differentiable (once) in ``query``, ``key``, ``value`` and ``state``.  ``decay`` is a constant of
-    the head: one that requires a gradient is refused.  An output is exact to about ``2^-21`` of the
-    magnitudes it sums, plus ``2^-28`` of that sum taken over the largest magnitudes of each step.
+    the head: one that requires a gradient is refused.
+
+    An output (gradient, state) is off by less than ``2^-23 (width + 280 + time / 64)`` of the sum of its
+    terms' magnitudes, whatever their sizes, as long as the states fit fp32; ``2^-21`` is usual.  Whole
+    sequences run in chunks whose vectors are held as pairs of 16-bit numbers with one exponent for each
+    step (each row of scores, each column of the state), 22 bits of fp32's 24: an element far below the
+    largest of its step keeps fewer (2^20 below, some 17), which adds up to ``2^-28`` of the same sum over the
+    largest magnitudes of each step's vectors.  ``precise`` walks step by step in fp32 instead, at about
+    0.5 us a step for few heads and many times a chunk's time for many.
+
     Values that are not finite make outputs of their own step and of later steps not finite (a
     value's in its own channel), never earlier ones; they may make any element of the state so.
 
@@ -33,6 +41,8 @@ def dynamics(query, key, value, decay, state=None, return_state=False):
         state before the first step, ``[batch, heads, width, width of the value]``; ``None`` is zero.
     return_state : bool
         also return the state after the last step.
+    precise : bool
+        fp32 throughout, forward and backward.
 
     Returns
     -------
@@ -40,11 +50,11 @@ def dynamics(query, key, value, decay, state=None, return_state=False):
         output, shaped like ``value`` (and the state).
     """
     if not torch.is_grad_enabled() and _ops.plain_call():
-        output, final = _ops.linear_attention_fwd(query, key, value, decay, state, return_state)
+        output, final = _ops.linear_attention_fwd(query, key, value, decay, state, return_state, precise)
     elif torch.is_grad_enabled() and decay.requires_grad:
         raise RuntimeError('linear attention has no gradient for its decay; pass decay.detach()')
     else:
-        output, final = _LinearAttention.apply(query, key, value, decay, state, return_state)
+        output, final = _LinearAttention.apply(query, key, value, decay, state, return_state, precise)
     return (output, final) if return_state else output
 
 
@@ -84,9 +94,10 @@ def step(query, key, value, decay, state):
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, decay, state, return_state):
+    def forward(ctx, query, key, value, decay, state, return_state, precise):
         ctx.set_materialize_grads(False)
-        output, final = _ops.linear_attention_fwd(query, key, value, decay, state, return_state)
+        ctx.precise = precise
+        output, final = _ops.linear_attention_fwd(query, key, value, decay, state, return_state, precise)
         ctx.save_for_backward(query, key, value, decay, state)
         return output, final
 
@@ -95,9 +106,9 @@ class _LinearAttention(torch.autograd.Function):
     def backward(ctx, grad_output, grad_final):
         query, key, value, decay, state = ctx.saved_tensors
         if grad_output is None and grad_final is None:
-            return None, None, None, None, None, None
+            return None, None, None, None, None, None, None
         if grad_output is None:
             grad_output = torch.zeros_like(value)
         grad_q, grad_k, grad_v, grad_s = _ops.linear_attention_bwd(
-            query, key, value, decay, state, grad_output, grad_final, ctx.needs_input_grad[4])
-        return grad_q, grad_k, grad_v, None, grad_s, None
+            query, key, value, decay, state, grad_output, grad_final, ctx.needs_input_grad[4], ctx.precise)
+        return grad_q, grad_k, grad_v, None, grad_s, None, None
