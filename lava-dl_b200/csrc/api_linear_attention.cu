@@ -163,9 +163,11 @@ int launch_walks(const Walk* walks, int n, cudaStream_t s) {
 
 // Whether sequences shorter than a chunk walk step by step, in us.  The chunked kernel takes 1.5 and 9.6 (Dk > 64:
 // 13.2) for every wave of items whatever their length; a launch of walks takes 3 and for each step 0.48 or, with
-// many blocks, 1.3 ns for each of them (twice that for Dk > 64).  Steps against chunks: [1, 8, 64, T] 9.4 and 10.9
-// at T = 16, 17.2 and 11.2 at 32; [64, 16, 64, T] 67 and 70 at T = 48, 90 and 68 at 64; their gradients 71 and 202
-// at T = 16, 199 and 203 at 48; [16, 16, 128, T] 49 and 52 at T = 32.
+// many blocks, 1.3 ns for each of them (twice that for Dk > 64).  Steps against chunks: [1, 8, 64, T] 9.5 and 11.4
+// at T = 16, 17.4 and 11.2 at 32; [64, 16, 64, T] 67 and 72 at T = 48, 90 and 70 at 64; their gradients 72 and 212
+// at T = 16, 199 and 213 at 48; [16, 16, 128, T] 49 and 52 at T = 32, their gradients 150 and 144 (the rule takes
+// steps).  At T = 48 and 1024 heads that is 9 times what the bytes need (7.7): a block has 128 threads, three
+// barriers for eight steps and loads of 32 bytes a row, and a chunk is 128 steps whatever the length.
 bool walks_by_steps(const Walk* w, int n) {
   const int64_t T = w[0].T;
   if (T >= 128) return false;

@@ -17,7 +17,8 @@
 // exponent per step, the state one per column of v, and a row of P one per step i: |q_i . k_j| is at most
 // Dk times the two largest elements, so the largest of 2^(f + g) over j <= i (a running maximum that
 // decays with r) bounds the row without looking at it, and no outlier costs the accuracy of a step that
-// does not read it.  A vector's largest element has 2^13 or more and an fp16 pair steps of 2^-24.
+// does not read it.  All exponents are whole numbers until they meet: the steps of a chunk and the powers of r
+// between them may lie further apart than a float's range.  A vector's largest element has 2^13 or more and an fp16 pair steps of 2^-24.
 //
 // Values that are not finite must not meet a zero of the causal mask in an MMA (0 * NaN): the loader
 // zeroes them and notes from which step on a column of the output is spoilt.
@@ -36,18 +37,22 @@
 // single threads issue the MMAs and the TMA loads and a warp works the items out.  Tensors that TMA cannot
 // describe (T % 4 != 0, unaligned) are loaded by the converting threads themselves.
 //
-// What bounds it is the instruction stream.  A chunk of 128 steps and 64 channels a side (131 KB, 3.0 us of
-// an SM's share of copy bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 to 5.7 us on 148 SMs (15.7 for
-// 128 channels a side, both halves of v), in which a scheduler issues 4,250 instructions, mostly the splitting
-// into fp16 pairs, at 0.31 to 0.38 per cycle, its warps without a fetched instruction 3 cycles of 14.  Steps on
-// the way: one loading warpgroup with two operands in registers 15.3 us, a warpgroup per operand 8.9, the same
-// code for the three 7.7, TMA with raw tiles 7.7, waits that hold the warp in hardware instead of polling 6.4,
-// what describes a head in shared memory instead of registers 5.5,
-// a register split with 96 for the state's warps too 5.3 (128 channels 18.2 before, 15.7 so).
+// What bounds it is the chain of roles, each a single warpgroup that hands a single buffer on: no unit of the SM
+// is near its limit.  A chunk of 128 steps and 64 channels a side (131 KB, 3.0 us of an SM's share of copy
+// bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 us on 148 SMs (16.7 for 128 channels a side, both
+// halves of v).  Of that time the loader of k works 54 %, of v 72 %, of q 51 %, the scores' warps 65 %, the
+// state's 71 % and the thread that issues MMAs 64 %; the rest they wait for one another.  While they work they
+// wait as well, for shared and tensor memory (6.0 of the 14 cycles between a warp's instructions) and for
+// instructions to be fetched (3.2): four warps have little to hide either behind.  Issue slots are 33 % used, the
+// tensor pipe 20 %, DRAM 25 %.  Steps on the way (us a chunk, each as measured then): one loading
+// warpgroup with two operands in registers 15.3, a warpgroup per operand 8.9, the same code for the three 7.7,
+// TMA with raw tiles 7.7, waits that hold the warp in hardware instead of polling 6.4, what describes a head in
+// shared memory instead of registers 5.5, a register split with 96 for the state's warps too 5.3 (128 channels
+// 18.2 before, 15.7 so; 16.7 since exponents meet as whole numbers and powers of r keep theirs).
 //
 // The grid is one CTA per SM, which takes its items (a head, one of the walks, 64 columns of v, a segment of the
 // axis) one after the other; the loaders are a chunk ahead across them, so short sequences do not fill and
-// drain for each head (1024 heads of 128 steps: 91 us with a CTA for each item, 67 so).  With fewer items than SMs
+// drain for each head (1024 heads of 128 steps: 91 us with a CTA for each item, 66 so).  With fewer items than SMs
 // the axis is cut into segments: a first launch takes each segment's growth from zero, a small one joins them,
 // and the walk starts every segment from its own state.
 #include <string.h>
@@ -67,8 +72,9 @@ constexpr int kL = 128;                      // steps per chunk
 constexpr int kTileB = kL * 128;             // bytes of a [128 steps][64 channels] fp16 tile
 constexpr int kThreads = 768;
 // Registers per thread of the six warpgroups: 80 at launch (65536 / 768, in steps of 8), moved to where
-// the vectors live.  The sum may not pass 6 * 80.  148 heads of 2048 steps, us: 99 (64 channels) and 270 (128);
-// with 88 for a loader, 104 for the state and 40 for the MMAs 108; with 88, 112 and 40 293 to 299.
+// the vectors live.  The sum may not pass 6 * 80.  148 heads of 2048 steps, us: 99 (64 channels) and 284 (128);
+// with 88 for a loader, 104 for the state and 40 for the MMAs 124 and 298; with 88, 112 and 40 127 and 300; with 88
+// for the state and 72 for the scores 100 and 289.
 struct Regs {
   static constexpr int load = 96, p = 64, s = 96, mma = 32;
   static_assert(3 * load + p + s + mma <= 480, "more registers than the block was launched with");
@@ -555,8 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             for (int d = 0; d < 32; ++d) x[d] = 0;
           }
         }
-        // the weighted rows first, the growth waits for them (148 heads of 2048 steps: 99 against 101 us, with
-        // 128 channels 298 against 318)
+        // the weighted rows first, the growth waits for them (when it was changed, 148 heads of 2048 steps: 101 to
+        // 99 us, with 128 channels 318 to 298)
         const bool weighted = is_v && pass == 0;
         const float by = weighted ? scale_w : scale;
         const uint64_t sc = pair(by, by);
@@ -1105,8 +1111,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
 // the items one after the other, each 0.8 longer than its chunks, and 1.6 to fill and drain; a cut axis is
 // walked by a first launch too, at half the cost of a chunk, and the join and the launches take 2, and a
 // twentieth for each segment.  Measured, us,
-// whole against cut in four: 16 heads of 128 channels and 8 chunks 69 and 53, 4 chunks 39 and 41; 35 heads of 64
-// and 8 chunks 47 and 41, 70 heads 47 and 63.
+// whole against cut in four: 16 heads of 128 channels and 8 chunks 65 and 47, 4 chunks 36 and 35 (the rule leaves
+// them whole); 35 heads of 64 and 8 chunks 43 and 35, 70 heads 43 and 55.
 struct Cut {
   int nseg;
   double cost;
@@ -1127,9 +1133,9 @@ static Cut plan_segments(int64_t ctas, int64_t chunks) {
 
 // Heads that are walked whole by a launch of their own before the others, whose axis is cut, by the same costs:
 // as many as fill the SMs evenly.  Measured, us, together against apart (and the ratio of the costs): 180 heads of
-// 64 channels and 4096 steps 339 and 285 (0.79), 100 heads of 128 channels and 4096 steps 560 and 514 (0.97), the
-// training step of 32 heads of 128 channels and 4096 steps 808 and 733 (0.86; 687 with today's registers), of 256
-// heads of 64 channels and 2000 steps 716 and 716 (0.96).
+// 64 channels and 4096 steps 343 and 270 (0.79), 100 heads of 128 channels and 4096 steps 553 and 503 (0.97), the
+// training step of 32 heads of 128 channels and 4096 steps 774 and 710 (0.86), of 256 heads of 64 channels and 2000
+// steps 712 and 699 (0.96).
 static int64_t whole_heads(int64_t heads, int64_t nsub, int64_t chunks) {
   const int64_t rounds = heads * nsub / sm_count(), first = rounds * sm_count() / nsub;
   if (rounds == 0 || first == heads) return 0;
