@@ -798,18 +798,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       for (int left = item->nc; left > 0; --left, t0 += kL, ++g) {
         if (FULL && out_g >= 0) write_output(out_n != n);
         // the state after the chunk
-        wait_phase(bar_ds, (uint32_t)g & 1u, dead);
-        tc_fence_after();
-        const Factors mw = p2_wide(mw_s[g & 3]);
         const int steps = min(kL, T - t0);
         const Power carry = power(item->pw[32 + steps], item->kappa * steps);
         const float carried = carry.m * p2(max(-126, min(carry.e, 126)));
-        const uint64_t ma = pair(mw.a, mw.a), mb = pair(mw.b, mw.b), cy = pair(carried, carried);
         if (carry.e < -126) {                    // what of the power is below a float
           const float rest = p2_low(carry.e + 126);
 #pragma unroll
           for (int i = 0; i < NSt; ++i) St[i] *= rest;
         }
+        wait_phase(bar_ds, (uint32_t)g & 1u, dead);
+        tc_fence_after();
+        const Factors mw = p2_wide(mw_s[g & 3]);
+        const uint64_t ma = pair(mw.a, mw.a), mb = pair(mw.b, mw.b), cy = pair(carried, carried);
         // (rows 64-127 of the accumulator repeat rows 0-63)
 #pragma unroll
         for (int b = 0; b < NSt; b += 32) {

@@ -169,6 +169,16 @@ def test_large_states_that_fade(cuda, dk, dv, T):
     O.assert_sum_close(final, ws, ss, head_tol(dk, T), 'state')
 
 
+@pytest.mark.parametrize('n, dk, dv, T', [(50, 16, 20, 260), (41, 24, 70, 131), (33, 70, 40, 128)])
+def test_short_memories_side_by_side(cuda, n, dk, dv, T):
+    """More heads than multiprocessors: each takes slow and fast ones in turn."""
+    (q, k, v, go), decay = far_apart(28, n, 9, dk, dv, T, 'random', 40, FAST + SLOW + [2.048])
+    check_forward(q, k, v, decay)
+    check_backward(q, k, v, go, decay, (0,))
+    (q, k, v, go), decay = far_apart(29, n, 9, dk, dv, T, 'random', 40, FAST + SLOW + [2.048], True)
+    check_backward(q, k, v, go, decay, (1, 2))
+
+
 def test_decay_that_is_not_a_number(cuda):
     """Nothing finite comes out of it, whichever kernel takes the length; other heads do not notice."""
     for T in (20, 300):
