@@ -39,16 +39,16 @@
 //
 // What bounds it is the chain of roles, each a single warpgroup that hands a single buffer on: no unit of the SM
 // is near its limit.  A chunk of 128 steps and 64 channels a side (131 KB, 3.0 us of an SM's share of copy
-// bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 us on 148 SMs (16.7 for 128 channels a side, both
+// bandwidth; 0.65 us of MMA time at the bf16 rate) takes 5.2 us on 148 SMs (17 for 128 channels a side, both
 // halves of v).  Of that time the loader of k works 54 %, of v 72 %, of q 51 %, the scores' warps 65 %, the
 // state's 71 % and the thread that issues MMAs 64 %; the rest they wait for one another.  While they work they
-// wait as well, for shared and tensor memory (6.0 of the 14 cycles between a warp's instructions) and for
+// wait as well, for shared and tensor memory (5.7 of the 14 cycles between a warp's instructions) and for
 // instructions to be fetched (3.2): four warps have little to hide either behind.  Issue slots are 33 % used, the
 // tensor pipe 20 %, DRAM 25 %.  Steps on the way (us a chunk, each as measured then): one loading
 // warpgroup with two operands in registers 15.3, a warpgroup per operand 8.9, the same code for the three 7.7,
 // TMA with raw tiles 7.7, waits that hold the warp in hardware instead of polling 6.4, what describes a head in
 // shared memory instead of registers 5.5, a register split with 96 for the state's warps too 5.3 (128 channels
-// 18.2 before, 15.7 so; 16.7 since exponents meet as whole numbers and powers of r keep theirs).
+// 18.2 before, 15.7 so; 17 since exponents meet as whole numbers and powers of r keep theirs).
 //
 // The grid is one CTA per SM, which takes its items (a head, one of the walks, 64 columns of v, a segment of the
 // axis) one after the other; the loaders are a chunk ahead across them, so short sequences do not fill and
@@ -72,9 +72,9 @@ constexpr int kL = 128;                      // steps per chunk
 constexpr int kTileB = kL * 128;             // bytes of a [128 steps][64 channels] fp16 tile
 constexpr int kThreads = 768;
 // Registers per thread of the six warpgroups: 80 at launch (65536 / 768, in steps of 8), moved to where
-// the vectors live.  The sum may not pass 6 * 80.  148 heads of 2048 steps, us: 99 (64 channels) and 284 (128);
-// with 88 for a loader, 104 for the state and 40 for the MMAs 124 and 298; with 88, 112 and 40 127 and 300; with 88
-// for the state and 72 for the scores 100 and 289.
+// the vectors live.  The sum may not pass 6 * 80.  148 heads of 2048 steps, us: 99 (64 channels) and 277 (128);
+// with 88 for a loader, 104 for the state and 40 for the MMAs 25 and 14 more; with 88, 112 and 40 28 and 16; with 88
+// for the state and 72 for the scores 1 and 5.
 struct Regs {
   static constexpr int load = 96, p = 64, s = 96, mma = 32;
   static_assert(3 * load + p + s + mma <= 480, "more registers than the block was launched with");
@@ -1133,8 +1133,8 @@ static Cut plan_segments(int64_t ctas, int64_t chunks) {
 
 // Heads that are walked whole by a launch of their own before the others, whose axis is cut, by the same costs:
 // as many as fill the SMs evenly.  Measured, us, together against apart (and the ratio of the costs): 180 heads of
-// 64 channels and 4096 steps 343 and 270 (0.79), 100 heads of 128 channels and 4096 steps 553 and 503 (0.97), the
-// training step of 32 heads of 128 channels and 4096 steps 774 and 710 (0.86), of 256 heads of 64 channels and 2000
+// 64 channels and 4096 steps 343 and 268 (0.79), 100 heads of 128 channels and 4096 steps 553 and 495 (0.97), the
+// training step of 32 heads of 128 channels and 4096 steps 774 and 692 (0.86), of 256 heads of 64 channels and 2000
 // steps 712 and 699 (0.96).
 static int64_t whole_heads(int64_t heads, int64_t nsub, int64_t chunks) {
   const int64_t rounds = heads * nsub / sm_count(), first = rounds * sm_count() / nsub;

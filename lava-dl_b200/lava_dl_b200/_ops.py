@@ -790,10 +790,13 @@ def _written(t):
     torch.autograd.graph.increment_version(t)
 
 
+_is_tracing = torch._C._is_tracing
+
+
 def plain_call():
     """Whether a call that needs no gradient may pass ``autograd.Function`` by, whose host time is that of a launch:
     not while forward-mode levels are open (it is what refuses a tangent) or a trace records."""
-    return forward_ad._current_level < 0 and torch._C._get_tracing_state() is None
+    return forward_ad._current_level < 0 and not _is_tracing()
 
 
 def refuse_tangents(what, *tensors):

@@ -86,7 +86,7 @@ def step(query, key, value, decay, state):
                            'or call step() under torch.no_grad()')
     if not _ops.plain_call():
         _ops.refuse_tangents('a linear attention step', query, key, value, decay, state)
-        if torch._C._get_tracing_state() is not None:
+        if torch.jit.is_tracing():
             raise RuntimeError('a linear attention step cannot be traced: traces do not see that its state changes; '
                                'capture it in a CUDA graph')
     return _ops.linear_attention_step(query, key, value, decay, state)
